@@ -53,6 +53,14 @@ class RopeTensor(ctypes.Structure):
     ]
 
 
+class PackedView(ctypes.Structure):
+    """Mirror of ``evg_packed_view``."""
+
+    _fields_ = [("data", c_void_p), ("stride_t", c_int64), ("stride_h", c_int64)]
+
+
+_VIEW = ctypes.POINTER(PackedView)
+
 # name -> (restype, argtypes); every symbol include/evg_b200.h declares.
 SIGNATURES = {
     "evg_abi_version": (c_int, []),
@@ -133,6 +141,20 @@ SIGNATURES = {
         c_int,
         [c_void_p] * 13 + [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_int,
                            c_void_p],
+    ),
+    "evg_packed_plan_bytes": (c_int64, [c_int64, c_int64]),
+    "evg_packed_plan": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
+    "evg_packed_attention_fwd": (
+        c_int,
+        [_VIEW] * 4 + [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
+                       c_int, c_void_p],
+    ),
+    "evg_packed_attention_bwd_workspace_bytes": (c_int64, [c_int64] * 4),
+    "evg_packed_attention_bwd": (
+        c_int,
+        [_VIEW] * 5 + [c_void_p] + [_VIEW] * 3 + [c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                                                  c_int64, c_int64, c_int64, c_float, c_int,
+                                                  c_void_p],
     ),
     "evg_selftest_bounded_wait": (c_int, [c_int64, c_void_p, c_void_p]),
     "evg_swiglu_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),

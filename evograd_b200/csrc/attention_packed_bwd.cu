@@ -1,0 +1,652 @@
+// Causal grouped-query attention over a packed batch, backward (sm_100a).
+//
+//   P = exp(scale q k^T - lse), delta_i = do_i . o_i, dS = P * (do v^T - delta),
+//   dv = P^T do, dk = scale dS^T q, dq = scale dS k
+//
+// One pass over the visible tiles, five products per (key tile, query tile). A block
+// owns one key tile of one k/v head and walks the query tiles behind it, for every
+// query head of the group, in chunks of 64 queries:
+//   S^T   = K Q_i^T                 [128 keys x 128 queries], once per tile
+//   dP^T  = V dO^T                  [128 keys x 64 queries]
+//   P^T, dS^T in registers, then 16 bits back into tensor memory over dP^T
+//   dV   += P^T dO,  dK += dS^T Q   (A from tensor memory)
+//   dQ^T  = K^T dS^T                [128 head columns x 64 queries]
+// dK and dV stay in tensor memory until the end (fixed order, no atomics). dQ^T also
+// belongs to other blocks' rows: four warps of their own add it to a float32 copy of
+// dQ (one 128-byte line per warp instruction), so dq can differ in the last bit from
+// run to run; a last kernel scales and rounds the copy.
+//
+// Tensor memory: S^T [0,128), dP^T / P^T / dS^T of the chunk [128,192), dQ^T of the
+// chunk [192,256), dV [256,256+HD), dK [384,384+HD). Shared memory: K, V, two dO and
+// two Q stages, two 16 KB dS^T chunks, row statistics (226 KB at head size 128).
+// At head size 64 the dQ^T product keeps its 128 rows: the A operand's second 64
+// columns are the V tile, which follows K in shared memory, and the rows they give
+// are not read (a 64-row product has another layout in tensor memory).
+//
+// Tiles start at the sequence's first token; rows of K, V, Q and dO behind its end are
+// other tokens and are zeroed in shared memory, and their statistics make P zero.
+//
+// Bound: the dependent chain products -> compute warps -> products through
+// single-buffered tensor memory, and the L2's float32 adders for dQ.
+#include "attention_bwd_parts.cuh"
+#include "packed.cuh"
+
+namespace evg {
+
+__device__ int g_attn_packed_bwd_status = 0;
+
+namespace {
+
+using namespace umma;
+using namespace attn;
+using namespace attn_bwd;
+using namespace packed;
+
+constexpr int kCG = 4;  // column groups of compute warps
+// TMA warp, MMA warp, 16 compute warps, 4 warps that take dQ^T out of tensor memory
+constexpr int kBwdThreads = 64 + 128 * kCG + 128;
+constexpr uint32_t kChunkBytes = 64 * 128 * 2;  // 64 queries x 128 keys of 16-bit dS^T
+constexpr uint32_t kStatBytes = 2048;
+
+template <int HD> __host__ __device__ constexpr uint32_t bwd_tile_region() {
+  return 6 * tile_bytes<HD>() + 2 * kChunkBytes + kStatBytes;
+}
+
+struct BwdParams {
+  const int* plan;
+  float* lse2;    // [Hq][slots * 128] log-sum-exp in log2 units, +inf behind a sequence
+  float* delta;   // [Hq][slots * 128]
+  float* dq_acc;  // [Hq][slots * 128][HD]
+  View dq, dk, dv;
+  int tokens, slots, units, head_group, group, D;
+  float scale;
+  long long wait_limit;
+  uint32_t smem_bytes;
+};
+
+__device__ __forceinline__ void fence_proxy_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void red_add_f32(float* addr, float v) {
+  asm volatile("red.global.add.f32 [%0], %1;" ::"l"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ uint8_t* view_row(const View& v, int64_t token, int head) {
+  return reinterpret_cast<uint8_t*>(v.p) + (token * v.st + (int64_t)head * v.sh) * 2;
+}
+
+// Rows of a [128 x HD] float32 accumulator in tensor memory -> 16-bit rows of a View;
+// the column groups of compute warps take HD / kCG columns each.
+template <int HD, int FMT>
+__device__ __forceinline__ void store_view_rows(uint32_t t_acc, const View& out, int head, int seq0,
+                                                int row0, int L, int D, float scale, const Roles& r) {
+  constexpr int CW = HD / kCG;  // 32 or 16 columns per warp
+  const uint32_t lane_base = (uint32_t)(r.quarter * 32) << 16;
+  const int row = row0 + r.row;
+  const bool ok = row < L;
+  uint8_t* dst = view_row(out, seq0 + (ok ? row : 0), head);
+  const int col = r.half * CW;
+  uint32_t acc[CW];
+  __syncwarp();
+  tmem_ld(t_acc + lane_base + col, acc);
+  tmem_wait_ld();
+  if (!ok) return;
+#pragma unroll
+  for (int v = 0; v < CW / 8; ++v) {
+    if (col + v * 8 < D) {
+      uint4 pk;
+      pk.x = pack2<FMT>(__uint_as_float(acc[8 * v + 0]) * scale, __uint_as_float(acc[8 * v + 1]) * scale);
+      pk.y = pack2<FMT>(__uint_as_float(acc[8 * v + 2]) * scale, __uint_as_float(acc[8 * v + 3]) * scale);
+      pk.z = pack2<FMT>(__uint_as_float(acc[8 * v + 4]) * scale, __uint_as_float(acc[8 * v + 5]) * scale);
+      pk.w = pack2<FMT>(__uint_as_float(acc[8 * v + 6]) * scale, __uint_as_float(acc[8 * v + 7]) * scale);
+      *reinterpret_cast<uint4*>(dst + (col + v * 8) * 2) = pk;
+    }
+  }
+}
+
+template <int HD, int FMT>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
+                       const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v,
+                       const __grid_constant__ CUtensorMap map_do, const BwdParams p) {
+  constexpr int CG = kCG;
+  constexpr int CPW = 64 / CG;  // query columns of a chunk per compute warp (16)
+  // Key tile n - w of a sequence of n tiles: w query tiles to visit, heaviest first.
+  int slot, bh;
+  map_block(blockIdx.x, p.slots, p.units, p.head_group, slot, bh);
+  const int4 item = plan_item(p.plan, slot);
+  if (item.z < 0) return;  // unused slot
+  const int seq0 = item.x, L = item.y;
+  if (item.z == 0) {  // rows behind the last sequence have zero gradients
+    const int vec = p.D / 8;
+    for (int i = threadIdx.x; i < L * vec; i += kBwdThreads) {
+      const int64_t token = seq0 + i / vec;
+      reinterpret_cast<uint4*>(view_row(p.dk, token, bh))[i % vec] = make_uint4(0, 0, 0, 0);
+      reinterpret_cast<uint4*>(view_row(p.dv, token, bh))[i % vec] = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  const int n_it = item.z;
+  const int last_tile = (L - 1) / kTile;
+  const int kvt = last_tile + 1 - n_it;
+  const int tail_rows = L - last_tile * kTile;  // valid rows of the last tile
+  const int kv0 = kvt * kTile;
+  const int n_git = p.group * n_it;  // iteration c = head in group * n_it + it
+  const int64_t P = (int64_t)p.slots * kTile;
+  const int64_t prow0 = (int64_t)(item.w + kvt) * kTile;  // padded row of query tile it = 0
+
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  constexpr uint32_t TB = tile_bytes<HD>();
+  constexpr uint32_t kRegion = bwd_tile_region<HD>();
+  BlockSetup bs = carve(smem_raw, kRegion);
+  if ((uint32_t)(bs.smem - smem_raw) + kRegion + (uint32_t)kControlBytes > p.smem_bytes) {
+    if (threadIdx.x == 0) atomicCAS(&g_attn_packed_bwd_status, 0, 899);
+    return;
+  }
+  uint8_t* sK = bs.smem;
+  uint8_t* sV = sK + TB;  // directly behind K (the dQ^T product of head size 64 reads on)
+  uint8_t* sDO0 = sV + TB;       // 2 stages
+  uint8_t* sQ0 = sDO0 + 2 * TB;  // 2 stages
+  uint8_t* sDS = sQ0 + 2 * TB;   // 2 chunks of dS^T
+  float* s_stat = reinterpret_cast<float*>(sDS + 2 * kChunkBytes);  // [stage][lse2 | delta][128]
+  uint64_t* kv_full = bs.bars + 0;
+  uint64_t* q_full = bs.bars + 1;    // [2]
+  uint64_t* q_empty = bs.bars + 3;   // [2]
+  uint64_t* do_full = bs.bars + 5;   // [2]
+  uint64_t* do_empty = bs.bars + 7;  // [2]
+  uint64_t* s_full = bs.bars + 9;
+  uint64_t* x_free = bs.bars + 10;
+  uint64_t* dp_full = bs.bars + 11;   // [2] by chunk parity
+  uint64_t* pds_full = bs.bars + 13;  // [2] P^T / dS^T of the chunk are in Y
+  uint64_t* ds_full = bs.bars + 15;   // [2] dS^T of the chunk is in shared memory
+  uint64_t* dq_full = bs.bars + 17;   // [2] dQ^T of the chunk is in D
+  uint64_t* d_free = bs.bars + 19;    // [2] D has been read
+  uint64_t* done = bs.bars + 21;
+  const Roles r = roles();  // r.half is the warp's column group, 0 .. CG-1
+  const float scale_log2 = p.scale * kLog2e;
+
+  if (threadIdx.x == 0) {
+    *bs.abort_flag = 0;
+    mbar_init(kv_full, 1); mbar_init(done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1); mbar_init(q_empty + i, 1);
+      mbar_init(do_full + i, 1); mbar_init(do_empty + i, 1);
+      mbar_init(dp_full + i, 1); mbar_init(pds_full + i, 4 * CG);
+      mbar_init(ds_full + i, 4 * CG); mbar_init(dq_full + i, 1); mbar_init(d_free + i, 4);
+    }
+    mbar_init(s_full, 1); mbar_init(x_free, 4 * CG);
+    fence_mbar_init();
+    prefetch_tensormap(&map_q); prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v); prefetch_tensormap(&map_do);
+  }
+  __syncthreads();
+  if (r.warp == 1) { tmem_alloc(bs.tmem_slot, 512); tmem_relinquish(); }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *bs.tmem_slot;
+  const WaitCtx ctx{bs.abort_flag, &g_attn_packed_bwd_status, p.wait_limit};
+  constexpr uint32_t idesc_s = instr_desc_f16(FMT, 128, 128, 0, 0);
+  constexpr uint32_t idesc_p = instr_desc_f16(FMT, 128, 64, 0, 0);
+  constexpr uint32_t idesc_d = instr_desc_f16(FMT, 128, HD, 0, 1);
+  constexpr uint32_t idesc_q = instr_desc_f16(FMT, 128, 64, 1, 1);
+  const uint32_t tX = tmem, tY = tmem + 128, tD = tmem + 192;
+  const uint32_t tDV = tmem + 256, tDK = tmem + 384;
+
+  if (r.is_tma && r.lane == 0) {
+    mbar_expect_tx(kv_full, 2 * TB);
+    load_tile<HD>(sK, &map_k, seq0 + kv0, bh, kv_full);
+    load_tile<HD>(sV, &map_v, seq0 + kv0, bh, kv_full);
+    int it = 0, head = bh * p.group, git = 0;
+    for (; git < n_git; ++git) {
+      const int st = git & 1;
+      const int q0 = seq0 + (kvt + it) * kTile;
+      if (git >= 2) mbar_wait(q_empty + st, ((git >> 1) - 1) & 1, ctx, 821);
+      if (*ctx.abort_flag) break;  // no new copies after a timeout
+      mbar_expect_tx(q_full + st, TB);
+      load_tile<HD>(sQ0 + st * TB, &map_q, q0, head, q_full + st);
+      if (git >= 2) mbar_wait(do_empty + st, ((git >> 1) - 1) & 1, ctx, 831);
+      if (!*ctx.abort_flag) {
+        const int64_t prow = head * P + prow0 + (int64_t)it * kTile;
+        mbar_expect_tx(do_full + st, TB + 1024);
+        load_tile<HD>(sDO0 + st * TB, &map_do, q0, head, do_full + st);
+        bulk_load_1d(s_stat + st * 256, p.lse2 + prow, 512, do_full + st);
+        bulk_load_1d(s_stat + st * 256 + 128, p.delta + prow, 512, do_full + st);
+      }
+      if (++it == n_it) { it = 0; ++head; }
+    }
+    if (*ctx.abort_flag) {
+      // Let the copies still in flight land before the block returns: each of
+      // these waits gives up after the same cycle budget.
+      mbar_drain(kv_full, 0, p.wait_limit);
+      for (int g = git > 2 ? git - 2 : 0; g < git; ++g) {
+        mbar_drain(q_full + (g & 1), (uint32_t)((g >> 1) & 1), p.wait_limit);
+        mbar_drain(do_full + (g & 1), (uint32_t)((g >> 1) & 1), p.wait_limit);
+      }
+    }
+  } else if (r.is_mma) {
+    const bool lead = elect_one();
+    const DescBase v_base = desc_base_kmajor(smem_u32(sV));
+    const DescBase kt_base = desc_base_mnmajor(smem_u32(sK), kTile);
+    // dP^T of query chunk ch: B operand = rows [64 ch, 64 ch + 64) of a dO tile.
+    auto issue_dp = [&](int ch, uint32_t do_saddr) {
+      const DescBase da = desc_base_kmajor(do_saddr + ch * 64 * 128);
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)
+        if (lead)
+          mma_ss(tY, desc_at(v_base, kstep_kmajor(kTile, ks)), desc_at(da, kstep_kmajor(kTile, ks)),
+                 idesc_p, ks > 0 ? 1u : 0u);
+      if (lead) mma_commit(dp_full + ch);
+    };
+    // Query k-step kk of the chunk (16 queries): P^T in Y columns [16 kk, 16 kk + 8),
+    // dS^T in the 8 columns behind it (the layout the compute warps write).
+    auto issue_dv = [&](int ch, uint32_t do_saddr, bool first) {
+      const DescBase dob = desc_base_mnmajor(do_saddr + ch * 64 * 128, kTile);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        if (lead)
+          mma_ts(tDV, tY + kk * CPW, desc_at(dob, kstep_mnmajor(kk)), idesc_d,
+                 (first && kk == 0) ? 0u : 1u);
+    };
+    auto issue_dk = [&](int ch, uint32_t q_saddr, bool first) {
+      const DescBase qb = desc_base_mnmajor(q_saddr + ch * 64 * 128, kTile);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        if (lead)
+          mma_ts(tDK, tY + kk * CPW + CPW / 2, desc_at(qb, kstep_mnmajor(kk)), idesc_d,
+                 (first && kk == 0) ? 0u : 1u);
+    };
+    // dQ^T of chunk ch: A = K^T (the K tile read MN-major), B = dS^T chunk.
+    auto issue_dq = [&](int ch) {
+      const DescBase dsb = desc_base_mnmajor(smem_u32(sDS) + ch * kChunkBytes, kTile);
+#pragma unroll
+      for (int ks = 0; ks < kTile / 16; ++ks)
+        if (lead)
+          mma_ss(tD, desc_at(kt_base, kstep_mnmajor(ks)), desc_at(dsb, kstep_mnmajor(ks)), idesc_q,
+                 ks > 0 ? 1u : 0u);
+      if (lead) mma_commit(dq_full + ch);
+    };
+    // Query iteration `it` reads the sequence's last tile: its rows behind the end are zeroed.
+    auto clear_tail = [&](uint8_t* tile, int it) {
+      if (it == n_it - 1 && tail_rows < kTile) clear_tile_rows<HD>(tile, tail_rows, r.lane);
+    };
+    mbar_wait(kv_full, 0, ctx, 822);
+    if (kvt == last_tile && tail_rows < kTile) {
+      clear_tile_rows<HD>(sK, tail_rows, r.lane);
+      clear_tile_rows<HD>(sV, tail_rows, r.lane);
+    }
+    mbar_wait(q_full + 0, 0, ctx, 823);
+    clear_tail(sQ0, 0);
+    tc_fence_after_sync();
+    issue_scores<HD>(lead, tX, smem_u32(sK), smem_u32(sQ0), idesc_s);
+    if (lead) mma_commit(s_full);
+    mbar_wait(do_full + 0, 0, ctx, 832);
+    clear_tail(sDO0, 0);
+    tc_fence_after_sync();
+    issue_dp(0, smem_u32(sDO0));
+    int it1 = 0;  // query tile of iteration c + 1
+    for (int c = 0; c < n_git; ++c) {
+      const int st = c & 1, st1 = st ^ 1;
+      const uint32_t par = (uint32_t)(c & 1), par1 = (uint32_t)(((c + 1) >> 1) & 1);
+      const bool more = c + 1 < n_git;
+      const uint32_t do_saddr = smem_u32(sDO0 + st * TB), q_saddr = smem_u32(sQ0 + st * TB);
+      if (++it1 == n_it) it1 = 0;
+      // One wait on the critical path per chunk (P^T / dS^T are ready), with the
+      // waits that are normally satisfied long before ahead of it. dQ^T runs one
+      // chunk behind, so its operand and its place in D are ready by the time it is
+      // issued.
+      // chunk 0
+      if (c > 0) {
+        mbar_wait(d_free + 0, par ^ 1u, ctx, 826);
+        mbar_wait(ds_full + 1, par ^ 1u, ctx, 825);
+      }
+      mbar_wait(pds_full + 0, par, ctx, 824);
+      tc_fence_after_sync();
+      issue_dv(0, do_saddr, c == 0);
+      issue_dk(0, q_saddr, c == 0);
+      issue_dp(1, do_saddr);
+      if (c > 0) issue_dq(1);  // of tile c - 1
+      if (more) {
+        mbar_wait(q_full + st1, par1, ctx, 827);
+        clear_tail(sQ0 + st1 * TB, it1);
+        mbar_wait(x_free, par, ctx, 828);
+        tc_fence_after_sync();
+        issue_scores<HD>(lead, tX, smem_u32(sK), smem_u32(sQ0 + st1 * TB), idesc_s);
+        if (lead) mma_commit(s_full);
+      }
+      // chunk 1
+      if (c > 0) mbar_wait(d_free + 1, par ^ 1u, ctx, 835);
+      mbar_wait(ds_full + 0, par, ctx, 834);
+      if (more) {
+        mbar_wait(do_full + st1, par1, ctx, 833);
+        clear_tail(sDO0 + st1 * TB, it1);
+      }
+      mbar_wait(pds_full + 1, par, ctx, 829);
+      tc_fence_after_sync();
+      issue_dv(1, do_saddr, false);
+      if (lead) mma_commit(do_empty + st);
+      issue_dk(1, q_saddr, false);
+      if (lead) mma_commit(q_empty + st);
+      if (more) issue_dp(0, smem_u32(sDO0 + st1 * TB));
+      issue_dq(0);
+      __syncwarp();
+    }
+    {
+      const uint32_t last = (uint32_t)((n_git - 1) & 1);
+      mbar_wait(d_free + 0, last, ctx, 836);
+      mbar_wait(ds_full + 1, last, ctx, 837);
+      tc_fence_after_sync();
+      issue_dq(1);
+    }
+    if (lead) mma_commit(done);
+  } else if (r.warp >= 2 + 4 * CG) {
+    // dQ^T of every chunk: this warp's 32 lanes (head columns) x 64 query columns of D,
+    // one 128-byte line of the float32 dQ copy per warp instruction.
+    const uint32_t lane_base = (uint32_t)(r.quarter * 32) << 16;
+    int it = 0, head = bh * p.group;
+    for (int c = 0; c < n_git; ++c) {
+      const uint32_t par = (uint32_t)(c & 1);
+      const int rows = (it == n_it - 1) ? tail_rows : kTile;  // queries of this tile
+      float* tile_dst = p.dq_acc + (head * P + prow0 + (int64_t)it * kTile) * HD + r.row;
+#pragma unroll
+      for (int ch = 0; ch < 2; ++ch) {
+        mbar_wait(dq_full + ch, par, ctx, 841);
+        __syncwarp();
+        tc_fence_after_sync();
+        uint32_t acc[2][32];
+        tmem_ld(tD + lane_base, acc[0]);
+        tmem_ld(tD + lane_base + 32, acc[1]);
+        tmem_wait_ld();
+        warp_arrive(d_free + ch, r.lane);
+        float* dst = tile_dst + ch * 64 * HD;
+        const int n = rows - ch * 64;
+        if (r.row < p.D) {
+          if (n >= 64) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) red_add_f32(dst + j * HD, __uint_as_float(acc[j >> 5][j & 31]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (j < n) red_add_f32(dst + j * HD, __uint_as_float(acc[j >> 5][j & 31]));
+          }
+        }
+      }
+      if (++it == n_it) { it = 0; ++head; }
+    }
+  } else if (r.is_compute) {
+    const uint32_t lane_base = (uint32_t)(r.quarter * 32) << 16;
+    const int kv_pos = kv0 + r.row;
+    const int col0 = r.half * CPW;  // first query column inside a chunk of this warp
+    f32x2 p2[CPW / 2];  // P^T of the chunk that comes next, two query columns per element
+    uint32_t pp[CPW / 2];
+    const f32x2 neg_scale2 = f2_splat(-scale_log2);
+    // P^T of one chunk from 16 columns of X, two columns per packed instruction:
+    // t = lse2 - s c, p = 2^-t. `diag`: queries before the key are masked. When
+    // `release` is set, X is handed back as soon as its columns are in registers.
+    auto exp_chunk = [&](uint32_t x_col, const float* lse_ptr, bool diag, int q_first, bool release) {
+      uint32_t sr[CPW];
+      tmem_ld(tX + lane_base + x_col, sr);
+      tmem_wait_ld();
+      if (release) warp_arrive(x_free, r.lane);
+      const float4* lse4 = reinterpret_cast<const float4*>(lse_ptr);
+#pragma unroll
+      for (int g = 0; g < CPW / 4; ++g) {
+        const float4 l4 = lse4[g];
+        const f32x2 t01 = f2_fma(f2_make(__uint_as_float(sr[4 * g]), __uint_as_float(sr[4 * g + 1])),
+                                 neg_scale2, f2_make(l4.x, l4.y));
+        const f32x2 t23 = f2_fma(f2_make(__uint_as_float(sr[4 * g + 2]), __uint_as_float(sr[4 * g + 3])),
+                                 neg_scale2, f2_make(l4.z, l4.w));
+        float t[4];
+        f2_split(t01, t[0], t[1]);
+        f2_split(t23, t[2], t[3]);
+        float pe[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pe[e] = fast_exp2(-t[e]);
+        if (diag) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (q_first + 4 * g + e < kv_pos) pe[e] = 0.f;
+        }
+        p2[2 * g] = f2_make(pe[0], pe[1]);
+        p2[2 * g + 1] = f2_make(pe[2], pe[3]);
+        pp[2 * g] = pack2<FMT>(pe[0], pe[1]);
+        pp[2 * g + 1] = pack2<FMT>(pe[2], pe[3]);
+      }
+    };
+    int it = 0;
+    // P^T of the very first chunk
+    mbar_wait(do_full + 0, 0, ctx, 842);
+    mbar_wait(s_full, 0, ctx, 843);
+    __syncwarp();
+    tc_fence_after_sync();
+    exp_chunk(col0, s_stat + col0, true, kv0 + col0, false);
+    for (int c = 0; c < n_git; ++c) {
+      const int st = c & 1;
+      const uint32_t par = (uint32_t)(c & 1);
+      const float* stat = s_stat + st * 256;
+      const int q0 = (kvt + it) * kTile;
+      const int it1 = it + 1 == n_it ? 0 : it + 1;
+#pragma unroll
+      for (int ch = 0; ch < 2; ++ch) {
+        // dS^T of chunk (c, ch): into Y behind P^T, and into shared memory
+        mbar_wait(dp_full + ch, par, ctx, 844);
+        __syncwarp();
+        tc_fence_after_sync();
+        uint32_t dr[CPW];
+        tmem_ld(tY + lane_base + col0, dr);
+        tmem_wait_ld();
+        const float4* del4 = reinterpret_cast<const float4*>(stat + 128 + ch * 64 + col0);
+        uint32_t dd[CPW / 2];
+        const f32x2 minus_one2 = f2_splat(-1.0f);
+#pragma unroll
+        for (int g = 0; g < CPW / 4; ++g) {
+          const float4 d4 = del4[g];
+          // dS = P (dP - delta), two columns at a time; rounded to 16 bits as an operand
+          const f32x2 a01 = f2_fma(f2_make(d4.x, d4.y), minus_one2,
+                                   f2_make(__uint_as_float(dr[4 * g]), __uint_as_float(dr[4 * g + 1])));
+          const f32x2 a23 = f2_fma(f2_make(d4.z, d4.w), minus_one2,
+                                   f2_make(__uint_as_float(dr[4 * g + 2]), __uint_as_float(dr[4 * g + 3])));
+          float d[4];
+          f2_split(f2_mul(p2[2 * g], a01), d[0], d[1]);
+          f2_split(f2_mul(p2[2 * g + 1], a23), d[2], d[3]);
+          dd[2 * g] = pack2<FMT>(d[0], d[1]);
+          dd[2 * g + 1] = pack2<FMT>(d[2], d[3]);
+        }
+        // P^T / dS^T into Y first: the products that wait for them are the critical path.
+        tmem_st(tY + lane_base + col0, pp);
+        tmem_st(tY + lane_base + col0 + CPW / 2, dd);
+        tmem_wait_st();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (r.lane == 0) mbar_arrive(pds_full + ch);
+        if (c > 0) mbar_wait(dq_full + ch, par ^ 1u, ctx, 848);  // the buffer's last reader is done
+        {
+          // dS^T for the dQ^T product: row r.row (a key) of the chunk's [128 keys x 64
+          // queries] tile, 16-byte pieces 2g and 2g+1 of its 128 bytes, at their
+          // swizzled places.
+          uint8_t* row_ptr = sDS + ch * kChunkBytes + r.row * 128;
+          const int sw = r.row & 7;
+          *reinterpret_cast<uint4*>(row_ptr + (((2 * r.half) ^ sw) << 4)) =
+              make_uint4(dd[0], dd[1], dd[2], dd[3]);
+          *reinterpret_cast<uint4*>(row_ptr + (((2 * r.half + 1) ^ sw) << 4)) =
+              make_uint4(dd[4], dd[5], dd[6], dd[7]);
+        }
+        // P^T of the chunk after this one
+        if (ch == 0) {
+          exp_chunk(64 + col0, stat + 64 + col0, it == 0, q0 + 64 + col0, true);
+        } else if (c + 1 < n_git) {
+          mbar_wait(do_full + (st ^ 1), (uint32_t)(((c + 1) >> 1) & 1), ctx, 845);
+          mbar_wait(s_full, par ^ 1u, ctx, 846);
+          __syncwarp();
+          tc_fence_after_sync();
+          exp_chunk(col0, s_stat + (st ^ 1) * 256 + col0, it1 == 0, (kvt + it1) * kTile + col0, false);
+        }
+        // The tensor pipe reads the shared-memory copy of dS^T a whole chunk later: its
+        // proxy fence waits here, behind the exponentials.
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (r.lane == 0) mbar_arrive(ds_full + ch);
+      }
+      it = it1;
+    }
+    mbar_wait(done, 0, ctx, 847);
+    __syncwarp();
+    tc_fence_after_sync();
+    store_view_rows<HD, FMT>(tDV, p.dv, bh, seq0, kv0, L, p.D, 1.0f, r);
+    store_view_rows<HD, FMT>(tDK, p.dk, bh, seq0, kv0, L, p.D, p.scale, r);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (r.warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// Row statistics of every item's query tile: delta = do . o and the log-sum-exp in log2
+// units, padded rows +inf / 0, and the tile's rows of the float32 dQ copy cleared.
+// A block takes 256 / (HD / 8) rows of one head.
+template <int HD, int FMT>
+__global__ void __launch_bounds__(256)
+packed_prepare_kernel(const View dout, const View o, const float* __restrict__ lse, const BwdParams p) {
+  constexpr int TPR = HD / 8;
+  constexpr int ROWS = 256 / TPR;
+  const int4 item = plan_item(p.plan, blockIdx.x);
+  if (item.z <= 0) return;
+  const int head = blockIdx.y;
+  const int part = threadIdx.x % TPR;
+  const int tile0 = (item.z - 1) * kTile;
+  const int64_t prow0 = (int64_t)head * p.slots * kTile + (int64_t)item.w * kTile + tile0;
+  for (int r = threadIdx.x / TPR + blockIdx.z * ROWS; r < kTile; r += ROWS * gridDim.z) {
+    const bool ok = tile0 + r < item.y;
+    const int64_t token = item.x + tile0 + r;
+    float s = 0.f;
+    if (ok) {
+      if (part * 8 < p.D) {
+        const uint4 a = ld_vec(view_row(dout, token, head) + part * 16);
+        const uint4 b = ld_vec(view_row(o, token, head) + part * 16);
+        float af[8], bf[8];
+        if constexpr (FMT == 1) { unpack<__nv_bfloat16>(a, af); unpack<__nv_bfloat16>(b, bf); }
+        else { unpack<__half>(a, af); unpack<__half>(b, bf); }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += af[i] * bf[i];
+      }
+      uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (prow0 + r) * HD + part * 8);
+      acc[0] = acc[1] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int off = TPR / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if (part == 0) {
+      p.delta[prow0 + r] = ok ? s : 0.f;
+      p.lse2[prow0 + r] = ok ? lse[(int64_t)head * p.tokens + token] * kLog2e : INFINITY;
+    }
+  }
+}
+
+// dq = round(scale * float32 copy), zero behind the last sequence.
+template <int HD, int FMT>
+__global__ void __launch_bounds__(256)
+packed_finish_kernel(const BwdParams p) {
+  constexpr int TPR = HD / 8;
+  constexpr int ROWS = 256 / TPR;
+  const int4 item = plan_item(p.plan, blockIdx.x);
+  if (item.z < 0) return;
+  const int head = blockIdx.y;
+  const int part = threadIdx.x % TPR;
+  if (part * 8 >= p.D) return;
+  const int tile0 = item.z > 0 ? (item.z - 1) * kTile : 0;
+  const int rows = min(kTile, item.y - tile0);
+  const int64_t prow0 = (int64_t)head * p.slots * kTile + (int64_t)item.w * kTile + tile0;
+  for (int r = threadIdx.x / TPR + blockIdx.z * ROWS; r < rows; r += ROWS * gridDim.z) {
+    uint4 pk = make_uint4(0, 0, 0, 0);
+    if (item.z > 0) {
+      const float4* src = reinterpret_cast<const float4*>(p.dq_acc + (prow0 + r) * HD + part * 8);
+      const float4 a = __ldcs(src), b = __ldcs(src + 1);
+      pk.x = pack2<FMT>(a.x * p.scale, a.y * p.scale);
+      pk.y = pack2<FMT>(a.z * p.scale, a.w * p.scale);
+      pk.z = pack2<FMT>(b.x * p.scale, b.y * p.scale);
+      pk.w = pack2<FMT>(b.z * p.scale, b.w * p.scale);
+    }
+    *reinterpret_cast<uint4*>(view_row(p.dq, item.x + tile0 + r, head) + part * 16) = pk;
+  }
+}
+
+int read_packed_bwd_status(int reset) {
+  int code = 0;
+  if (cudaMemcpyFromSymbol(&code, g_attn_packed_bwd_status, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  if (reset && code != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_attn_packed_bwd_status, &zero, sizeof(int));
+  }
+  return code;
+}
+const bool g_packed_bwd_registered = (register_device_status(read_packed_bwd_status), true);
+
+template <int HD, int FMT>
+int launch(const View& dout, const View& q, const View& k, const View& v, const View& o,
+           const float* lse, BwdParams& p, int64_t Hq, int64_t Hkv, cudaStream_t stream) {
+  CUtensorMap mq, mk, mv, mdo;
+  if (!encode_view_map(&mq, q, FMT, p.D, p.tokens, Hq) ||
+      !encode_view_map(&mk, k, FMT, p.D, p.tokens, Hkv) ||
+      !encode_view_map(&mv, v, FMT, p.D, p.tokens, Hkv) ||
+      !encode_view_map(&mdo, dout, FMT, p.D, p.tokens, Hq))
+    return fail(EVG_ELAUNCH, "packed_attention_bwd: cuTensorMapEncodeTiled failed");
+  size_t smem = bwd_tile_region<HD>() + kControlBytes + 1024;
+  const size_t most = (size_t)device_info().max_smem_optin;
+  if (smem > most) smem = most;
+  p.smem_bytes = (uint32_t)smem;
+  auto kern = attn_packed_bwd_kernel<HD, FMT>;
+  if (int rc = reserve_smem(kern, smem)) return rc;
+  // rows of one tile are cut into `parts` blocks while there are few tiles
+  const int64_t tiles = (int64_t)p.slots * Hq;
+  constexpr int kMostParts = kTile / (256 / (HD / 8));
+  const int64_t want = (4 * (int64_t)device_info().sm_count + tiles - 1) / tiles;
+  const int parts = (int)(want < 1 ? 1 : want > kMostParts ? kMostParts : want);
+  const dim3 rows_grid((unsigned)p.slots, (unsigned)Hq, (unsigned)parts);
+  packed_prepare_kernel<HD, FMT><<<rows_grid, 256, 0, stream>>>(dout, o, lse, p);
+  if (int rc = check_launch("packed_attention_bwd statistics")) return rc;
+  kern<<<(unsigned)((int64_t)p.slots * p.units), kBwdThreads, smem, stream>>>(mq, mk, mv, mdo, p);
+  if (int rc = check_launch("packed_attention_bwd")) return rc;
+  packed_finish_kernel<HD, FMT><<<rows_grid, 256, 0, stream>>>(p);
+  return check_launch("packed_attention_bwd dq");
+}
+
+}  // namespace
+
+namespace packed {
+
+int64_t bwd_workspace_bytes(int64_t tokens, int64_t sequences, int64_t Hq, int64_t D) {
+  const int64_t rows = plan_slots(tokens, sequences) * kTile * Hq;
+  return rows * ((D > 64 ? 128 : 64) + 2) * 4;
+}
+
+int launch_bwd(const View& dout, const View& q, const View& k, const View& v, const View& o,
+               const float* lse, const View& dq, const View& dk, const View& dv, void* workspace,
+               const void* plan, int64_t tokens, int64_t sequences, int64_t Hq, int64_t Hkv,
+               int64_t D, float scale, int fmt, cudaStream_t stream) {
+  BwdParams p{};
+  p.plan = (const int*)plan;
+  p.tokens = (int)tokens;
+  p.slots = (int)plan_slots(tokens, sequences);
+  const int64_t rows = (int64_t)p.slots * kTile * Hq;
+  p.lse2 = (float*)workspace;
+  p.delta = p.lse2 + rows;
+  p.dq_acc = p.delta + rows;
+  p.dq = dq;
+  p.dk = dk;
+  p.dv = dv;
+  p.group = (int)(Hq / Hkv);
+  p.units = (int)Hkv;
+  p.D = (int)D;
+  p.head_group = head_group_for((int64_t)p.slots * Hkv, Hkv);
+  p.scale = scale;
+  p.wait_limit = wait_limit_cycles2();
+  if (D > 64)
+    return fmt == 1 ? launch<128, 1>(dout, q, k, v, o, lse, p, Hq, Hkv, stream)
+                    : launch<128, 0>(dout, q, k, v, o, lse, p, Hq, Hkv, stream);
+  return fmt == 1 ? launch<64, 1>(dout, q, k, v, o, lse, p, Hq, Hkv, stream)
+                  : launch<64, 0>(dout, q, k, v, o, lse, p, Hq, Hkv, stream);
+}
+
+}  // namespace packed
+}  // namespace evg

@@ -11,7 +11,7 @@ import math
 import torch
 
 from . import _cabi
-from ._cabi import EVG_BF16, EVG_F16, EVG_F32, RopeTensor, call, lib
+from ._cabi import EVG_BF16, EVG_F16, EVG_F32, EvgError, PackedView, RopeTensor, call, lib
 
 _DTYPES = {torch.float32: EVG_F32, torch.float16: EVG_F16, torch.bfloat16: EVG_BF16}
 
@@ -572,6 +572,156 @@ def causal_gqa_attention_bwd_tm(do_tm, q, k, v_tm, o_tm, lse, scale: float | Non
              v2.data_ptr(), o2.data_ptr(), lse.contiguous().data_ptr(), dq.data_ptr(),
              dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes, B, Hq, Hkv, S, D, float(scale),
              en, _stream(dev))
+    return dq, dk, dv
+
+
+# ------------------------------------------------- packed causal attention
+PACKED_MAX_TOKENS = 1 << 27
+
+
+class PackedPlan:
+    """Work plan of a packed batch, made by :func:`packed_plan` and read by every attention
+    call on that batch (all layers, forward and backward). It lives on the device and
+    follows the offsets it was made from, not their later values."""
+
+    __slots__ = ("data", "tokens", "sequences")
+
+    def __init__(self, data: torch.Tensor, tokens: int, sequences: int):
+        self.data, self.tokens, self.sequences = data, tokens, sequences
+
+    def check(self) -> None:
+        """Synchronise and raise :class:`EvgError` if the offsets were not ``0 = cu[0] <=
+        cu[1] <= ... <= tokens`` (such a plan has no sequences: every row is treated as
+        lying behind the last one)."""
+        status = int(self.data[0].item())
+        if status:
+            raise EvgError("evg_packed_plan", status,
+                           "cu_seqlens must start at 0, never fall and end inside the token axis")
+
+
+def packed_plan(cu_seqlens: torch.Tensor, tokens: int) -> PackedPlan:
+    """Plan for ``n`` sequences packed into ``tokens`` rows: ``cu_seqlens`` is a device tensor
+    of ``n + 1`` int32 (or int64) offsets, sequence ``s`` being rows ``cu[s] .. cu[s+1] - 1``.
+    Lengths may be zero; rows behind ``cu[n]`` belong to no sequence. Nothing is read back:
+    :meth:`PackedPlan.check` validates the offsets for a caller that wants to wait."""
+    dev = _require_cuda(cu_seqlens)
+    if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1:
+        raise ValueError(f"cu_seqlens must be 1-D with at least one entry, got {tuple(cu_seqlens.shape)}")
+    if cu_seqlens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
+    n, tokens = cu_seqlens.numel() - 1, int(tokens)
+    if not 0 <= tokens <= PACKED_MAX_TOKENS or n > PACKED_MAX_TOKENS:
+        raise ValueError(f"{tokens} tokens in {n} sequences: 0 .. {PACKED_MAX_TOKENS} each")
+    if cu_seqlens.dtype == torch.int64:
+        # offsets that int32 cannot hold must stay invalid, not wrap around
+        cu_seqlens = cu_seqlens.clamp(-1, PACKED_MAX_TOKENS + 1).to(torch.int32)
+    cu = cu_seqlens.contiguous()
+    nbytes = lib.evg_packed_plan_bytes(tokens, n)
+    data = torch.empty(nbytes // 4, device=dev, dtype=torch.int32)
+    with torch.cuda.device(dev):
+        call("evg_packed_plan", cu.data_ptr(), n, tokens, data.data_ptr(), nbytes, _stream(dev))
+    return PackedPlan(data, tokens, n)
+
+
+def _check_packed(q, k, v, plan):
+    if not isinstance(plan, PackedPlan):
+        raise TypeError("plan must come from packed_plan()")
+    if q.ndim != 3 or k.ndim != 3:
+        raise ValueError(f"packed attention expects [T, H, D], got {tuple(q.shape)} / {tuple(k.shape)}")
+    _same("k", k, "v", v)
+    if q.dtype != k.dtype:
+        raise ValueError(f"q is {q.dtype} but k is {k.dtype}")
+    T, Hq, D = q.shape
+    if k.shape[0] != T or k.shape[2] != D or k.shape[1] == 0 or Hq == 0 or D == 0 or Hq % k.shape[1]:
+        raise ValueError(f"q {tuple(q.shape)} and k/v {tuple(k.shape)} do not form grouped-query "
+                         "attention (same T, D; query heads a multiple of k/v heads)")
+    if T != plan.tokens:
+        raise ValueError(f"q has {T} rows but the plan was made for {plan.tokens}")
+    if plan.data.device != q.device:
+        raise RuntimeError(f"tensors on different devices: {q.device} and {plan.data.device}")
+    return T, Hq, k.shape[1], D
+
+
+def _packed_in(t):
+    """Input as the kernels take it: last dimension contiguous, no repeated rows or heads,
+    and 16-byte aligned views for 16-bit tensors (a copy otherwise)."""
+    T, H, D = t.shape
+    ok = t.stride(2) == 1 and (T == 1 or t.stride(0) > 0) and (H == 1 or t.stride(1) > 0)
+    if t.element_size() == 2 and D % 8 == 0:
+        ok = ok and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
+    return t if ok else t.contiguous()
+
+
+def _check_out(name, out, like):
+    if not torch.is_tensor(out) or tuple(out.shape) != tuple(like.shape) or out.dtype != like.dtype \
+            or out.device != like.device:
+        raise ValueError(f"{name} must be a tensor of shape {tuple(like.shape)}, {like.dtype} on {like.device}")
+    sizes_strides = sorted((st, n) for n, st in zip(out.shape, out.stride()) if n > 1)
+    reach = 0  # elements the axes so far span; the next stride has to step over them
+    for st, n in sizes_strides:
+        if st <= reach:
+            raise ValueError(f"{name} has overlapping rows (strides {tuple(out.stride())})")
+        reach += st * (n - 1)
+    if out.shape[-1] > 1 and out.stride(-1) != 1:
+        raise ValueError(f"{name} must have a contiguous last dimension")
+    return out
+
+
+def _pv(t):
+    return ctypes.byref(PackedView(t.data_ptr(), t.stride(0), t.stride(1)))
+
+
+def packed_attention_fwd(q, k, v, plan: PackedPlan, scale: float | None = None, out=None):
+    """Causal grouped-query attention over a packed batch: q ``[T, Hq, D]``, k / v
+    ``[T, Hkv, D]`` (strided views such as the thirds of one projection are taken as they
+    are), each token attending to its own sequence's tokens up to itself. Returns
+    ``(o, lse)`` with o like q and ``lse`` float32 ``[Hq, T]``; rows behind the last
+    sequence are 0 and ``-inf``. float16 / bfloat16 with D a multiple of 8 up to 128 run on
+    the tensor cores, float32 and other D <= 256 on plain kernels. ``out`` receives o
+    (it must not overlap an input)."""
+    dev = _require_cuda(q, k, v)
+    T, Hq, Hkv, D = _check_packed(q, k, v, plan)
+    en = _dtype_enum(q)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    o = torch.empty(T, Hq, D, device=dev, dtype=q.dtype) if out is None else _check_out("out", out, q)
+    lse = torch.empty(Hq, T, device=dev, dtype=torch.float32)
+    q2, k2, v2 = _packed_in(q), _packed_in(k), _packed_in(v)
+    with torch.cuda.device(dev):
+        call("evg_packed_attention_fwd", _pv(q2), _pv(k2), _pv(v2), _pv(o), lse.data_ptr(),
+             plan.data.data_ptr(), T, plan.sequences, Hq, Hkv, D, float(scale), en, _stream(dev))
+    return o, lse
+
+
+def packed_attention_bwd(do, q, k, v, o, lse, plan: PackedPlan, scale: float | None = None, outs=None):
+    """Returns ``(dq, dk, dv)`` of :func:`packed_attention_fwd`; dk / dv are summed over the
+    query heads of each group, rows behind the last sequence are zero. ``outs`` supplies the
+    three output tensors, which may be strided views (the thirds of one projection's
+    gradient) but overlap neither an input nor one another. dq of the tensor-core path can
+    differ in the last bit from run to run (float32 global adds)."""
+    dev = _require_cuda(do, q, k, v, o, lse)
+    T, Hq, Hkv, D = _check_packed(q, k, v, plan)
+    _same("do", do, "q", q)
+    _same("o", o, "q", q)
+    en = _dtype_enum(q)
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T):
+        raise ValueError("lse must be float32 [Hq, T]")
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if outs is None:
+        dq, dk, dv = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
+    else:
+        if len(outs) != 3:
+            raise ValueError("outs must hold dq, dk and dv")
+        dq, dk, dv = (_check_out(n, t, like) for n, t, like in zip(("dq", "dk", "dv"), outs, (q, k, v)))
+    do2, q2, k2, v2, o2 = (_packed_in(t) for t in (do, q, k, v, o))
+    lse2 = lse.contiguous()
+    with torch.cuda.device(dev):
+        ws_bytes = lib.evg_packed_attention_bwd_workspace_bytes(T, plan.sequences, Hq, D)
+        ws = torch.empty(max(ws_bytes, 16), device=dev, dtype=torch.uint8)
+        call("evg_packed_attention_bwd", _pv(do2), _pv(q2), _pv(k2), _pv(v2), _pv(o2), lse2.data_ptr(),
+             _pv(dq), _pv(dk), _pv(dv), ws.data_ptr(), ws_bytes, plan.data.data_ptr(), T,
+             plan.sequences, Hq, Hkv, D, float(scale), en, _stream(dev))
     return dq, dk, dv
 
 

@@ -36,8 +36,11 @@ extern "C" {
  * 3: added the evg_exchange_* calls (cross-GPU sum of parameter-gradient
  *    partial sums over peer memory); evoattention head sizes 32 / 64 run on the
  *    tensor cores; attention entry points reject a scale that is not positive
- *    and finite. */
-#define EVG_ABI_VERSION 4
+ *    and finite.
+ * 5: added the operators of a training step over packed sequences (evg_packed_*,
+ *    evg_rope_positions, evg_post_pre_norm_*, evg_clip_grads); every earlier entry
+ *    point is unchanged. */
+#define EVG_ABI_VERSION 5
 
 enum evg_dtype { EVG_F32 = 0, EVG_F16 = 1, EVG_BF16 = 2 };
 
@@ -367,6 +370,70 @@ int evg_evoattention_bwd(const void* dout, const void* q, const void* k,
                          void* workspace, int64_t workspace_bytes, int64_t B,
                          int64_t S, int64_t N, int64_t H, int64_t D, float scale,
                          int dtype, void* stream);
+
+/* ------------------------------------------------- packed causal attention
+ * A packed batch holds `sequences` documents one behind the other in one token
+ * axis of `tokens` entries: sequence s is tokens [cu_seqlens[s],
+ * cu_seqlens[s+1]), cu_seqlens[0] = 0, lengths may be zero, and tokens behind
+ * cu_seqlens[sequences] belong to nobody.
+ *
+ * evg_packed_plan turns the offsets (int32, device) into a work plan in device
+ * memory (evg_packed_plan_bytes(tokens, sequences) bytes, 16-byte aligned) that
+ * every attention call on that batch reads; nothing of it reaches the host, so
+ * it can be captured and replayed with other offsets. Offsets that fall, are
+ * negative or end behind `tokens` make a plan without sequences, and the plan's
+ * first 32-bit word, 0 otherwise, is then EVG_EBADSHAPE.
+ * No counterpart in the reference, whose layers take dense [B, S] batches
+ * (ops/level3/llama3_decoder_layer/forward_ref.py:85-111).
+ */
+#define EVG_PACKED_MAX_TOKENS (1 << 27)
+int64_t evg_packed_plan_bytes(int64_t tokens, int64_t sequences);
+int evg_packed_plan(const int32_t* cu_seqlens, int64_t sequences, int64_t tokens,
+                    void* plan, int64_t plan_bytes, void* stream);
+
+/* A [tokens, heads, D] tensor whose last dimension is contiguous; strides of the
+ * token and head axes in elements. `data` is a device pointer. */
+typedef struct evg_packed_view {
+  void* data;
+  int64_t stride_t, stride_h;
+} evg_packed_view;
+
+/*
+ * o_i = softmax_j(scale q_i . k_j) v_j over the tokens j <= i of i's own
+ * sequence, lse [Hq, tokens] float32 the log-sum-exp (natural log) of the scaled
+ * scores. q, o: Hq heads; k, v: Hkv heads (Hq % Hkv == 0). Rows behind the last
+ * sequence get o = 0 and lse = -inf; what q, k, v hold there reaches nothing, and
+ * neither does one sequence's content (infinities and NaN included) another's.
+ * 16-bit tensors with D a multiple of 8 up to 128 and 16-byte aligned views
+ * (pointers, strides in multiples of 8 elements) run on the tensor cores;
+ * everything else (float32, D <= 256) on plain CUDA-core kernels. Views are HOST
+ * structs, read before the call returns. `plan` must have been made for the same
+ * `tokens` and `sequences`.
+ */
+int evg_packed_attention_fwd(const evg_packed_view* q, const evg_packed_view* k,
+                             const evg_packed_view* v, const evg_packed_view* o,
+                             float* lse, const void* plan, int64_t tokens,
+                             int64_t sequences, int64_t Hq, int64_t Hkv, int64_t D,
+                             float scale, int dtype, void* stream);
+int64_t evg_packed_attention_bwd_workspace_bytes(int64_t tokens, int64_t sequences,
+                                                 int64_t Hq, int64_t D);
+/*
+ * dq, dk, dv of that forward from its o and lse; dk/dv add up the query heads of
+ * a group. Rows behind the last sequence get zero gradients. dk and dv are
+ * bit-reproducible; on the tensor-core path dq is summed with float32 global
+ * adds and can differ in the last bit from run to run. The workspace (16-byte
+ * aligned) holds the row statistics and a float32 copy of dq, padded to whole
+ * 128-row tiles per sequence.
+ */
+int evg_packed_attention_bwd(const evg_packed_view* dout, const evg_packed_view* q,
+                             const evg_packed_view* k, const evg_packed_view* v,
+                             const evg_packed_view* o, const float* lse,
+                             const evg_packed_view* dq, const evg_packed_view* dk,
+                             const evg_packed_view* dv, void* workspace,
+                             int64_t workspace_bytes, const void* plan,
+                             int64_t tokens, int64_t sequences, int64_t Hq,
+                             int64_t Hkv, int64_t D, float scale, int dtype,
+                             void* stream);
 
 /*
  * Synchronises the current device (the one exception to "nothing synchronises")
