@@ -59,6 +59,20 @@ class PackedView(ctypes.Structure):
     _fields_ = [("data", c_void_p), ("stride_t", c_int64), ("stride_h", c_int64)]
 
 
+class RopePositionsTensor(ctypes.Structure):
+    """Mirror of ``evg_rope_positions_tensor``."""
+
+    _fields_ = [
+        ("x", c_void_p),
+        ("y", c_void_p),
+        ("heads", c_int64),
+        ("x_stride_t", c_int64),
+        ("x_stride_h", c_int64),
+        ("y_stride_t", c_int64),
+        ("y_stride_h", c_int64),
+    ]
+
+
 _VIEW = ctypes.POINTER(PackedView)
 
 # name -> (restype, argtypes); every symbol include/evg_b200.h declares.
@@ -155,6 +169,26 @@ SIGNATURES = {
         [_VIEW] * 5 + [c_void_p] + [_VIEW] * 3 + [c_void_p, c_int64, c_void_p, c_int64, c_int64,
                                                   c_int64, c_int64, c_int64, c_float, c_int,
                                                   c_void_p],
+    ),
+    "evg_rope_positions": (
+        c_int,
+        [ctypes.POINTER(RopePositionsTensor), c_int, c_void_p, c_int, c_void_p, c_int, c_int64, c_int64,
+         c_int64, c_int, c_float, c_int, c_int, c_void_p],
+    ),
+    "evg_post_pre_norm_fwd": (
+        c_int,
+        [c_void_p] * 5 + [c_int] + [c_void_p] * 4 + [c_int64, c_int64, c_float, c_float, c_int, c_void_p],
+    ),
+    "evg_post_pre_norm_bwd_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "evg_post_pre_norm_bwd": (
+        c_int,
+        [c_void_p] * 7 + [c_int] + [c_void_p] * 8 + [c_int64, c_int64, c_int64, c_float, c_int, c_void_p],
+    ),
+    "evg_clip_grads_workspace_bytes": (c_int64, [c_int64]),
+    "evg_clip_grads": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_float, c_int, c_void_p, c_void_p, c_int64,
+         c_void_p],
     ),
     "evg_selftest_bounded_wait": (c_int, [c_int64, c_void_p, c_void_p]),
     "evg_swiglu_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p]),

@@ -11,7 +11,8 @@ import math
 import torch
 
 from . import _cabi
-from ._cabi import EVG_BF16, EVG_F16, EVG_F32, EvgError, PackedView, RopeTensor, call, lib
+from ._cabi import EVG_BF16, EVG_F16, EVG_F32, EvgError, PackedView, RopePositionsTensor, RopeTensor, \
+    call, lib
 
 _DTYPES = {torch.float32: EVG_F32, torch.float16: EVG_F16, torch.bfloat16: EVG_BF16}
 
@@ -723,6 +724,253 @@ def packed_attention_bwd(do, q, k, v, o, lse, plan: PackedPlan, scale: float | N
              _pv(dq), _pv(dk), _pv(dv), ws.data_ptr(), ws_bytes, plan.data.data_ptr(), T,
              plan.sequences, Hq, Hkv, D, float(scale), en, _stream(dev))
     return dq, dk, dv
+
+
+# ------------------------------------------- rotary from position numbers
+def rope_inv_freq(rotary_dim: int, base: float = 10000.0, *, scaling: str | None = None,
+                  factor: float = 1.0, original_context: int = 8192, slow: float = 1.0,
+                  fast: float = 4.0, device=None):
+    """Frequencies ``[rotary_dim/2]`` (float64) and the factor on cos / sin for
+    :func:`rope_positions_fwd`: ``(inv_freq, mscale)``. ``scaling`` stretches the context by
+    ``factor``: ``"linear"`` divides every frequency; ``"base"`` raises the base so that the
+    slowest component is divided and the fastest kept; ``"wavelength"`` divides the
+    components that turn less than ``slow`` times over ``original_context`` positions,
+    keeps those above ``fast`` turns and blends linearly in the number of turns between;
+    ``"ramp"`` blends linearly in the component's index between the (rounded) indices
+    that make ``fast`` and ``slow`` turns and sets ``mscale = 0.1 ln(factor) + 1``."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if not base > 1.0 or not factor > 0.0 or original_context < 1 or not 0.0 < slow < fast:
+        raise ValueError("need base > 1, factor > 0, original_context >= 1 and 0 < slow < fast")
+    n = rotary_dim // 2
+    i = torch.arange(n, dtype=torch.float64)
+    mscale = 1.0
+    if scaling == "base":
+        base = base * factor ** (rotary_dim / max(rotary_dim - 2, 1))
+    f = base ** (-2.0 * i / rotary_dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "wavelength":
+        turns = original_context * f / (2.0 * math.pi)
+        keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
+        f = f * (keep + (1.0 - keep) / factor)
+    elif scaling == "ramp":
+        def index_of(turns):
+            return n * math.log(original_context / (turns * 2.0 * math.pi)) / math.log(base)
+
+        lo, hi = max(math.floor(index_of(fast)), 0), min(math.ceil(index_of(slow)), n - 1)
+        keep = 1.0 - ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
+        f = f * (keep + (1.0 - keep) / factor)
+        mscale = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    elif scaling not in (None, "base"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    return f.to(device), mscale
+
+
+def _rope_positions(xs, positions, inv_freq, interleaved, mscale, inverse, outs):
+    xs = [x for x in xs if x is not None]
+    dev = _require_cuda(*xs, positions, inv_freq)
+    x0 = xs[0]
+    for x in xs:
+        if x.ndim != 3 or x.shape[0] != x0.shape[0] or x.shape[2] != x0.shape[2] or x.dtype != x0.dtype:
+            raise ValueError("rope_positions expects [T, H, D] tensors that share T, D and dtype; got "
+                             + ", ".join(f"{tuple(t.shape)} {t.dtype}" for t in xs))
+    T, _, D = x0.shape
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (T,):
+        raise ValueError(f"positions must be int32 or int64 [{T}], got {positions.dtype} "
+                         f"{tuple(positions.shape)}")
+    if inv_freq.dtype not in (torch.float32, torch.float64) or inv_freq.ndim != 1 \
+            or not 0 < 2 * inv_freq.shape[0] <= D:
+        raise ValueError(f"inv_freq must be float32 or float64 with 1 .. {D // 2} entries, got "
+                         f"{inv_freq.dtype} {tuple(inv_freq.shape)}")
+    if outs is not None and len(outs) != len(xs):
+        raise ValueError(f"outs must hold {len(xs)} tensors")
+    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    arr = (RopePositionsTensor * len(xs))()
+    keep, results = [], []
+    for i, x in enumerate(xs):
+        if x.stride(2) != 1:
+            x = x.contiguous()
+        keep.append(x)
+        y = torch.empty(x.shape, device=dev, dtype=x.dtype) if outs is None else _check_out("out", outs[i], x)
+        results.append(y)
+        arr[i] = RopePositionsTensor(x.data_ptr(), y.data_ptr(), x.shape[1], x.stride(0), x.stride(1),
+                                     y.stride(0), y.stride(1))
+    with torch.cuda.device(dev):
+        call("evg_rope_positions", arr, len(xs), positions.data_ptr(), positions.element_size(),
+             inv_freq.data_ptr(), inv_freq.element_size(), T, D, 2 * inv_freq.shape[0],
+             1 if interleaved else 0, float(mscale), _dtype_enum(x0), 1 if inverse else 0, _stream(dev))
+    return tuple(results)
+
+
+def rope_positions_fwd(q, k, positions, inv_freq, *, interleaved: bool = False, mscale: float = 1.0,
+                       outs=None):
+    """Rotate q ``[T, Hq, D]`` and k ``[T, Hk, D]`` (or q alone, with k None) by
+    ``positions[t] * inv_freq[i]`` in one launch. The first ``2 * len(inv_freq)`` columns
+    rotate, in two halves or, ``interleaved``, in neighbouring pairs; the rest is copied.
+    cos and sin are multiplied by ``mscale``. Strided views are taken as they are; ``outs``
+    supplies the results and may be the inputs themselves (in place). Returns a tuple with
+    one tensor per input."""
+    return _rope_positions((q, k), positions, inv_freq, interleaved, mscale, False, outs)
+
+
+def rope_positions_bwd(dq, dk, positions, inv_freq, *, interleaved: bool = False, mscale: float = 1.0,
+                       outs=None):
+    """Gradients of the inputs of :func:`rope_positions_fwd` from those of its outputs."""
+    return _rope_positions((dq, dk), positions, inv_freq, interleaved, mscale, True, outs)
+
+
+# ------------------------------------------- norms after and before a block
+def _gate_kind(gate, x) -> int:
+    if gate is None:
+        return 0
+    if gate.dtype != x.dtype:
+        raise ValueError(f"gate is {gate.dtype} but x is {x.dtype}")
+    shape, want = tuple(gate.shape), tuple(x.shape)
+    if shape == (want[-1],):
+        return 1
+    if shape == want:
+        return 3
+    if shape == want[:-1] + (1,):
+        return 2
+    raise ValueError(f"gate must be [{want[-1]}], {want[:-1] + (1,)} or {want}, got {shape}")
+
+
+def post_pre_norm_fwd(x, residual, post_weight, pre_weight, gate=None, *, alpha: float = 1.0,
+                      eps: float = 1e-6):
+    """A block boundary in one pass: ``h = residual + alpha * gate * rmsnorm(x) * post_weight``,
+    ``y = rmsnorm(h) * pre_weight`` (from h before its rounding). ``gate`` is None, ``[C]``,
+    ``[..., 1]`` or shaped like x. Returns ``(h, y, rstd_post, rstd_pre)``; the rstd are
+    float32 ``[rows]``, saved for the backward with x and h."""
+    dev = _require_cuda(*(t for t in (x, residual, post_weight, pre_weight, gate) if t is not None))
+    _same("x", x, "residual", residual)
+    _check_param("post_weight", post_weight, x)
+    _check_param("pre_weight", pre_weight, x)
+    kind = _gate_kind(gate, x)
+    en = _dtype_enum(x)
+    hidden = x.shape[-1]
+    x2, r2 = _rows_view(x, hidden), _rows_view(residual, hidden)
+    rows = x2.shape[0]
+    h, y = torch.empty_like(x2), torch.empty_like(x2)
+    rstd = torch.empty(2, rows, device=dev, dtype=torch.float32)
+    if rows and hidden:
+        wp, wn = post_weight.contiguous(), pre_weight.contiguous()
+        g = None if gate is None else gate.contiguous()
+        with torch.cuda.device(dev):
+            call("evg_post_pre_norm_fwd", x2.data_ptr(), r2.data_ptr(), wp.data_ptr(), wn.data_ptr(),
+                 _p(g), kind, h.data_ptr(), y.data_ptr(), rstd[0].data_ptr(), rstd[1].data_ptr(), rows,
+                 hidden, float(alpha), float(eps), en, _stream(dev))
+    return h.view(x.shape), y.view(x.shape), rstd[0], rstd[1]
+
+
+def post_pre_norm_bwd(dy, dh, x, h, post_weight, pre_weight, gate, rstd_post, rstd_pre, *,
+                      alpha: float = 1.0):
+    """Gradients of :func:`post_pre_norm_fwd` from those of its y and h (x and its h as saved).
+    Returns ``(dx, dresidual, dpost_weight, dpre_weight, dgate)``; dgate has the gate's
+    shape, None without one. Column sums are float32 and bit-reproducible."""
+    dev = _require_cuda(*(t for t in (dy, dh, x, h, post_weight, pre_weight, gate, rstd_post, rstd_pre)
+                          if t is not None))
+    for name, t in (("dy", dy), ("dh", dh), ("h", h)):
+        _same(name, t, "x", x)
+    _check_param("post_weight", post_weight, x)
+    _check_param("pre_weight", pre_weight, x)
+    kind = _gate_kind(gate, x)
+    en = _dtype_enum(x)
+    hidden = x.shape[-1]
+    dy2, dh2, x2, h2 = (_rows_view(t, hidden) for t in (dy, dh, x, h))
+    rows = x2.shape[0]
+    for name, t in (("rstd_post", rstd_post), ("rstd_pre", rstd_pre)):
+        if t.dtype != torch.float32 or t.numel() != rows:
+            raise ValueError(f"{name} must be float32 with one entry per row")
+    dx, dres = torch.empty_like(x2), torch.empty_like(x2)
+    g = None if gate is None else gate.contiguous()
+    if not rows or not hidden:
+        dgate = None if g is None else torch.zeros_like(g)
+        return (dx.view(x.shape), dres.view(x.shape), torch.zeros_like(post_weight),
+                torch.zeros_like(pre_weight), dgate)
+    wp, wn = post_weight.contiguous(), pre_weight.contiguous()
+    r1, r2 = rstd_post.contiguous(), rstd_pre.contiguous()
+    dwp, dwn = torch.empty_like(wp), torch.empty_like(wn)
+    dgate = None if g is None else torch.empty_like(g)
+    with torch.cuda.device(dev):
+        ws_bytes = lib.evg_post_pre_norm_bwd_workspace_bytes(rows, hidden)
+        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+        call("evg_post_pre_norm_bwd", dy2.data_ptr(), dh2.data_ptr(), x2.data_ptr(), h2.data_ptr(),
+             wp.data_ptr(), wn.data_ptr(), _p(g), kind, r1.data_ptr(), r2.data_ptr(), dx.data_ptr(),
+             dres.data_ptr(), dwp.data_ptr(), dwn.data_ptr(), _p(dgate), ws.data_ptr(), ws_bytes, rows,
+             hidden, float(alpha), en, _stream(dev))
+    return dx.view(x.shape), dres.view(x.shape), dwp, dwn, dgate
+
+
+# ---------------------------------------------- gradient norm and clipping
+def _dense(t) -> bool:
+    """Every element once, no gaps: any order of the dimensions."""
+    if t.is_contiguous():
+        return True
+    reach = 1
+    for st, n in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n != 1):
+        if st != reach:
+            return False
+        reach *= n
+    return True
+
+
+def _grad_list(grads, what):
+    grads = list(grads)
+    if not grads:
+        raise ValueError(f"{what}: no tensors")
+    dev = _require_cuda(*grads)
+    codes = [_dtype_enum(t) for t in grads]
+    for i, t in enumerate(grads):
+        if not _dense(t):
+            raise ValueError(f"{what}: tensor {i} has gaps or repeated elements (strides {tuple(t.stride())})")
+    return grads, dev, codes
+
+
+def _clip_call(grads, dev, codes, outs, max_norm, clip):
+    n = len(grads)
+    norm = torch.empty((), device=dev, dtype=torch.float32)
+    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in grads])
+    optrs = None if outs is None else (ctypes.c_void_p * n)(*[t.data_ptr() for t in outs])
+    numel = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
+    kinds = (ctypes.c_int * n)(*codes)
+    ws_bytes = lib.evg_clip_grads_workspace_bytes(n)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    with torch.cuda.device(dev):
+        call("evg_clip_grads", ptrs, optrs, numel, kinds, n, float(max_norm), 1 if clip else 0,
+             norm.data_ptr(), ws.data_ptr(), ws_bytes, _stream(dev))
+    return norm
+
+
+def grad_norm(grads) -> torch.Tensor:
+    """2-norm over all elements of all tensors (float32 / float16 / bfloat16, mixed), as a
+    float32 scalar on their device."""
+    grads, dev, codes = _grad_list(grads, "grad_norm")
+    return _clip_call(grads, dev, codes, None, 0.0, False)
+
+
+def clip_grad_norm(grads, max_norm: float, outs=None) -> torch.Tensor:
+    """Scale all tensors by ``min(1, max_norm / (norm + 1e-6))`` with ``norm`` their global
+    2-norm, in place or into ``outs`` (same shapes, types and strides; not overlapping the
+    gradients unless it is them). Returns the norm before clipping, a float32 scalar on the
+    device; nothing is read back. A norm that is not finite scales as the formula says
+    (infinite: finite elements to zero; NaN: everything to NaN). The same tensor must not
+    be listed twice."""
+    grads, dev, codes = _grad_list(grads, "clip_grad_norm")
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    if outs is not None:
+        outs = list(outs)
+        if len(outs) != len(grads):
+            raise ValueError(f"{len(outs)} outs for {len(grads)} gradients")
+        _require_cuda(*outs, grads[0])
+        for i, (o, t) in enumerate(zip(outs, grads)):
+            if o.dtype != t.dtype or o.shape != t.shape or (o.stride() != t.stride() and t.numel() > 1):
+                raise ValueError(f"outs[{i}] must have the shape, dtype and strides of its gradient")
+    written = [t.data_ptr() for t in (grads if outs is None else outs) if t.numel()]
+    if len(set(written)) != len(written):
+        raise ValueError("clip_grad_norm: the same tensor is listed twice")
+    return _clip_call(grads, dev, codes, outs, max_norm, True)
 
 
 # ------------------------------------------------------------- evoattention

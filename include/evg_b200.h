@@ -435,6 +435,76 @@ int evg_packed_attention_bwd(const evg_packed_view* dout, const evg_packed_view*
                              int64_t Hkv, int64_t D, float scale, int dtype,
                              void* stream);
 
+/* ---------------------------------------------- rotary from position numbers
+ * Rotates the first rotary_dim columns (even) of [tokens, heads, head_dim]
+ * tensors; row t turns pair i by theta = positions[t] * inv_freq[i]:
+ *   y1 = m (x1 cos - x2 sin),  y2 = m (x2 cos + x1 sin),  m = mscale;
+ * `inverse` != 0 is the backward (the transpose: sine negated, same m). Pairs are
+ * columns (i, i + rotary_dim/2), or (2i, 2i + 1) when `interleaved` != 0; the
+ * columns behind rotary_dim are copied. The angle is formed and reduced in
+ * float64. positions: int32 or int64 (position_bytes 4 / 8), any sign; inv_freq
+ * [rotary_dim/2] float32 or float64 (freq_bytes 4 / 8), both on the device.
+ * Strides in elements, last dimension contiguous; y may be x (same strides).
+ * Where the reference's rope takes ready cos/sin tables, full heads and the half
+ * layout (ops/level1/rope/forward_ref.py:28-47).
+ */
+typedef struct evg_rope_positions_tensor {
+  const void* x;
+  void* y;
+  int64_t heads;
+  int64_t x_stride_t, x_stride_h, y_stride_t, y_stride_h;
+} evg_rope_positions_tensor;
+int evg_rope_positions(const evg_rope_positions_tensor* tensors /* HOST pointer */,
+                       int count, const void* positions, int position_bytes,
+                       const void* inv_freq, int freq_bytes, int64_t tokens,
+                       int64_t head_dim, int64_t rotary_dim, int interleaved,
+                       float mscale, int dtype, int inverse, void* stream);
+
+/* --------------------------------------- norms after and before a block
+ * One pass over a block boundary, [rows, hidden] contiguous: x the block's output,
+ * h the residual stream,
+ *   h_out = h + alpha * gate * (x * rstd_post * w_post)
+ *   y     = h_out * rstd_pre * w_pre           (h_out before its rounding)
+ * with rstd = 1/sqrt(mean square + eps), float32 [rows], saved for the backward.
+ * gate_kind: 0 no gate, 1 [hidden], 2 [rows], 3 [rows, hidden]. Outputs may not
+ * alias inputs. Next to the reference's fused_add_rms_norm
+ * (ops/level2/fused_add_rms_norm/forward_ref.py:6-14), which has one norm, no gate
+ * and does not keep the sum.
+ */
+int evg_post_pre_norm_fwd(const void* x, const void* h, const void* w_post,
+                          const void* w_pre, const void* gate, int gate_kind,
+                          void* h_out, void* y, float* rstd_post, float* rstd_pre,
+                          int64_t rows, int64_t hidden, float alpha, float eps,
+                          int dtype, void* stream);
+int64_t evg_post_pre_norm_bwd_workspace_bytes(int64_t rows, int64_t hidden);
+/*
+ * dy, dh: gradients of y and of h_out; dx, dres: gradients of x and of h; dw_post,
+ * dw_pre [hidden] and dgate (the gate's shape, NULL without one). Column sums are
+ * two-stage, float32, in a fixed order (bit-reproducible). rows must be positive.
+ */
+int evg_post_pre_norm_bwd(const void* dy, const void* dh, const void* x,
+                          const void* h_out, const void* w_post, const void* w_pre,
+                          const void* gate, int gate_kind, const float* rstd_post,
+                          const float* rstd_pre, void* dx, void* dres,
+                          void* dw_post, void* dw_pre, void* dgate, void* workspace,
+                          int64_t workspace_bytes, int64_t rows, int64_t hidden,
+                          float alpha, int dtype, void* stream);
+
+/* ------------------------------------------- global gradient norm, clipping
+ * norm (device float32) = sqrt(sum over `count` tensors of all squares); with
+ * clip != 0 every tensor is multiplied by min(1, max_norm / (norm + 1e-6)), in
+ * place, or into `outs` when that is not NULL. grads, outs, numel, dtypes are HOST
+ * arrays (of device pointers, element counts, evg_dtype), read before the call
+ * returns. Squares and a thread's sums are float32, sums of blocks float64, in a
+ * fixed order: bit-reproducible. A norm that is not finite scales as the formula
+ * says (infinite: to zero, NaN: to NaN). No counterpart in the reference.
+ */
+int64_t evg_clip_grads_workspace_bytes(int64_t count);
+int evg_clip_grads(const void* const* grads, void* const* outs, const int64_t* numel,
+                   const int* dtypes, int64_t count, float max_norm, int clip,
+                   float* norm, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+
 /*
  * Synchronises the current device (the one exception to "nothing synchronises")
  * and reports the sticky device-side status of the kernels that wait on
