@@ -6,6 +6,7 @@ there is no non-CUDA path: a CPU tensor raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -27,21 +28,34 @@ def _dtype_enum(t: torch.Tensor) -> int:
 def _require_cuda(*tensors: torch.Tensor) -> torch.device:
     dev = None
     for t in tensors:
-        if not torch.is_tensor(t):
+        if not isinstance(t, torch.Tensor):
             raise TypeError(f"expected a tensor, got {type(t).__name__}")
-        if not t.is_cuda:
-            raise RuntimeError(
-                "evograd_b200 kernels run on CUDA (sm_100a) tensors only; there is no CPU path"
-            )
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
+        d = t.device
+        if d != dev:
+            if d.type != "cuda":
+                raise RuntimeError(
+                    "evograd_b200 kernels run on CUDA (sm_100a) tensors only; there is no CPU path"
+                )
+            if dev is not None:
+                raise RuntimeError(f"tensors on different devices: {dev} and {d}")
+            dev = d
     return dev
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    # the current stream's handle without the Stream object around it, which costs more host
+    # time than a short kernel runs
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _enqueue(dev: torch.device, fn_name: str, *args) -> None:
+    """``call(fn_name, *args, current stream of dev)`` with ``dev`` the current device."""
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:
+        call(fn_name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            call(fn_name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _p(t) -> int | None:
@@ -49,7 +63,7 @@ def _p(t) -> int | None:
 
 
 def _same(name_a, a, name_b, b, *, shape=True, dtype=True):
-    if shape and tuple(a.shape) != tuple(b.shape):
+    if shape and a.shape != b.shape:
         raise ValueError(f"{name_a} {tuple(a.shape)} and {name_b} {tuple(b.shape)} differ in shape")
     if dtype and a.dtype != b.dtype:
         raise ValueError(f"{name_a} is {a.dtype} but {name_b} is {b.dtype}")
@@ -600,57 +614,72 @@ class PackedPlan:
                            "cu_seqlens must start at 0, never fall and end inside the token axis")
 
 
+@functools.lru_cache(maxsize=1024)
+def _plan_bytes(tokens: int, sequences: int) -> int:
+    return lib.evg_packed_plan_bytes(tokens, sequences)
+
+
 def packed_plan(cu_seqlens: torch.Tensor, tokens: int) -> PackedPlan:
     """Plan for ``n`` sequences packed into ``tokens`` rows: ``cu_seqlens`` is a device tensor
     of ``n + 1`` int32 (or int64) offsets, sequence ``s`` being rows ``cu[s] .. cu[s+1] - 1``.
     Lengths may be zero; rows behind ``cu[n]`` belong to no sequence. Nothing is read back:
     :meth:`PackedPlan.check` validates the offsets for a caller that wants to wait."""
     dev = _require_cuda(cu_seqlens)
-    if cu_seqlens.ndim != 1 or cu_seqlens.numel() < 1:
+    if cu_seqlens.ndim != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError(f"cu_seqlens must be 1-D with at least one entry, got {tuple(cu_seqlens.shape)}")
-    if cu_seqlens.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
-    n, tokens = cu_seqlens.numel() - 1, int(tokens)
+    n, tokens = cu_seqlens.shape[0] - 1, int(tokens)
     if not 0 <= tokens <= PACKED_MAX_TOKENS or n > PACKED_MAX_TOKENS:
         raise ValueError(f"{tokens} tokens in {n} sequences: 0 .. {PACKED_MAX_TOKENS} each")
-    if cu_seqlens.dtype == torch.int64:
+    if cu_seqlens.dtype != torch.int32:
+        if cu_seqlens.dtype != torch.int64:
+            raise TypeError(f"cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
         # offsets that int32 cannot hold must stay invalid, not wrap around
         cu_seqlens = cu_seqlens.clamp(-1, PACKED_MAX_TOKENS + 1).to(torch.int32)
     cu = cu_seqlens.contiguous()
-    nbytes = lib.evg_packed_plan_bytes(tokens, n)
+    nbytes = _plan_bytes(tokens, n)
     data = torch.empty(nbytes // 4, device=dev, dtype=torch.int32)
-    with torch.cuda.device(dev):
-        call("evg_packed_plan", cu.data_ptr(), n, tokens, data.data_ptr(), nbytes, _stream(dev))
+    _enqueue(dev, "evg_packed_plan", cu.data_ptr(), n, tokens, data.data_ptr(), nbytes)
     return PackedPlan(data, tokens, n)
 
 
-def _check_packed(q, k, v, plan):
+def _check_packed(q, k, v, plan, dev):
     if not isinstance(plan, PackedPlan):
         raise TypeError("plan must come from packed_plan()")
-    if q.ndim != 3 or k.ndim != 3:
-        raise ValueError(f"packed attention expects [T, H, D], got {tuple(q.shape)} / {tuple(k.shape)}")
-    _same("k", k, "v", v)
-    if q.dtype != k.dtype:
-        raise ValueError(f"q is {q.dtype} but k is {k.dtype}")
-    T, Hq, D = q.shape
-    if k.shape[0] != T or k.shape[2] != D or k.shape[1] == 0 or Hq == 0 or D == 0 or Hq % k.shape[1]:
-        raise ValueError(f"q {tuple(q.shape)} and k/v {tuple(k.shape)} do not form grouped-query "
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3:
+        raise ValueError(f"packed attention expects [T, H, D], got {tuple(qs)} / {tuple(ks)}")
+    if v.shape != ks or v.dtype != k.dtype or k.dtype != q.dtype:
+        raise ValueError(f"q {q.dtype}, k {tuple(ks)} {k.dtype}, v {tuple(v.shape)} {v.dtype}: k and v must "
+                         "share their shape, all three their dtype")
+    T, Hq, D = qs
+    Hkv = ks[1]
+    if ks[0] != T or ks[2] != D or Hkv == 0 or Hq == 0 or D == 0 or Hq % Hkv:
+        raise ValueError(f"q {tuple(qs)} and k/v {tuple(ks)} do not form grouped-query "
                          "attention (same T, D; query heads a multiple of k/v heads)")
     if T != plan.tokens:
         raise ValueError(f"q has {T} rows but the plan was made for {plan.tokens}")
-    if plan.data.device != q.device:
-        raise RuntimeError(f"tensors on different devices: {q.device} and {plan.data.device}")
-    return T, Hq, k.shape[1], D
+    if plan.data.device != dev:
+        raise RuntimeError(f"tensors on different devices: {dev} and {plan.data.device}")
+    return T, Hq, Hkv, D
 
 
 def _packed_in(t):
-    """Input as the kernels take it: last dimension contiguous, no repeated rows or heads,
-    and 16-byte aligned views for 16-bit tensors (a copy otherwise)."""
+    """An input as the kernels take it: last dimension contiguous, no repeated rows or heads,
+    and 16-byte aligned for 16-bit tensors (a copy otherwise). Returns ``(tensor, view)``."""
     T, H, D = t.shape
-    ok = t.stride(2) == 1 and (T == 1 or t.stride(0) > 0) and (H == 1 or t.stride(1) > 0)
-    if t.element_size() == 2 and D % 8 == 0:
-        ok = ok and t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
-    return t if ok else t.contiguous()
+    st, sh, sd = t.stride()
+    p = t.data_ptr()
+    if sd != 1 or (st <= 0 and T > 1) or (sh <= 0 and H > 1) or (
+            D % 8 == 0 and t.element_size() == 2 and (p | st * 2 | sh * 2) & 15):
+        t = t.contiguous()
+        if t.data_ptr() & 15:  # contiguous already, off a 16-byte boundary
+            t = t.clone()
+        p, st, sh = t.data_ptr(), H * D, D
+    return t, PackedView(p, st, sh)
+
+
+def _packed_out(t):
+    return PackedView(t.data_ptr(), t.stride(0), t.stride(1))
 
 
 def _check_out(name, out, like):
@@ -668,10 +697,6 @@ def _check_out(name, out, like):
     return out
 
 
-def _pv(t):
-    return ctypes.byref(PackedView(t.data_ptr(), t.stride(0), t.stride(1)))
-
-
 def packed_attention_fwd(q, k, v, plan: PackedPlan, scale: float | None = None, out=None):
     """Causal grouped-query attention over a packed batch: q ``[T, Hq, D]``, k / v
     ``[T, Hkv, D]`` (strided views such as the thirds of one projection are taken as they
@@ -681,17 +706,20 @@ def packed_attention_fwd(q, k, v, plan: PackedPlan, scale: float | None = None, 
     the tensor cores, float32 and other D <= 256 on plain kernels. ``out`` receives o
     (it must not overlap an input)."""
     dev = _require_cuda(q, k, v)
-    T, Hq, Hkv, D = _check_packed(q, k, v, plan)
+    T, Hq, Hkv, D = _check_packed(q, k, v, plan, dev)
     en = _dtype_enum(q)
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
     o = torch.empty(T, Hq, D, device=dev, dtype=q.dtype) if out is None else _check_out("out", out, q)
     lse = torch.empty(Hq, T, device=dev, dtype=torch.float32)
-    q2, k2, v2 = _packed_in(q), _packed_in(k), _packed_in(v)
-    with torch.cuda.device(dev):
-        call("evg_packed_attention_fwd", _pv(q2), _pv(k2), _pv(v2), _pv(o), lse.data_ptr(),
-             plan.data.data_ptr(), T, plan.sequences, Hq, Hkv, D, float(scale), en, _stream(dev))
+    (q, vq), (k, vk), (v, vv) = _packed_in(q), _packed_in(k), _packed_in(v)
+    _enqueue(dev, "evg_packed_attention_fwd", vq, vk, vv, _packed_out(o), lse.data_ptr(),
+             plan.data.data_ptr(), T, plan.sequences, Hq, Hkv, D,
+             1.0 / math.sqrt(D) if scale is None else float(scale), en)
     return o, lse
+
+
+@functools.lru_cache(maxsize=1024)
+def _packed_bwd_bytes(tokens: int, sequences: int, heads: int, head_dim: int) -> int:
+    return max(lib.evg_packed_attention_bwd_workspace_bytes(tokens, sequences, heads, head_dim), 16)
 
 
 def packed_attention_bwd(do, q, k, v, o, lse, plan: PackedPlan, scale: float | None = None, outs=None):
@@ -701,28 +729,27 @@ def packed_attention_bwd(do, q, k, v, o, lse, plan: PackedPlan, scale: float | N
     gradient) but overlap neither an input nor one another. dq of the tensor-core path can
     differ in the last bit from run to run (float32 global adds)."""
     dev = _require_cuda(do, q, k, v, o, lse)
-    T, Hq, Hkv, D = _check_packed(q, k, v, plan)
+    T, Hq, Hkv, D = _check_packed(q, k, v, plan, dev)
     _same("do", do, "q", q)
     _same("o", o, "q", q)
     en = _dtype_enum(q)
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (Hq, T):
+    if lse.dtype != torch.float32 or lse.shape != (Hq, T):
         raise ValueError("lse must be float32 [Hq, T]")
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
     if outs is None:
-        dq, dk, dv = (torch.empty(t.shape, device=dev, dtype=t.dtype) for t in (q, k, v))
+        dq = torch.empty(T, Hq, D, device=dev, dtype=q.dtype)
+        dk = torch.empty(T, Hkv, D, device=dev, dtype=q.dtype)
+        dv = torch.empty(T, Hkv, D, device=dev, dtype=q.dtype)
     else:
         if len(outs) != 3:
             raise ValueError("outs must hold dq, dk and dv")
         dq, dk, dv = (_check_out(n, t, like) for n, t, like in zip(("dq", "dk", "dv"), outs, (q, k, v)))
-    do2, q2, k2, v2, o2 = (_packed_in(t) for t in (do, q, k, v, o))
-    lse2 = lse.contiguous()
-    with torch.cuda.device(dev):
-        ws_bytes = lib.evg_packed_attention_bwd_workspace_bytes(T, plan.sequences, Hq, D)
-        ws = torch.empty(max(ws_bytes, 16), device=dev, dtype=torch.uint8)
-        call("evg_packed_attention_bwd", _pv(do2), _pv(q2), _pv(k2), _pv(v2), _pv(o2), lse2.data_ptr(),
-             _pv(dq), _pv(dk), _pv(dv), ws.data_ptr(), ws_bytes, plan.data.data_ptr(), T,
-             plan.sequences, Hq, Hkv, D, float(scale), en, _stream(dev))
+    (do, vdo), (q, vq), (k, vk), (v, vv), (o, vo) = (_packed_in(t) for t in (do, q, k, v, o))
+    lse = lse.contiguous()
+    ws_bytes = _packed_bwd_bytes(T, plan.sequences, Hq, D)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    _enqueue(dev, "evg_packed_attention_bwd", vdo, vq, vk, vv, vo, lse.data_ptr(), _packed_out(dq),
+             _packed_out(dk), _packed_out(dv), ws.data_ptr(), ws_bytes, plan.data.data_ptr(), T,
+             plan.sequences, Hq, Hkv, D, 1.0 / math.sqrt(D) if scale is None else float(scale), en)
     return dq, dk, dv
 
 
@@ -767,6 +794,9 @@ def rope_inv_freq(rotary_dim: int, base: float = 10000.0, *, scaling: str | None
     return f.to(device), mscale
 
 
+_ROPE_ROWS = (None, RopePositionsTensor * 1, RopePositionsTensor * 2)
+
+
 def _rope_positions(xs, positions, inv_freq, interleaved, mscale, inverse, outs):
     xs = [x for x in xs if x is not None]
     dev = _require_cuda(*xs, positions, inv_freq)
@@ -776,30 +806,35 @@ def _rope_positions(xs, positions, inv_freq, interleaved, mscale, inverse, outs)
             raise ValueError("rope_positions expects [T, H, D] tensors that share T, D and dtype; got "
                              + ", ".join(f"{tuple(t.shape)} {t.dtype}" for t in xs))
     T, _, D = x0.shape
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (T,):
-        raise ValueError(f"positions must be int32 or int64 [{T}], got {positions.dtype} "
-                         f"{tuple(positions.shape)}")
-    if inv_freq.dtype not in (torch.float32, torch.float64) or inv_freq.ndim != 1 \
-            or not 0 < 2 * inv_freq.shape[0] <= D:
+    en = _dtype_enum(x0)
+    pdt, fdt, n = positions.dtype, inv_freq.dtype, inv_freq.numel()
+    if (pdt != torch.int32 and pdt != torch.int64) or positions.shape != (T,):
+        raise ValueError(f"positions must be int32 or int64 [{T}], got {pdt} {tuple(positions.shape)}")
+    if (fdt != torch.float64 and fdt != torch.float32) or inv_freq.ndim != 1 or not 0 < 2 * n <= D:
         raise ValueError(f"inv_freq must be float32 or float64 with 1 .. {D // 2} entries, got "
-                         f"{inv_freq.dtype} {tuple(inv_freq.shape)}")
+                         f"{fdt} {tuple(inv_freq.shape)}")
     if outs is not None and len(outs) != len(xs):
         raise ValueError(f"outs must hold {len(xs)} tensors")
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    arr = (RopePositionsTensor * len(xs))()
-    keep, results = [], []
+    rows, keep, results = [], [], []
     for i, x in enumerate(xs):
-        if x.stride(2) != 1:
+        st, sh, sd = x.stride()
+        if sd != 1:
             x = x.contiguous()
+            st, sh, _ = x.stride()
         keep.append(x)
-        y = torch.empty(x.shape, device=dev, dtype=x.dtype) if outs is None else _check_out("out", outs[i], x)
+        if outs is None:
+            H = x.shape[1]
+            y = torch.empty(T, H, D, device=dev, dtype=x.dtype)
+            yst, ysh = H * D, D
+        else:
+            y = _check_out("out", outs[i], x)
+            yst, ysh, _ = y.stride()
         results.append(y)
-        arr[i] = RopePositionsTensor(x.data_ptr(), y.data_ptr(), x.shape[1], x.stride(0), x.stride(1),
-                                     y.stride(0), y.stride(1))
-    with torch.cuda.device(dev):
-        call("evg_rope_positions", arr, len(xs), positions.data_ptr(), positions.element_size(),
-             inv_freq.data_ptr(), inv_freq.element_size(), T, D, 2 * inv_freq.shape[0],
-             1 if interleaved else 0, float(mscale), _dtype_enum(x0), 1 if inverse else 0, _stream(dev))
+        rows.append((x.data_ptr(), y.data_ptr(), x.shape[1], st, sh, yst, ysh))
+    _enqueue(dev, "evg_rope_positions", _ROPE_ROWS[len(rows)](*rows), len(rows), positions.data_ptr(),
+             4 if pdt == torch.int32 else 8, inv_freq.data_ptr(), 8 if fdt == torch.float64 else 4, T, D,
+             2 * n, 1 if interleaved else 0, float(mscale), en, 1 if inverse else 0)
     return tuple(results)
 
 
@@ -836,31 +871,48 @@ def _gate_kind(gate, x) -> int:
     raise ValueError(f"gate must be [{want[-1]}], {want[:-1] + (1,)} or {want}, got {shape}")
 
 
+def _rows2(t, hidden):
+    """``[rows, hidden]`` contiguous, the tensor itself where it is that already."""
+    if t.ndim == 2 and t.is_contiguous():
+        return t
+    return t.contiguous().view(-1, hidden)
+
+
 def post_pre_norm_fwd(x, residual, post_weight, pre_weight, gate=None, *, alpha: float = 1.0,
                       eps: float = 1e-6):
     """A block boundary in one pass: ``h = residual + alpha * gate * rmsnorm(x) * post_weight``,
     ``y = rmsnorm(h) * pre_weight`` (from h before its rounding). ``gate`` is None, ``[C]``,
     ``[..., 1]`` or shaped like x. Returns ``(h, y, rstd_post, rstd_pre)``; the rstd are
     float32 ``[rows]``, saved for the backward with x and h."""
-    dev = _require_cuda(*(t for t in (x, residual, post_weight, pre_weight, gate) if t is not None))
+    given = (x, residual, post_weight, pre_weight)
+    dev = _require_cuda(*given) if gate is None else _require_cuda(*given, gate)
+    shape = x.shape
     _same("x", x, "residual", residual)
     _check_param("post_weight", post_weight, x)
     _check_param("pre_weight", pre_weight, x)
-    kind = _gate_kind(gate, x)
+    kind = 0 if gate is None else _gate_kind(gate, x)
     en = _dtype_enum(x)
-    hidden = x.shape[-1]
-    x2, r2 = _rows_view(x, hidden), _rows_view(residual, hidden)
+    hidden = shape[-1]
+    x2, r2 = _rows2(x, hidden), _rows2(residual, hidden)
     rows = x2.shape[0]
     h, y = torch.empty_like(x2), torch.empty_like(x2)
-    rstd = torch.empty(2, rows, device=dev, dtype=torch.float32)
+    rstd_post = torch.empty(rows, device=dev, dtype=torch.float32)
+    rstd_pre = torch.empty(rows, device=dev, dtype=torch.float32)
     if rows and hidden:
         wp, wn = post_weight.contiguous(), pre_weight.contiguous()
         g = None if gate is None else gate.contiguous()
-        with torch.cuda.device(dev):
-            call("evg_post_pre_norm_fwd", x2.data_ptr(), r2.data_ptr(), wp.data_ptr(), wn.data_ptr(),
-                 _p(g), kind, h.data_ptr(), y.data_ptr(), rstd[0].data_ptr(), rstd[1].data_ptr(), rows,
-                 hidden, float(alpha), float(eps), en, _stream(dev))
-    return h.view(x.shape), y.view(x.shape), rstd[0], rstd[1]
+        _enqueue(dev, "evg_post_pre_norm_fwd", x2.data_ptr(), r2.data_ptr(), wp.data_ptr(), wn.data_ptr(),
+                 None if g is None else g.data_ptr(), kind, h.data_ptr(), y.data_ptr(),
+                 rstd_post.data_ptr(), rstd_pre.data_ptr(), rows, hidden, float(alpha), float(eps), en)
+    if len(shape) != 2:
+        h, y = h.view(shape), y.view(shape)
+    return h, y, rstd_post, rstd_pre
+
+
+@functools.lru_cache(maxsize=1024)
+def _post_pre_bwd_bytes(device_index: int, rows: int, hidden: int) -> int:
+    with torch.cuda.device(device_index):
+        return lib.evg_post_pre_norm_bwd_workspace_bytes(rows, hidden)
 
 
 def post_pre_norm_bwd(dy, dh, x, h, post_weight, pre_weight, gate, rstd_post, rstd_pre, *,
@@ -868,16 +920,17 @@ def post_pre_norm_bwd(dy, dh, x, h, post_weight, pre_weight, gate, rstd_post, rs
     """Gradients of :func:`post_pre_norm_fwd` from those of its y and h (x and its h as saved).
     Returns ``(dx, dresidual, dpost_weight, dpre_weight, dgate)``; dgate has the gate's
     shape, None without one. Column sums are float32 and bit-reproducible."""
-    dev = _require_cuda(*(t for t in (dy, dh, x, h, post_weight, pre_weight, gate, rstd_post, rstd_pre)
-                          if t is not None))
+    given = (dy, dh, x, h, post_weight, pre_weight, rstd_post, rstd_pre)
+    dev = _require_cuda(*given) if gate is None else _require_cuda(*given, gate)
+    shape = x.shape
     for name, t in (("dy", dy), ("dh", dh), ("h", h)):
         _same(name, t, "x", x)
     _check_param("post_weight", post_weight, x)
     _check_param("pre_weight", pre_weight, x)
-    kind = _gate_kind(gate, x)
+    kind = 0 if gate is None else _gate_kind(gate, x)
     en = _dtype_enum(x)
-    hidden = x.shape[-1]
-    dy2, dh2, x2, h2 = (_rows_view(t, hidden) for t in (dy, dh, x, h))
+    hidden = shape[-1]
+    dy2, dh2, x2, h2 = _rows2(dy, hidden), _rows2(dh, hidden), _rows2(x, hidden), _rows2(h, hidden)
     rows = x2.shape[0]
     for name, t in (("rstd_post", rstd_post), ("rstd_pre", rstd_pre)):
         if t.dtype != torch.float32 or t.numel() != rows:
@@ -886,20 +939,22 @@ def post_pre_norm_bwd(dy, dh, x, h, post_weight, pre_weight, gate, rstd_post, rs
     g = None if gate is None else gate.contiguous()
     if not rows or not hidden:
         dgate = None if g is None else torch.zeros_like(g)
-        return (dx.view(x.shape), dres.view(x.shape), torch.zeros_like(post_weight),
+        return (dx.view(shape), dres.view(shape), torch.zeros_like(post_weight),
                 torch.zeros_like(pre_weight), dgate)
     wp, wn = post_weight.contiguous(), pre_weight.contiguous()
     r1, r2 = rstd_post.contiguous(), rstd_pre.contiguous()
     dwp, dwn = torch.empty_like(wp), torch.empty_like(wn)
     dgate = None if g is None else torch.empty_like(g)
-    with torch.cuda.device(dev):
-        ws_bytes = lib.evg_post_pre_norm_bwd_workspace_bytes(rows, hidden)
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-        call("evg_post_pre_norm_bwd", dy2.data_ptr(), dh2.data_ptr(), x2.data_ptr(), h2.data_ptr(),
-             wp.data_ptr(), wn.data_ptr(), _p(g), kind, r1.data_ptr(), r2.data_ptr(), dx.data_ptr(),
-             dres.data_ptr(), dwp.data_ptr(), dwn.data_ptr(), _p(dgate), ws.data_ptr(), ws_bytes, rows,
-             hidden, float(alpha), en, _stream(dev))
-    return dx.view(x.shape), dres.view(x.shape), dwp, dwn, dgate
+    ws_bytes = _post_pre_bwd_bytes(dev.index, rows, hidden)
+    ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
+    _enqueue(dev, "evg_post_pre_norm_bwd", dy2.data_ptr(), dh2.data_ptr(), x2.data_ptr(), h2.data_ptr(),
+             wp.data_ptr(), wn.data_ptr(), None if g is None else g.data_ptr(), kind, r1.data_ptr(),
+             r2.data_ptr(), dx.data_ptr(), dres.data_ptr(), dwp.data_ptr(), dwn.data_ptr(),
+             None if dgate is None else dgate.data_ptr(), ws.data_ptr(), ws_bytes, rows, hidden,
+             float(alpha), en)
+    if len(shape) != 2:
+        dx, dres = dx.view(shape), dres.view(shape)
+    return dx, dres, dwp, dwn, dgate
 
 
 # ---------------------------------------------- gradient norm and clipping
@@ -916,29 +971,43 @@ def _dense(t) -> bool:
 
 
 def _grad_list(grads, what):
+    """The tensors as a list, their device and dtype enums. One pass per property over the
+    whole list: a model has hundreds of them and the kernels take microseconds."""
     grads = list(grads)
     if not grads:
         raise ValueError(f"{what}: no tensors")
-    dev = _require_cuda(*grads)
-    codes = [_dtype_enum(t) for t in grads]
-    for i, t in enumerate(grads):
-        if not _dense(t):
-            raise ValueError(f"{what}: tensor {i} has gaps or repeated elements (strides {tuple(t.stride())})")
+    if not all([isinstance(t, torch.Tensor) for t in grads]):
+        raise TypeError(f"{what}: expected tensors")
+    devices = {t.device for t in grads}
+    dev = grads[0].device
+    if len(devices) != 1 or dev.type != "cuda":
+        _require_cuda(*grads)
+    try:
+        codes = [_DTYPES[t.dtype] for t in grads]
+    except KeyError as e:
+        raise TypeError(f"unsupported dtype {e.args[0]}; expected float32/float16/bfloat16") from None
+    if not all([t.is_contiguous() for t in grads]):
+        for i, t in enumerate(grads):
+            if not _dense(t):
+                raise ValueError(f"{what}: tensor {i} has gaps or repeated elements "
+                                 f"(strides {tuple(t.stride())})")
     return grads, dev, codes
 
 
-def _clip_call(grads, dev, codes, outs, max_norm, clip):
+@functools.lru_cache(maxsize=256)
+def _clip_bytes(count: int) -> int:
+    return lib.evg_clip_grads_workspace_bytes(count)
+
+
+def _clip_call(grads, dev, codes, ptrs, out_ptrs, max_norm, clip):
     n = len(grads)
     norm = torch.empty((), device=dev, dtype=torch.float32)
-    ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in grads])
-    optrs = None if outs is None else (ctypes.c_void_p * n)(*[t.data_ptr() for t in outs])
-    numel = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
-    kinds = (ctypes.c_int * n)(*codes)
-    ws_bytes = lib.evg_clip_grads_workspace_bytes(n)
+    words = ctypes.c_int64 * n
+    ws_bytes = _clip_bytes(n)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
-        call("evg_clip_grads", ptrs, optrs, numel, kinds, n, float(max_norm), 1 if clip else 0,
-             norm.data_ptr(), ws.data_ptr(), ws_bytes, _stream(dev))
+    _enqueue(dev, "evg_clip_grads", words(*ptrs), None if out_ptrs is None else words(*out_ptrs),
+             words(*[t.numel() for t in grads]), (ctypes.c_int * n)(*codes), n, float(max_norm),
+             1 if clip else 0, norm.data_ptr(), ws.data_ptr(), ws_bytes)
     return norm
 
 
@@ -946,7 +1015,7 @@ def grad_norm(grads) -> torch.Tensor:
     """2-norm over all elements of all tensors (float32 / float16 / bfloat16, mixed), as a
     float32 scalar on their device."""
     grads, dev, codes = _grad_list(grads, "grad_norm")
-    return _clip_call(grads, dev, codes, None, 0.0, False)
+    return _clip_call(grads, dev, codes, [t.data_ptr() for t in grads], None, 0.0, False)
 
 
 def clip_grad_norm(grads, max_norm: float, outs=None) -> torch.Tensor:
@@ -959,18 +1028,22 @@ def clip_grad_norm(grads, max_norm: float, outs=None) -> torch.Tensor:
     grads, dev, codes = _grad_list(grads, "clip_grad_norm")
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    ptrs = [t.data_ptr() for t in grads]
+    out_ptrs = None
     if outs is not None:
-        outs = list(outs)
-        if len(outs) != len(grads):
-            raise ValueError(f"{len(outs)} outs for {len(grads)} gradients")
-        _require_cuda(*outs, grads[0])
-        for i, (o, t) in enumerate(zip(outs, grads)):
-            if o.dtype != t.dtype or o.shape != t.shape or (o.stride() != t.stride() and t.numel() > 1):
-                raise ValueError(f"outs[{i}] must have the shape, dtype and strides of its gradient")
-    written = [t.data_ptr() for t in (grads if outs is None else outs) if t.numel()]
-    if len(set(written)) != len(written):
+        outs, odev, ocodes = _grad_list(outs, "clip_grad_norm outs")
+        if odev != dev:
+            raise RuntimeError(f"tensors on different devices: {dev} and {odev}")
+        if ocodes != codes or [t.shape for t in outs] != [t.shape for t in grads] or \
+                [t.stride() for t in outs] != [t.stride() for t in grads]:
+            raise ValueError("outs must have the shapes, dtypes and strides of their gradients")
+        out_ptrs = [t.data_ptr() for t in outs]
+    written = out_ptrs or ptrs
+    # (an empty tensor has no address of its own)
+    if len(set(written)) != len(written) and \
+            len({p for p, t in zip(written, grads) if t.numel()}) != sum([1 for t in grads if t.numel()]):
         raise ValueError("clip_grad_norm: the same tensor is listed twice")
-    return _clip_call(grads, dev, codes, outs, max_norm, True)
+    return _clip_call(grads, dev, codes, ptrs, out_ptrs, max_norm, True)
 
 
 # ------------------------------------------------------------- evoattention
