@@ -11,7 +11,12 @@
 // both tensors: with 40 heads of 128 the 64 angles of a token cost a sixth of the
 // instructions of its 320 vectors. No table of positions exists in device memory.
 //
-// HBM-bound: one read and one write per element.
+// HBM-bound: one read and one write per element. q, k [16384, 32 + 8, 128] bf16, forward
+// and backward: 108 us, 6.2 TB/s. A thread holds ONE item (two 16-byte vectors) and 40
+// registers keep six blocks on an SM: more blocks in different phases (angles, loads,
+// stores) hide the latencies better than more loads per thread (two items per thread,
+// four blocks: 125 us; four items, 71 registers: 171 us). Blocks of about 768 items
+// (three rounds) against 512 and 2048: 108, 110, 115 us.
 #include "evg_common.cuh"
 
 namespace evg {
@@ -19,16 +24,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTensors = 2;
-constexpr int kUnroll = 4;           // items in flight per thread
 constexpr int kTableFloats = 8192;   // shared memory for angles: 32 KB
 
 // n / d for 0 <= n, n * d < 2^32.
 struct Divisor {
-  uint32_t d, m;
+  uint32_t m;
   __host__ void set(uint32_t v) {
-    d = v;
-    m = (uint32_t)((0xffffffffull + v) / v);  // ceil(2^32 / v), 0 for v = 1 is fixed below
-    if (v == 1) m = 0;
+    m = v == 1 ? 0 : (uint32_t)((0xffffffffull + v) / v);  // ceil(2^32 / v)
   }
   __device__ __forceinline__ uint32_t div(uint32_t n) const { return m ? __umulhi(n, m) : n; }
 };
@@ -46,7 +48,9 @@ struct PosArgs {
   int64_t tokens;
   int tokens_per_block, heads_per_block, total_heads;
   int rd, pairs;       // rotated columns, rd / 2
-  int rot_items, items;  // per row: items that rotate, and with the copied columns
+  int rot_vecs, rot_items;    // vectors of V columns that rotate (one half of them in the half layout)
+  int copy_vecs, copy_items;  // and that are copied; an item is up to two vectors
+  int items;                  // per row
   Divisor by_items, by_heads;
   int pos64, freq64;
   float mscale;
@@ -57,18 +61,10 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Pack {
   T v[V];
 };
 
-// V elements per vector. Half layout: an item is V pairs, two vectors rd / 2 apart.
-// Interleaved: an item is one vector of V / 2 pairs. A copy item is one vector.
-template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(kThreads)
-rope_positions_kernel(const __grid_constant__ PosArgs a) {
-  constexpr int PV = INTER ? V / 2 : V;  // pairs per item
-  extern __shared__ float2 table[];      // [token][pair e of item][item]: (cos, sin)
-  const int64_t t0 = (int64_t)blockIdx.x * a.tokens_per_block;
-  const int nt = (int)(a.tokens - t0 < a.tokens_per_block ? a.tokens - t0 : a.tokens_per_block);
-  const int h0 = blockIdx.y * a.heads_per_block;
-  const int nh = a.total_heads - h0 < a.heads_per_block ? a.total_heads - h0 : a.heads_per_block;
-
+// (cos, sin) of the block's tokens into shared memory, [token][pair e of a vector][vector]
+// with PV pairs per vector, so the threads of a warp read neighbouring words.
+template <int PV>
+__device__ __forceinline__ void fill_table(const PosArgs& a, int64_t t0, int nt, int vecs, float2* table) {
   for (int j = threadIdx.x; j < nt * a.pairs; j += kThreads) {
     const int tok = j / a.pairs, i = j % a.pairs;
     const double pos = a.pos64 ? (double)((const int64_t*)a.positions)[t0 + tok]
@@ -77,55 +73,69 @@ rope_positions_kernel(const __grid_constant__ PosArgs a) {
     const double turns = pos * (f * 0.15915494309189533576888);  // 1 / (2 pi)
     float s, c;
     sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    // item-major within the pair number, so the threads of a warp read neighbouring words
-    table[(tok * PV + i % PV) * a.rot_items + i / PV] = make_float2(c * a.mscale, (a.inverse ? -s : s) * a.mscale);
+    table[(tok * PV + i % PV) * vecs + i / PV] = make_float2(c * a.mscale, (a.inverse ? -s : s) * a.mscale);
   }
+}
+
+// V elements per vector, an item is two of them. Half layout: V pairs, the vectors rd / 2
+// apart. Interleaved, and the columns that are only copied: two vectors of V / 2 pairs
+// (or V copied columns) each, half of the row's vectors apart; the second is missing in the
+// last item of an odd number.
+// COPY: there are columns that are only copied.
+template <typename T, int V, bool INTER, bool COPY>
+__global__ void __launch_bounds__(kThreads, 6)
+rope_positions_kernel(const __grid_constant__ PosArgs a) {
+  constexpr int PV = INTER ? V / 2 : V;  // pairs per vector
+  extern __shared__ float2 table[];
+  const int64_t t0 = (int64_t)blockIdx.x * a.tokens_per_block;
+  const int nt = (int)(a.tokens - t0 < a.tokens_per_block ? a.tokens - t0 : a.tokens_per_block);
+  const int h0 = blockIdx.y * a.heads_per_block;
+  const int nh = a.total_heads - h0 < a.heads_per_block ? a.total_heads - h0 : a.heads_per_block;
+  fill_table<PV>(a, t0, nt, a.rot_vecs, table);
   __syncthreads();
 
   const int n = nt * nh * a.items;
-  for (int base = threadIdx.x; base < n; base += kThreads * kUnroll) {
-    Pack<T, V> lo[kUnroll], hi[kUnroll];
-    T* dst[kUnroll];
-    int item[kUnroll], tok[kUnroll];
+  for (int idx = threadIdx.x; idx < n; idx += kThreads) {
+    const uint32_t row = a.by_items.div(idx);
+    int item = idx - row * a.items;
+    const int tok = a.by_heads.div(row);
+    const int h = h0 + row - tok * nh;
+    const int which = h >= a.t[0].heads;
+    const PosTensor& tz = a.t[which];
+    const int head = h - (which ? a.t[0].heads : 0);
+    const int64_t t = t0 + tok;
+    const bool rot = !COPY || item < a.rot_items;
+    item -= rot ? 0 : a.rot_items;
+    const int apart = rot ? a.rot_items : a.copy_items;  // vectors between the item's two
+    const int col = (rot ? 0 : a.rd) + item * V;
+    const bool two = (rot && !INTER) || item + apart < (rot ? a.rot_vecs : a.copy_vecs);
+    const T* src = (const T*)tz.x + t * tz.xst + head * tz.xsh + col;
+    T* dst = (T*)tz.y + t * tz.yst + head * tz.ysh + col;
+    Pack<T, V> lo = *reinterpret_cast<const Pack<T, V>*>(src), hi = lo;
+    if (two) hi = *reinterpret_cast<const Pack<T, V>*>(src + apart * V);
+    if (rot) {
+      const float2* cs = table + tok * PV * a.rot_vecs + item;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int idx = base + u * kThreads;
-      if (idx < n) {
-        const uint32_t row = a.by_items.div(idx);
-        item[u] = idx - row * a.items;
-        tok[u] = a.by_heads.div(row);
-        const int h = h0 + row - tok[u] * nh;
-        const int which = h >= a.t[0].heads;
-        const PosTensor& tz = a.t[which];
-        const int head = h - (which ? a.t[0].heads : 0);
-        const int64_t t = t0 + tok[u];
-        const bool rot = item[u] < a.rot_items;
-        const int col = rot ? item[u] * V : a.rd + (item[u] - a.rot_items) * V;
-        const T* src = (const T*)tz.x + t * tz.xst + head * tz.xsh + col;
-        dst[u] = (T*)tz.y + t * tz.yst + head * tz.ysh + col;
-        lo[u] = *reinterpret_cast<const Pack<T, V>*>(src);
-        if (!INTER && rot) hi[u] = *reinterpret_cast<const Pack<T, V>*>(src + a.pairs);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (base + u * kThreads < n) {
-        if (item[u] < a.rot_items) {
-          const float2* cs = table + tok[u] * PV * a.rot_items + item[u];
-#pragma unroll
-          for (int e = 0; e < PV; ++e) {
-            const float2 w = cs[e * a.rot_items];
-            T& p1 = INTER ? lo[u].v[2 * e < V ? 2 * e : 0] : lo[u].v[e];
-            T& p2 = INTER ? lo[u].v[2 * e + 1 < V ? 2 * e + 1 : 0] : hi[u].v[e];
-            const float x1 = to_f32<T>(p1), x2 = to_f32<T>(p2);
-            p1 = from_f32<T>(fmaf(x1, w.x, -(x2 * w.y)));
-            p2 = from_f32<T>(fmaf(x2, w.x, x1 * w.y));
-          }
-          if (!INTER) *reinterpret_cast<Pack<T, V>*>(dst[u] + a.pairs) = hi[u];
+      for (int e = 0; e < PV; ++e) {
+        if constexpr (INTER) {
+          const float2 w = cs[e * a.rot_vecs];
+          const float2 z = two ? cs[e * a.rot_vecs + apart] : w;
+          const float a1 = to_f32<T>(lo.v[2 * e]), a2 = to_f32<T>(lo.v[2 * e + 1]);
+          const float b1 = to_f32<T>(hi.v[2 * e]), b2 = to_f32<T>(hi.v[2 * e + 1]);
+          lo.v[2 * e] = from_f32<T>(fmaf(a1, w.x, -(a2 * w.y)));
+          lo.v[2 * e + 1] = from_f32<T>(fmaf(a2, w.x, a1 * w.y));
+          hi.v[2 * e] = from_f32<T>(fmaf(b1, z.x, -(b2 * z.y)));
+          hi.v[2 * e + 1] = from_f32<T>(fmaf(b2, z.x, b1 * z.y));
+        } else {
+          const float2 w = cs[e * a.rot_vecs];
+          const float x1 = to_f32<T>(lo.v[e]), x2 = to_f32<T>(hi.v[e]);
+          lo.v[e] = from_f32<T>(fmaf(x1, w.x, -(x2 * w.y)));
+          hi.v[e] = from_f32<T>(fmaf(x2, w.x, x1 * w.y));
         }
-        *reinterpret_cast<Pack<T, V>*>(dst[u]) = lo[u];
       }
     }
+    *reinterpret_cast<Pack<T, V>*>(dst) = lo;
+    if (two) *reinterpret_cast<Pack<T, V>*>(dst + apart * V) = hi;
   }
 }
 
@@ -138,16 +148,7 @@ rope_positions_scalar_kernel(const __grid_constant__ PosArgs a) {
   const int nt = (int)(a.tokens - t0 < a.tokens_per_block ? a.tokens - t0 : a.tokens_per_block);
   const int h0 = blockIdx.y * a.heads_per_block;
   const int nh = a.total_heads - h0 < a.heads_per_block ? a.total_heads - h0 : a.heads_per_block;
-  for (int j = threadIdx.x; j < nt * a.pairs; j += kThreads) {
-    const int tok = j / a.pairs, i = j % a.pairs;
-    const double pos = a.pos64 ? (double)((const int64_t*)a.positions)[t0 + tok]
-                               : (double)((const int32_t*)a.positions)[t0 + tok];
-    const double f = a.freq64 ? ((const double*)a.inv_freq)[i] : (double)((const float*)a.inv_freq)[i];
-    const double turns = pos * (f * 0.15915494309189533576888);
-    float s, c;
-    sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-    table[j] = make_float2(c * a.mscale, (a.inverse ? -s : s) * a.mscale);
-  }
+  fill_table<1>(a, t0, nt, a.pairs, table);
   __syncthreads();
   const int n = nt * nh * a.items;
   for (int idx = threadIdx.x; idx < n; idx += kThreads) {
@@ -189,14 +190,17 @@ int launch_positions(PosArgs& a, int count, int64_t D, bool interleaved, cudaStr
   };
   while (V > 1 && !fits(V)) V /= 2;
   const bool scalar = interleaved && V == 1;
-  a.rot_items = scalar ? a.pairs : (interleaved ? a.rd : a.pairs) / V;
-  a.items = a.rot_items + (int)((D - a.rd) / V);
-  // A block takes whole tokens with all their heads, about eight rounds of items, fewer
+  a.rot_vecs = scalar ? a.pairs : (interleaved ? a.rd : a.pairs) / V;
+  a.rot_items = interleaved && !scalar ? (a.rot_vecs + 1) / 2 : a.rot_vecs;
+  a.copy_vecs = (int)((D - a.rd) / V);
+  a.copy_items = scalar ? a.copy_vecs : (a.copy_vecs + 1) / 2;
+  a.items = a.rot_items + a.copy_items;
+  // A block takes whole tokens with all their heads, about three rounds of items, fewer
   // when that would leave SMs without a block; heads are cut when one token is too much
   // for a block or there are few tokens.
   const int64_t per_token = (int64_t)a.total_heads * a.items;
   const int sms = device_info().sm_count;
-  int64_t tb = (kThreads * 8 + per_token - 1) / per_token;
+  int64_t tb = (kThreads * 3 + per_token - 1) / per_token;
   if (tb > (a.tokens + 2 * sms - 1) / (2 * sms)) tb = (a.tokens + 2 * sms - 1) / (2 * sms);
   if (tb > kTableFloats / 2 / a.pairs) tb = kTableFloats / 2 / a.pairs;
   if (tb < 1) tb = 1;
@@ -225,10 +229,13 @@ int launch_positions(PosArgs& a, int count, int64_t D, bool interleaved, cudaStr
     rope_positions_scalar_kernel<T><<<grid, kThreads, smem, stream>>>(a);
     return check_launch("rope_positions");
   }
-#define EVG_ROPE_V(v)                                                                              \
-  if (V == v) {                                                                                    \
-    if (interleaved) rope_positions_kernel<T, v < 2 ? 2 : v, true><<<grid, kThreads, smem, stream>>>(a); \
-    else rope_positions_kernel<T, v, false><<<grid, kThreads, smem, stream>>>(a);                  \
+#define EVG_ROPE_V(v)                                                                           \
+  if (V == v) {                                                                                 \
+    constexpr int w = v < 2 ? 2 : v; /* interleaved pairs are whole vectors */                  \
+    if (interleaved && a.copy_vecs) rope_positions_kernel<T, w, true, true><<<grid, kThreads, smem, stream>>>(a); \
+    else if (interleaved) rope_positions_kernel<T, w, true, false><<<grid, kThreads, smem, stream>>>(a);          \
+    else if (a.copy_vecs) rope_positions_kernel<T, v, false, true><<<grid, kThreads, smem, stream>>>(a);          \
+    else rope_positions_kernel<T, v, false, false><<<grid, kThreads, smem, stream>>>(a);        \
   }
   if constexpr (sizeof(T) == 2) EVG_ROPE_V(8)
   EVG_ROPE_V(4) EVG_ROPE_V(2) EVG_ROPE_V(1)
