@@ -17,12 +17,16 @@
 // need eight and fourteen.
 //
 // A row belongs to one warp (up to 64 16-byte vectors) or to one block whose threads
-// hold V vectors each; blocks are persistent, a thread keeps its columns for all its
+// hold V vectors each and whose next rows come through a shared-memory ring; blocks are persistent, a thread keeps its columns for all its
 // rows, so the weights and the column sums stay in registers. Column sums leave as one
 // float32 partial row per block and are added by a second kernel in a fixed order.
 #include "evg_common.cuh"
+#include "sm100_umma.cuh"
 
 namespace evg {
+
+__device__ int g_post_pre_device_status = 0;
+
 namespace {
 
 enum Gate { kNone = 0, kChannel = 1, kToken = 2, kFull = 3 };
@@ -36,259 +40,448 @@ struct NormArgs {
   float* partial;                             // [2][blocks][C]: dw_pre, dw_post sums
   int64_t rows, C;
   float alpha, eps, inv_c;
+  int stages;                                 // of the ring
 };
 
-__device__ __forceinline__ uint4 ld_stream(const void* base, int64_t row, int64_t C, int vec, int elem_bytes) {
-  return ld_vec(reinterpret_cast<const uint8_t*>(base) + row * C * elem_bytes + (int64_t)vec * 16);
+// How a row reaches its threads.
+//   kWarp    a warp per row, global loads (rows of up to 64 16-byte vectors)
+//   kDirect  a block per row, global loads (rows of which two do not fit shared memory)
+//   kRing    a block per row; the block's next rows are on their way into a ring of
+//            shared-memory stages (untiled bulk copies, one issuing thread, bounded waits)
+// kWarp and kRing keep both weights in shared memory as float32 (the post weight times a
+// channel's gate), kDirect reads them from global memory for every row.
+enum Mode { kWarp = 0, kDirect = 1, kRing = 2 };
+constexpr int kMaxStages = 4;
+constexpr long long kWaitCycles = 2000000000ll;
+
+struct Ring {
+  uint64_t full[kMaxStages];
+  int abort_flag;
+};
+
+template <int N_ARRAYS, int MODE>
+struct Rows {
+  const uint8_t* base[N_ARRAYS];
+  uint8_t* stages;
+  Ring* ring;
+  int64_t rows, stride;
+  uint32_t row_bytes;
+  int n_stages, stage;
+  uint32_t parity;
+  const uint8_t* at[N_ARRAYS];  // the current row's arrays
+
+  // Ring mode, one thread: row -> stage.
+  __device__ __forceinline__ void issue(int s, int64_t row) {
+    using namespace umma;
+    uint8_t* dst = stages + (size_t)s * N_ARRAYS * row_bytes;
+    mbar_expect_tx(ring->full + s, N_ARRAYS * row_bytes);
+#pragma unroll
+    for (int i = 0; i < N_ARRAYS; ++i)
+      bulk_load_1d(dst + i * row_bytes, base[i] + row * row_bytes, row_bytes, ring->full + s);
+  }
+  __device__ __forceinline__ void start(int64_t first) {
+    using namespace umma;
+    stage = 0;
+    parity = 0;
+    if constexpr (MODE == kRing) {
+      if (threadIdx.x == 0) {
+        ring->abort_flag = 0;
+        for (int s = 0; s < n_stages; ++s) mbar_init(ring->full + s, 1);
+        fence_mbar_init();
+      }
+      __syncthreads();
+      if (threadIdx.x == 0)
+        for (int s = 0; s < n_stages; ++s)
+          if (first + s * stride < rows) issue(s, first + s * stride);
+    }
+  }
+  __device__ __forceinline__ void open(int64_t row) {
+    if constexpr (MODE == kRing) {
+      const umma::WaitCtx ctx{&ring->abort_flag, &g_post_pre_device_status, kWaitCycles};
+      umma::mbar_wait(ring->full + stage, parity, ctx, 411);
+    }
+#pragma unroll
+    for (int i = 0; i < N_ARRAYS; ++i)
+      at[i] = MODE == kRing ? stages + ((size_t)stage * N_ARRAYS + i) * row_bytes : base[i] + row * row_bytes;
+  }
+  __device__ __forceinline__ uint4 get(int array, int vec) const {
+    if constexpr (MODE == kRing) return *reinterpret_cast<const uint4*>(at[array] + vec * 16);
+    else return ld_vec(at[array] + vec * 16);
+  }
+  // Behind a block barrier that follows the row's last get(): the stage takes the row
+  // n_stages further on.
+  __device__ __forceinline__ void close(int64_t row) {
+    if constexpr (MODE == kRing) {
+      const int64_t next = row + n_stages * stride;
+      if (threadIdx.x == 0 && next < rows && !*(volatile int*)&ring->abort_flag) issue(stage, next);
+      if (++stage == n_stages) { stage = 0; parity ^= 1; }
+    }
+  }
+  __device__ __forceinline__ void finish() {
+    if constexpr (MODE == kRing)
+      if (threadIdx.x == 0 && *(volatile int*)&ring->abort_flag) umma::settle_after_abort();
+  }
+};
+
+// Pairs of neighbouring elements as packed float32 (one instruction for both).
+template <typename T> __device__ __forceinline__ void unpack2(const uint4& v, f32x2 (&f)[Vec<T>::N / 2]) {
+  float e[Vec<T>::N];
+  unpack<T>(v, e);
+#pragma unroll
+  for (int i = 0; i < Vec<T>::N / 2; ++i) f[i] = f2_make(e[2 * i], e[2 * i + 1]);
 }
-__device__ __forceinline__ void st_stream(void* base, int64_t row, int64_t C, int vec, int elem_bytes, const uint4& v) {
-  st_vec(reinterpret_cast<uint8_t*>(base) + row * C * elem_bytes + (int64_t)vec * 16, v);
+template <typename T> __device__ __forceinline__ uint4 pack2f(const f32x2 (&f)[Vec<T>::N / 2]) {
+  float e[Vec<T>::N];
+#pragma unroll
+  for (int i = 0; i < Vec<T>::N / 2; ++i) f2_split(f[i], e[2 * i], e[2 * i + 1]);
+  return pack<T>(e);
+}
+__device__ __forceinline__ float f2_sum(f32x2 v) {
+  float lo, hi;
+  f2_split(v, lo, hi);
+  return lo + hi;
 }
 
-// Sum of NV values over the row's threads: a warp, or the whole block (partials through
-// shared memory, [2][NV][32] floats, one barrier: the halves alternate).
-template <int NV, bool WARP>
-__device__ __forceinline__ void row_sum(float (&v)[NV], float* scratch, int& phase) {
-  if constexpr (WARP) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-#pragma unroll
-      for (int i = 0; i < NV; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], off);
-  } else {
-    block_allreduce<NV, SumOp>(v, scratch, phase);
-  }
+__device__ __forceinline__ void st_row(void* base, int64_t row, uint32_t row_bytes, int vec, const uint4& v) {
+  st_vec(reinterpret_cast<uint8_t*>(base) + row * row_bytes + vec * 16, v);
 }
+
+// Sum over the row's threads: a warp, or the whole block (one partial per warp through
+// shared memory, [2][32] floats that are zero behind the last warp; one barrier, the
+// halves alternate).
+template <int MODE>
+__device__ __forceinline__ float row_sum(float v, float* scratch, int& phase) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  if constexpr (MODE != kWarp) {
+    float* buf = scratch + phase * 32;
+    phase ^= 1;
+    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.f;
+    for (int w = 0; w < (int)blockDim.x; w += 128) {
+      const float4 p = *reinterpret_cast<const float4*>(buf + w / 32);
+      v += (p.x + p.y) + (p.z + p.w);
+    }
+  }
+  return v;
+}
+
+constexpr int max_threads(int mode) { return mode == kWarp ? 256 : 512; }
+constexpr size_t ring_bytes(int stages, int arrays, int64_t C, size_t elem) {
+  return (size_t)stages * arrays * C * elem + 2 * C * sizeof(float);
+}
+
+// The weights of a block: float32 in shared memory (w_pre, then w_post times a channel's
+// gate), or global memory. Columns of vector `vec` as packed pairs.
+template <typename T, int GATE, int MODE>
+struct Weights {
+  static constexpr int N = Vec<T>::N, P = N / 2;
+  float *pre_s, *post_s;
+  const NormArgs* a;
+  __device__ __forceinline__ void load(const NormArgs& args, float* smem) {
+    a = &args;
+    pre_s = smem;
+    post_s = smem + args.C;
+    if constexpr (MODE != kDirect) {
+      for (int c = threadIdx.x; c < (int)args.C; c += blockDim.x) {
+        pre_s[c] = to_f32<T>(((const T*)args.w_pre)[c]);
+        float w = to_f32<T>(((const T*)args.w_post)[c]);
+        if (GATE == kChannel) w *= to_f32<T>(((const T*)args.gate)[c]);
+        post_s[c] = w;
+      }
+      __syncthreads();
+    }
+  }
+  __device__ __forceinline__ void from_shared(const float* p, f32x2 (&w)[P]) const {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const float4 q = *reinterpret_cast<const float4*>(p + 4 * i);
+      w[2 * i] = f2_make(q.x, q.y);
+      w[2 * i + 1] = f2_make(q.z, q.w);
+    }
+  }
+  __device__ __forceinline__ void pre(int vec, f32x2 (&w)[P]) const {
+    if constexpr (MODE != kDirect) from_shared(pre_s + vec * N, w);
+    else unpack2<T>(__ldg(reinterpret_cast<const uint4*>(a->w_pre) + vec), w);
+  }
+  __device__ __forceinline__ void post(int vec, f32x2 (&w)[P]) const {
+    if constexpr (MODE != kDirect) {
+      from_shared(post_s + vec * N, w);
+    } else {
+      unpack2<T>(__ldg(reinterpret_cast<const uint4*>(a->w_post) + vec), w);
+      if constexpr (GATE == kChannel) {
+        f32x2 g[P];
+        unpack2<T>(__ldg(reinterpret_cast<const uint4*>(a->gate) + vec), g);
+#pragma unroll
+        for (int i = 0; i < P; ++i) w[i] = f2_mul(w[i], g[i]);
+      }
+    }
+  }
+};
 
 // ------------------------------------------------------------------ forward
-template <typename T, int V, int GATE, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024)
+template <typename T, int V, int GATE, int MODE>
+__global__ void __launch_bounds__(max_threads(MODE))
 post_pre_fwd_kernel(const NormArgs a) {
-  constexpr int N = Vec<T>::N, E = sizeof(T);
-  __shared__ float scratch[2 * 32];
+  constexpr int N = Vec<T>::N, P = N / 2;
+  constexpr int NA = GATE == kFull ? 3 : 2;  // x, h, gate
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ __align__(16) float scratch[2 * 32];
+  __shared__ Ring ring;
   int phase = 0;
-  const int lane = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int width = WARP ? 32 : blockDim.x;
+  const int lane = MODE == kWarp ? threadIdx.x & 31 : threadIdx.x;
+  const int width = MODE == kWarp ? 32 : blockDim.x;
   const int nvec = (int)(a.C / N);
-  const int64_t stride = WARP ? (int64_t)gridDim.x * (blockDim.x / 32) : gridDim.x;
-  int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
-  int vec[V];
-  bool on[V];
-  uint4 wpost[V], wpre[V], gch[V];
+  const int64_t stride = MODE == kWarp ? (int64_t)gridDim.x * (blockDim.x / 32) : gridDim.x;
+  int64_t row = MODE == kWarp ? (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+  if (threadIdx.x < 64) scratch[threadIdx.x] = 0.f;
+  Rows<NA, MODE> in;
+  in.base[0] = (const uint8_t*)a.x;
+  in.base[1] = (const uint8_t*)a.h;
+  if constexpr (GATE == kFull) in.base[2] = (const uint8_t*)a.gate;
+  in.stages = dyn;
+  in.ring = &ring;
+  in.rows = a.rows;
+  in.stride = stride;
+  in.row_bytes = nvec * 16;
+  in.n_stages = a.stages;
+  in.start(row);
+  Weights<T, GATE, MODE> w;
+  w.load(a, reinterpret_cast<float*>(dyn + (MODE == kRing ? (size_t)a.stages * NA * in.row_bytes : 0)));
+  float gt_next = GATE == kToken && row < a.rows ? to_f32<T>(((const T*)a.gate)[row]) : 1.f;
+  for (; row < a.rows; row += stride) {
+    in.open(row);
+    const float gt = gt_next;
+    if (GATE == kToken && row + stride < a.rows) gt_next = to_f32<T>(((const T*)a.gate)[row + stride]);
+    f32x2 x[V][P], hn[V][P], acc = 0ull;
+    uint4 hv[V], gv[V];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    vec[j] = lane + j * width;
-    on[j] = vec[j] < nvec;
-    wpost[j] = wpre[j] = gch[j] = make_uint4(0, 0, 0, 0);
-    if (on[j]) {
-      wpost[j] = ld_vec((const uint8_t*)a.w_post + vec[j] * 16);
-      wpre[j] = ld_vec((const uint8_t*)a.w_pre + vec[j] * 16);
-      if (GATE == kChannel) gch[j] = ld_vec((const uint8_t*)a.gate + vec[j] * 16);
+    for (int j = 0; j < V; ++j) {
+      const int vec = lane + j * width;
+      const bool on = vec < nvec;
+      unpack2<T>(on ? in.get(0, vec) : make_uint4(0, 0, 0, 0), x[j]);
+      hv[j] = on ? in.get(1, vec) : make_uint4(0, 0, 0, 0);
+      if constexpr (GATE == kFull) gv[j] = on ? in.get(2, vec) : make_uint4(0, 0, 0, 0);
     }
-  }
-  uint4 xv[V], hv[V], gv[V];
-  auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (on[j]) {
-        xv[j] = ld_stream(a.x, r, a.C, vec[j], E);
-        hv[j] = ld_stream(a.h, r, a.C, vec[j], E);
-        if (GATE == kFull) gv[j] = ld_stream(a.gate, r, a.C, vec[j], E);
-      } else {
-        xv[j] = hv[j] = gv[j] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < P; ++i) acc = f2_fma(x[j][i], x[j][i], acc);
+    const float r1 = rsqrtf(fmaf(row_sum<MODE>(f2_sum(acc), scratch, phase), a.inv_c, a.eps));
+    in.close(row);
+    const f32x2 scale = f2_splat(r1 * a.alpha * gt);
+    acc = 0ull;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int vec = lane + j * width;
+      unpack2<T>(hv[j], hn[j]);
+      if (vec < nvec) {
+        f32x2 wp[P], g[P];
+        w.post(vec, wp);
+        if constexpr (GATE == kFull) unpack2<T>(gv[j], g);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          f32x2 n = f2_mul(x[j][i], wp[i]);
+          if constexpr (GATE == kFull) n = f2_mul(n, g[i]);
+          hn[j][i] = f2_fma(n, scale, hn[j][i]);
+          acc = f2_fma(hn[j][i], hn[j][i], acc);
+        }
+        st_row(a.h_out, row, in.row_bytes, vec, pack2f<T>(hn[j]));
       }
-  };
-  if (row < a.rows) fetch(row);
-  for (; row < a.rows; row += stride) {
-    float hn[V][N], x[V][N];
-    float s[1] = {0.f};
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      unpack<T>(xv[j], x[j]);
-      unpack<T>(hv[j], hn[j]);
-#pragma unroll
-      for (int i = 0; i < N; ++i) s[0] = fmaf(x[j][i], x[j][i], s[0]);
     }
-    const float gt = GATE == kToken ? to_f32<T>(((const T*)a.gate)[row]) : 1.f;
-    uint4 gnow[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) gnow[j] = GATE == kFull ? gv[j] : gch[j];
-    if (row + stride < a.rows) fetch(row + stride);  // the next row is on its way during the sums
-    row_sum<1, WARP>(s, scratch, phase);
-    const float r1 = rsqrtf(fmaf(s[0], a.inv_c, a.eps));
-    const float scale = r1 * a.alpha * gt;
-    s[0] = 0.f;
+    const float r2 = rsqrtf(fmaf(row_sum<MODE>(f2_sum(acc), scratch, phase), a.inv_c, a.eps));
+    const f32x2 rr = f2_splat(r2);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float w[N], g[N];
-      unpack<T>(wpost[j], w);
-      if (GATE == kChannel || GATE == kFull) unpack<T>(gnow[j], g);
+      const int vec = lane + j * width;
+      if (vec < nvec) {
+        f32x2 wn[P];
+        w.pre(vec, wn);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        float n = x[j][i] * scale * w[i];
-        if (GATE == kChannel || GATE == kFull) n *= g[i];
-        hn[j][i] += n;
-        s[0] = fmaf(hn[j][i], hn[j][i], s[0]);
+        for (int i = 0; i < P; ++i) wn[i] = f2_mul(f2_mul(hn[j][i], rr), wn[i]);
+        st_row(a.y, row, in.row_bytes, vec, pack2f<T>(wn));
       }
-      if (on[j]) st_stream(a.h_out, row, a.C, vec[j], E, pack<T>(hn[j]));
-    }
-    row_sum<1, WARP>(s, scratch, phase);
-    const float r2 = rsqrtf(fmaf(s[0], a.inv_c, a.eps));
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float w[N], y[N];
-      unpack<T>(wpre[j], w);
-#pragma unroll
-      for (int i = 0; i < N; ++i) y[i] = hn[j][i] * r2 * w[i];
-      if (on[j]) st_stream(a.y, row, a.C, vec[j], E, pack<T>(y));
     }
     if (lane == 0) {
       a.rstd_post[row] = r1;
       a.rstd_pre[row] = r2;
     }
   }
+  in.finish();
 }
 
 // ----------------------------------------------------------------- backward
-template <typename T, int V, int GATE, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : (V == 1 ? 1024 : 512))
+// With U = G w_post gate (the gate of a full or channel kind; a row's number stays outside):
+//   sum u xhat = alpha gate_row rstd1 sum U x,  dx = rstd1 alpha gate_row U - x rstd1^2 c2
+// so that each of the three steps between the two reductions needs few instructions and
+// only U and x cross the second one.
+template <typename T, int V, int GATE, int MODE>
+__global__ void __launch_bounds__(max_threads(MODE))
 post_pre_bwd_kernel(const NormArgs a) {
-  constexpr int N = Vec<T>::N, E = sizeof(T);
-  extern __shared__ float fold[];  // WARP: one partial row, [2][C]
-  __shared__ float scratch[2 * 2 * 32];
+  constexpr int N = Vec<T>::N, P = N / 2;
+  constexpr int NA = GATE == kFull ? 5 : 4;  // dy, h', dh', x, gate
+  extern __shared__ __align__(128) uint8_t dyn[];  // ring stages, weights; kWarp: weights, a partial row
+  __shared__ __align__(16) float scratch[2 * 32];
+  __shared__ Ring ring;
   int phase = 0;
-  const int lane = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int width = WARP ? 32 : blockDim.x;
+  const int lane = MODE == kWarp ? threadIdx.x & 31 : threadIdx.x;
+  const int width = MODE == kWarp ? 32 : blockDim.x;
   const int nvec = (int)(a.C / N);
-  const int64_t stride = WARP ? (int64_t)gridDim.x * (blockDim.x / 32) : gridDim.x;
-  int64_t row = WARP ? (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
-  int vec[V];
-  bool on[V];
-  uint4 wpost[V], wpre[V], gch[V];
-  float spost[V][N], spre[V][N];
+  const int64_t stride = MODE == kWarp ? (int64_t)gridDim.x * (blockDim.x / 32) : gridDim.x;
+  int64_t row = MODE == kWarp ? (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
+  if (threadIdx.x < 64) scratch[threadIdx.x] = 0.f;
+  Rows<NA, MODE> in;
+  in.base[0] = (const uint8_t*)a.dy;
+  in.base[1] = (const uint8_t*)a.h;
+  in.base[2] = (const uint8_t*)a.dh_in;
+  in.base[3] = (const uint8_t*)a.x;
+  if constexpr (GATE == kFull) in.base[4] = (const uint8_t*)a.gate;
+  in.stages = dyn;
+  in.ring = &ring;
+  in.rows = a.rows;
+  in.stride = stride;
+  in.row_bytes = nvec * 16;
+  in.n_stages = a.stages;
+  in.start(row);
+  Weights<T, GATE, MODE> w;
+  w.load(a, reinterpret_cast<float*>(dyn + (MODE == kRing ? (size_t)a.stages * NA * in.row_bytes : 0)));
+  f32x2 spost[V][P], spre[V][P];
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    vec[j] = lane + j * width;
-    on[j] = vec[j] < nvec;
-    wpost[j] = wpre[j] = gch[j] = make_uint4(0, 0, 0, 0);
-    if (on[j]) {
-      wpost[j] = ld_vec((const uint8_t*)a.w_post + vec[j] * 16);
-      wpre[j] = ld_vec((const uint8_t*)a.w_pre + vec[j] * 16);
-      if (GATE == kChannel) gch[j] = ld_vec((const uint8_t*)a.gate + vec[j] * 16);
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < P; ++i) spost[j][i] = spre[j][i] = 0ull;
+  // the row's numbers come one row ahead: nothing else hides their latency
+  float r1_next = 0.f, r2_next = 0.f, gt_next = 1.f;
+  auto ahead = [&](int64_t r) {
+    if (r < a.rows) {
+      r1_next = a.rstd_post[r];
+      r2_next = a.rstd_pre[r];
+      if (GATE == kToken) gt_next = to_f32<T>(((const T*)a.gate)[r]);
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) spost[j][i] = spre[j][i] = 0.f;
-  }
+  };
+  ahead(row);
   for (; row < a.rows; row += stride) {
-    uint4 yv[V], dv[V], xv[V], hv[V], gv[V];
+    const float r1 = r1_next, r2 = r2_next, gt = gt_next;
+    ahead(row + stride);
+    in.open(row);
+    f32x2 t[V][P], h[V][P], acc = 0ull;
+    uint4 dv[V], xv[V], gv[V];
+    if constexpr (MODE != kRing) {  // loads of the second step already now
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      yv[j] = dv[j] = xv[j] = hv[j] = gv[j] = make_uint4(0, 0, 0, 0);
-      if (on[j]) {
-        yv[j] = ld_stream(a.dy, row, a.C, vec[j], E);
-        hv[j] = ld_stream(a.h, row, a.C, vec[j], E);
-        dv[j] = ld_stream(a.dh_in, row, a.C, vec[j], E);
-        xv[j] = ld_stream(a.x, row, a.C, vec[j], E);
-        if (GATE == kFull) gv[j] = ld_stream(a.gate, row, a.C, vec[j], E);
+      for (int j = 0; j < V; ++j) {
+        const int vec = lane + j * width;
+        dv[j] = vec < nvec ? in.get(2, vec) : make_uint4(0, 0, 0, 0);
+        xv[j] = vec < nvec ? in.get(3, vec) : make_uint4(0, 0, 0, 0);
+        if constexpr (GATE == kFull) gv[j] = vec < nvec ? in.get(4, vec) : make_uint4(0, 0, 0, 0);
       }
     }
-    const float r1 = a.rstd_post[row], r2 = a.rstd_pre[row];
-    const float gt = GATE == kToken ? to_f32<T>(((const T*)a.gate)[row]) : 1.f;
-    float s1[1] = {0.f};
+    const f32x2 rr2 = f2_splat(r2);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float dy[N], h[N], w[N];
-      unpack<T>(yv[j], dy);
-      unpack<T>(hv[j], h);
-      unpack<T>(wpre[j], w);
+      const int vec = lane + j * width;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float p = dy[i] * (h[i] * r2);
-        spre[j][i] += p;
-        s1[0] = fmaf(p, w[i], s1[0]);
+      for (int i = 0; i < P; ++i) t[j][i] = h[j][i] = 0ull;
+      if (vec < nvec) {
+        f32x2 dy[P], wn[P];
+        unpack2<T>(in.get(0, vec), dy);
+        unpack2<T>(in.get(1, vec), h[j]);
+        w.pre(vec, wn);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          h[j][i] = f2_mul(h[j][i], rr2);                     // h'hat
+          t[j][i] = f2_mul(dy[i], wn[i]);
+          spre[j][i] = f2_fma(dy[i], h[j][i], spre[j][i]);
+          acc = f2_fma(t[j][i], h[j][i], acc);
+        }
       }
     }
-    row_sum<1, WARP>(s1, scratch, phase);
-    const float c1 = s1[0] * a.inv_c;
-    float G[V][N];
-    float s2[2] = {0.f, 0.f};  // sum u xhat; sum G n / alpha (token gate)
+    const float c1 = row_sum<MODE>(f2_sum(acc), scratch, phase) * a.inv_c;
+    const f32x2 k1 = f2_splat(-r2 * c1);
     const float ag = a.alpha * gt;
+    const f32x2 kpost = f2_splat(r1 * ag);
+    f32x2 x[V][P];
+    acc = 0ull;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float dy[N], h[N], w[N], d[N], x[N], wp[N], g[N];
-      unpack<T>(yv[j], dy);
-      unpack<T>(hv[j], h);
-      unpack<T>(wpre[j], w);
-      unpack<T>(dv[j], d);
-      unpack<T>(xv[j], x);
-      unpack<T>(wpost[j], wp);
-      if (GATE == kChannel) unpack<T>(gch[j], g);
-      if (GATE == kFull) unpack<T>(gv[j], g);
+      const int vec = lane + j * width;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        G[j][i] = fmaf(r2, fmaf(dy[i], w[i], -(h[i] * r2 * c1)), d[i]);
-        const float q = G[j][i] * (x[i] * r1);  // G xhat
-        const float qw = q * wp[i];
-        const float gg = GATE == kChannel || GATE == kFull ? ag * g[i] : ag;
-        // the column sum leaves out what does not depend on the row (a channel's gate)
-        spost[j][i] = fmaf(q, GATE == kFull ? gg : ag, spost[j][i]);
-        s2[0] = fmaf(qw, gg, s2[0]);
-        if (GATE == kToken) s2[1] += qw;
-        if (GATE == kFull) d[i] = a.alpha * qw;
-      }
-      if (on[j]) {
-        st_stream(a.dh_out, row, a.C, vec[j], E, pack<T>(G[j]));
-        if (GATE == kFull) st_stream(a.dgate, row, a.C, vec[j], E, pack<T>(d));
+      for (int i = 0; i < P; ++i) x[j][i] = 0ull;
+      if (vec < nvec) {
+        f32x2 d[P], wp[P], g[P];
+        unpack2<T>(MODE == kRing ? in.get(2, vec) : dv[j], d);
+        unpack2<T>(MODE == kRing ? in.get(3, vec) : xv[j], x[j]);
+        if constexpr (GATE == kFull) unpack2<T>(MODE == kRing ? in.get(4, vec) : gv[j], g);
+        w.post(vec, wp);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const f32x2 G = f2_fma(t[j][i], rr2, f2_fma(h[j][i], k1, d[i]));
+          f32x2 q = f2_mul(G, x[j][i]);
+          d[i] = G;
+          t[j][i] = f2_mul(G, wp[i]);                          // U
+          if constexpr (GATE == kFull) {
+            wp[i] = f2_mul(f2_mul(q, wp[i]), kpost);           // dgate (kpost = rstd1 alpha)
+            t[j][i] = f2_mul(t[j][i], g[i]);
+            q = f2_mul(q, g[i]);
+          }
+          spost[j][i] = f2_fma(q, kpost, spost[j][i]);
+          acc = f2_fma(t[j][i], x[j][i], acc);
+        }
+        st_row(a.dh_out, row, in.row_bytes, vec, pack2f<T>(d));
+        if constexpr (GATE == kFull) st_row(a.dgate, row, in.row_bytes, vec, pack2f<T>(wp));
       }
     }
-    row_sum<2, WARP>(s2, scratch, phase);
-    const float c2 = s2[0] * a.inv_c;
-    if (GATE == kToken && lane == 0) ((T*)a.dgate)[row] = from_f32<T>(a.alpha * s2[1]);
+    const float sum = row_sum<MODE>(f2_sum(acc), scratch, phase) * r1;  // sum U xhat
+    in.close(row);
+    if (GATE == kToken && lane == 0) ((T*)a.dgate)[row] = from_f32<T>(a.alpha * sum);
+    const f32x2 ku = f2_splat(r1 * ag), kx = f2_splat(-r1 * r1 * ag * sum * a.inv_c);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float x[N], wp[N], g[N], o[N];
-      unpack<T>(xv[j], x);
-      unpack<T>(wpost[j], wp);
-      if (GATE == kChannel) unpack<T>(gch[j], g);
-      if (GATE == kFull) unpack<T>(gv[j], g);
+      const int vec = lane + j * width;
+      if (vec < nvec) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float gg = GATE == kChannel || GATE == kFull ? ag * g[i] : ag;
-        o[i] = r1 * fmaf(gg * G[j][i], wp[i], -(x[i] * r1 * c2));
+        for (int i = 0; i < P; ++i) t[j][i] = f2_fma(t[j][i], ku, f2_mul(x[j][i], kx));
+        st_row(a.dx, row, in.row_bytes, vec, pack2f<T>(t[j]));
       }
-      if (on[j]) st_stream(a.dx, row, a.C, vec[j], E, pack<T>(o));
     }
   }
+  in.finish();
   // one float32 partial row per block
-  float* pre = a.partial + (int64_t)blockIdx.x * a.C;
-  float* post = a.partial + ((int64_t)gridDim.x + blockIdx.x) * a.C;
-  if constexpr (!WARP) {
+  f32x2* pre = reinterpret_cast<f32x2*>(a.partial + (int64_t)blockIdx.x * a.C);
+  f32x2* post = reinterpret_cast<f32x2*>(a.partial + ((int64_t)gridDim.x + blockIdx.x) * a.C);
+  if constexpr (MODE != kWarp) {
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (on[j])
+    for (int j = 0; j < V; ++j) {
+      const int vec = lane + j * width;
+      if (vec < nvec)
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-          *reinterpret_cast<float4*>(pre + vec[j] * N + i) = make_float4(spre[j][i], spre[j][i + 1], spre[j][i + 2], spre[j][i + 3]);
-          *reinterpret_cast<float4*>(post + vec[j] * N + i) = make_float4(spost[j][i], spost[j][i + 1], spost[j][i + 2], spost[j][i + 3]);
+        for (int i = 0; i < P; ++i) {
+          pre[vec * P + i] = spre[j][i];
+          post[vec * P + i] = spost[j][i];
         }
+    }
   } else {
-    const int C = (int)a.C;  // at most 64 vectors
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) {  // the warps' rows in warp order
-      if ((int)threadIdx.x / 32 == w) {
+    const int pairs = (int)a.C / 2;  // at most 64 vectors
+    f32x2* fold = reinterpret_cast<f32x2*>(dyn) + pairs * 2;  // behind the weights
+    for (int wi = 0; wi < (int)blockDim.x / 32; ++wi) {  // the warps' rows in warp order
+      if ((int)threadIdx.x / 32 == wi) {
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (on[j])
+        for (int j = 0; j < V; ++j) {
+          const int vec = lane + j * width;
+          if (vec < nvec)
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-              float* f = fold + vec[j] * N + i;
-              f[0] = w ? f[0] + spre[j][i] : spre[j][i];
-              f[C] = w ? f[C] + spost[j][i] : spost[j][i];
+            for (int i = 0; i < P; ++i) {
+              f32x2* f = fold + vec * P + i;
+              f[0] = wi ? f2_add(f[0], spre[j][i]) : spre[j][i];
+              f[pairs] = wi ? f2_add(f[pairs], spost[j][i]) : spost[j][i];
             }
+        }
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < C; c += blockDim.x) {
+    for (int c = threadIdx.x; c < pairs; c += blockDim.x) {
       pre[c] = fold[c];
-      post[c] = fold[C + c];
+      post[c] = fold[pairs + c];
     }
   }
 }
@@ -420,31 +613,50 @@ post_pre_columns_kernel(const float* __restrict__ partial, int blocks, int64_t C
 }
 
 // ---------------------------------------------------------------- host side
+int read_post_pre_status(int reset) {
+  int code = 0;
+  if (cudaMemcpyFromSymbol(&code, g_post_pre_device_status, sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();
+    return -1;
+  }
+  if (reset && code != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_post_pre_device_status, &zero, sizeof(int));
+  }
+  return code;
+}
+const bool g_post_pre_registered = (register_device_status(read_post_pre_status), true);
+
 struct Shape {
-  bool any;   // the kernels without vectors
-  bool warp;  // a warp per row
-  int V, threads;
+  bool any;  // the kernels without vectors
+  int mode, V, threads, stages;
 };
-// Vectors per thread: two from 257 vectors on (half the threads share each row's two
-// reductions), four above 2048; a warp per row up to 64 vectors.
-Shape pick_shape(int64_t C, size_t elem, bool aligned) {
+// Two vectors per thread from 257 vectors on (half the threads share each row's two
+// reductions), four above 1024; a warp per row up to 64 vectors; rows of more than 2048
+// vectors, or off a 16-byte boundary, take the kernels without vectors. `arrays`: rows
+// read per row.
+Shape pick_shape(int64_t C, size_t elem, bool aligned, int arrays) {
   Shape s{};
+  s.threads = kAnyThreads;
   if (!aligned || (C * elem) % 16 != 0 || C * elem / 16 > 2048) {
     s.any = true;
-    s.threads = kAnyThreads;
     return s;
   }
   const int nvec = (int)(C * elem / 16);
   if (nvec <= 64) {
-    s.warp = true;
+    s.mode = kWarp;
     s.V = nvec <= 32 ? 1 : 2;
     s.threads = 256;
     return s;
   }
-  s.V = nvec <= 256 ? 1 : nvec <= 1024 ? 2 : 1;
-  s.threads = (nvec + s.V - 1) / s.V;
-  s.threads = (s.threads + 31) / 32 * 32;
-  if (s.threads > 1024) { s.any = true; s.threads = kAnyThreads; }
+  s.V = nvec <= 256 ? 1 : nvec <= 1024 ? 2 : 4;
+  s.threads = ((nvec + s.V - 1) / s.V + 31) / 32 * 32;
+  // stages: as many as leave two blocks on an SM, or two in all
+  const int64_t room = device_info().max_smem_optin - 2048, stage = (int64_t)arrays * C * elem;
+  const int64_t two_blocks = (room / 2 - 2 * C * 4) / stage, one_block = (room - 2 * C * 4) / stage;
+  s.stages = (int)(two_blocks >= 2 ? two_blocks : one_block);
+  if (s.stages > kMaxStages) s.stages = kMaxStages;
+  s.mode = s.stages >= 2 && s.V <= 2 ? kRing : kDirect;
   return s;
 }
 // Most blocks a backward launches, and with that partial rows.
@@ -459,35 +671,52 @@ int blocks_for(Kernel kernel, const Shape& s, int64_t rows, size_t smem) {
   }
   if (occ < 1) occ = 1;
   int64_t n = (int64_t)device_info().sm_count * occ;
-  const int64_t per = s.warp ? s.threads / 32 : 1;
+  const int64_t per = !s.any && s.mode == kWarp ? s.threads / 32 : 1;
   const int64_t need = (rows + per - 1) / per;
   if (n > need) n = need;
   if (n > most_blocks()) n = most_blocks();
   return (int)(n < 1 ? 1 : n);
 }
 
-template <typename T, int V, int GATE, bool WARP>
-int launch_fwd(const NormArgs& a, const Shape& s, cudaStream_t st) {
-  auto k = post_pre_fwd_kernel<T, V, GATE, WARP>;
-  k<<<blocks_for(k, s, a.rows, 0), s.threads, 0, st>>>(a);
-  return check_launch("post_pre_norm_fwd");
-}
-template <typename T, int V, int GATE, bool WARP>
-int launch_bwd(const NormArgs& a, const Shape& s, cudaStream_t st, int& blocks) {
-  auto k = post_pre_bwd_kernel<T, V, GATE, WARP>;
-  const size_t smem = WARP ? 2 * a.C * sizeof(float) : 0;
-  blocks = blocks_for(k, s, a.rows, smem);
-  k<<<blocks, s.threads, smem, st>>>(a);
-  return check_launch("post_pre_norm_bwd");
+template <typename Kernel>
+int launch_rows(const char* what, Kernel kernel, const NormArgs& a, const Shape& s, size_t smem,
+                cudaStream_t st, int& blocks) {
+  // (the limit without the attribute, 48 KB, includes the static part)
+  if (smem > 32 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)smem) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(EVG_ELAUNCH, "%s: cannot reserve %zu bytes of shared memory", what, smem);
+  }
+  blocks = blocks_for(kernel, s, a.rows, smem);
+  kernel<<<blocks, s.threads, smem, st>>>(a);
+  return check_launch(what);
 }
 
-#define EVG_PP_GATES(call)                          \
-  switch (gate) {                                   \
-    case kNone: return call(kNone);                 \
-    case kChannel: return call(kChannel);           \
-    case kToken: return call(kToken);               \
-    default: return call(kFull);                    \
+template <typename T, int V, int MODE>
+int launch_fwd(const NormArgs& a, int gate, const Shape& s, cudaStream_t st) {
+  const size_t smem = MODE == kDirect ? 0 : ring_bytes(MODE == kRing ? s.stages : 0, gate == kFull ? 3 : 2, a.C, sizeof(T));
+  const char* what = "post_pre_norm_fwd";
+  int blocks;
+  switch (gate) {
+    case kNone: return launch_rows(what, post_pre_fwd_kernel<T, V, kNone, MODE>, a, s, smem, st, blocks);
+    case kChannel: return launch_rows(what, post_pre_fwd_kernel<T, V, kChannel, MODE>, a, s, smem, st, blocks);
+    case kToken: return launch_rows(what, post_pre_fwd_kernel<T, V, kToken, MODE>, a, s, smem, st, blocks);
+    default: return launch_rows(what, post_pre_fwd_kernel<T, V, kFull, MODE>, a, s, smem, st, blocks);
   }
+}
+template <typename T, int V, int MODE>
+int launch_bwd(const NormArgs& a, int gate, const Shape& s, cudaStream_t st, int& blocks) {
+  const size_t smem = MODE == kDirect ? 0
+                      : MODE == kWarp ? 4 * a.C * sizeof(float)
+                                      : ring_bytes(s.stages, gate == kFull ? 5 : 4, a.C, sizeof(T));
+  const char* what = "post_pre_norm_bwd";
+  switch (gate) {
+    case kNone: return launch_rows(what, post_pre_bwd_kernel<T, V, kNone, MODE>, a, s, smem, st, blocks);
+    case kChannel: return launch_rows(what, post_pre_bwd_kernel<T, V, kChannel, MODE>, a, s, smem, st, blocks);
+    case kToken: return launch_rows(what, post_pre_bwd_kernel<T, V, kToken, MODE>, a, s, smem, st, blocks);
+    default: return launch_rows(what, post_pre_bwd_kernel<T, V, kFull, MODE>, a, s, smem, st, blocks);
+  }
+}
 
 template <typename T>
 int run_fwd(const NormArgs& a, int gate, const Shape& s, cudaStream_t st) {
@@ -495,24 +724,9 @@ int run_fwd(const NormArgs& a, int gate, const Shape& s, cudaStream_t st) {
     post_pre_fwd_any_kernel<T><<<blocks_for(post_pre_fwd_any_kernel<T>, s, a.rows, 0), s.threads, 0, st>>>(a, gate);
     return check_launch("post_pre_norm_fwd");
   }
-  if (s.warp && s.V == 1) {
-#define EVG_PP(g) launch_fwd<T, 1, g, true>(a, s, st)
-    EVG_PP_GATES(EVG_PP)
-#undef EVG_PP
-  }
-  if (s.warp) {
-#define EVG_PP(g) launch_fwd<T, 2, g, true>(a, s, st)
-    EVG_PP_GATES(EVG_PP)
-#undef EVG_PP
-  }
-  if (s.V == 1) {
-#define EVG_PP(g) launch_fwd<T, 1, g, false>(a, s, st)
-    EVG_PP_GATES(EVG_PP)
-#undef EVG_PP
-  }
-#define EVG_PP(g) launch_fwd<T, 2, g, false>(a, s, st)
-  EVG_PP_GATES(EVG_PP)
-#undef EVG_PP
+  if (s.mode == kWarp) return s.V == 1 ? launch_fwd<T, 1, kWarp>(a, gate, s, st) : launch_fwd<T, 2, kWarp>(a, gate, s, st);
+  if (s.mode == kRing) return s.V == 1 ? launch_fwd<T, 1, kRing>(a, gate, s, st) : launch_fwd<T, 2, kRing>(a, gate, s, st);
+  return s.V == 2 ? launch_fwd<T, 2, kDirect>(a, gate, s, st) : launch_fwd<T, 4, kDirect>(a, gate, s, st);
 }
 
 template <typename T>
@@ -522,24 +736,11 @@ int run_bwd_rows(const NormArgs& a, int gate, const Shape& s, cudaStream_t st, i
     post_pre_bwd_any_kernel<T><<<blocks, s.threads, 0, st>>>(a, gate);
     return check_launch("post_pre_norm_bwd");
   }
-  if (s.warp && s.V == 1) {
-#define EVG_PP(g) launch_bwd<T, 1, g, true>(a, s, st, blocks)
-    EVG_PP_GATES(EVG_PP)
-#undef EVG_PP
-  }
-  if (s.warp) {
-#define EVG_PP(g) launch_bwd<T, 2, g, true>(a, s, st, blocks)
-    EVG_PP_GATES(EVG_PP)
-#undef EVG_PP
-  }
-  if (s.V == 1) {
-#define EVG_PP(g) launch_bwd<T, 1, g, false>(a, s, st, blocks)
-    EVG_PP_GATES(EVG_PP)
-#undef EVG_PP
-  }
-#define EVG_PP(g) launch_bwd<T, 2, g, false>(a, s, st, blocks)
-  EVG_PP_GATES(EVG_PP)
-#undef EVG_PP
+  if (s.mode == kWarp)
+    return s.V == 1 ? launch_bwd<T, 1, kWarp>(a, gate, s, st, blocks) : launch_bwd<T, 2, kWarp>(a, gate, s, st, blocks);
+  if (s.mode == kRing)
+    return s.V == 1 ? launch_bwd<T, 1, kRing>(a, gate, s, st, blocks) : launch_bwd<T, 2, kRing>(a, gate, s, st, blocks);
+  return s.V == 2 ? launch_bwd<T, 2, kDirect>(a, gate, s, st, blocks) : launch_bwd<T, 4, kDirect>(a, gate, s, st, blocks);
 }
 
 int check_norm_args(const char* what, int64_t rows, int64_t C, int gate, float alpha, int dtype) {
@@ -573,7 +774,8 @@ extern "C" int evg_post_pre_norm_fwd(const void* x, const void* h, const void* w
   bool aligned = true;
   for (const void* p : {x, h, w_post, w_pre, (const void*)h_out, (const void*)y}) aligned = aligned && aligned16(p);
   if (gate_kind == kChannel || gate_kind == kFull) aligned = aligned && aligned16(gate);
-  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned);
+  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned, gate_kind == kFull ? 3 : 2);
+  a.stages = s.stages;
   return EVG_DISPATCH_DTYPE(dtype, [&] { return run_fwd<T>(a, gate_kind, s, (cudaStream_t)stream); });
 }
 
@@ -610,7 +812,8 @@ extern "C" int evg_post_pre_norm_bwd(const void* dy, const void* dh, const void*
   for (const void* p : {dy, dh, x, h_out, w_post, w_pre, (const void*)dx, (const void*)dres}) aligned = aligned && aligned16(p);
   if (gate_kind == kChannel) aligned = aligned && aligned16(gate);
   if (gate_kind == kFull) aligned = aligned && aligned16(gate) && aligned16(dgate);
-  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned);
+  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned, gate_kind == kFull ? 5 : 4);
+  a.stages = s.stages;
   cudaStream_t st = (cudaStream_t)stream;
   return EVG_DISPATCH_DTYPE(dtype, [&] {
     int blocks = 0;

@@ -83,8 +83,14 @@ def test_shapes_strides_and_empty():
     # a gate broadcast over rows by its strides is one of full width
     gate = t["wp"].expand(24, 64)
     hf, yf, *_ = ops.post_pre_norm_fwd(t["x"], t["h"], t["wp"], t["wn"], gate)
-    hc, yc, *_ = ops.post_pre_norm_fwd(t["x"], t["h"], t["wp"], t["wn"], t["wp"])
-    assert torch.allclose(hf, hc, rtol=1e-6) and torch.allclose(yf, yc, rtol=1e-5)
+    hc, yc, _, rc = ops.post_pre_norm_fwd(t["x"], t["h"], t["wp"], t["wn"], t["wp"])
+    # n = x (w g) rstd or (x w) g rstd: at most five float32 roundings each way, relative to
+    # n and not to the sum h + n, which can cancel; the sum rounds once more. y is off by
+    # that times rstd w, and by its own roundings and the rstd's (a sum of 64 squares).
+    n = hc - t["h"]
+    off = 10 * 2.0 ** -24 * n.abs() + 2 * 2.0 ** -24 * hc.abs()
+    assert bool(((hf - hc).abs() <= off).all())
+    assert bool(((yf - yc).abs() <= off * (rc[:, None] * t["wn"]).abs() + 1e-5 * yc.abs()).all())
     # tensors that start off a 16-byte boundary take the kernels without vectors
     buf = torch.zeros(24 * 64 + 1, device="cuda")
     off = buf[1:].view(24, 64)
