@@ -67,8 +67,11 @@ struct BwdParams {
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-__device__ __forceinline__ void red_add_f32(float* addr, float v) {
-  asm volatile("red.global.add.f32 [%0], %1;" ::"l"(addr), "f"(v) : "memory");
+__device__ __forceinline__ void red_add_f32x4(float* addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(addr),
+               "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)),
+               "f"(__uint_as_float(d))
+               : "memory");
 }
 __device__ __forceinline__ uint8_t* view_row(const View& v, int64_t token, int head) {
   return reinterpret_cast<uint8_t*>(v.p) + (token * v.st + (int64_t)head * v.sh) * 2;
@@ -346,8 +349,7 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     int it = 0, head = bh * p.group;
     for (int c = 0; c < n_git; ++c) {
       const uint32_t par = (uint32_t)(c & 1);
-      const int rows = (it == n_it - 1) ? tail_rows : kTile;  // queries of this tile
-      float* tile_dst = p.dq_acc + (head * P + prow0 + (int64_t)it * kTile) * HD + r.row;
+      float* tile_dst = p.dq_acc + (head * P + prow0 + (int64_t)it * kTile) * HD + r.row * 4;
 #pragma unroll
       for (int ch = 0; ch < 2; ++ch) {
         mbar_wait(dq_full + ch, par, ctx, 841);
@@ -359,16 +361,11 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
         tmem_wait_ld();
         warp_arrive(d_free + ch, r.lane);
         float* dst = tile_dst + ch * 64 * HD;
-        const int n = rows - ch * 64;
         if (r.row < p.D) {
-          if (n >= 64) {
 #pragma unroll
-            for (int j = 0; j < 64; ++j) red_add_f32(dst + j * HD, __uint_as_float(acc[j >> 5][j & 31]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (j < n) red_add_f32(dst + j * HD, __uint_as_float(acc[j >> 5][j & 31]));
-          }
+          for (int j = 0; j < 64; j += 4)
+            red_add_f32x4(dst + j * HD, acc[j >> 5][j & 31], acc[j >> 5][(j & 31) + 1],
+                          acc[j >> 5][(j & 31) + 2], acc[j >> 5][(j & 31) + 3]);
         }
       }
       if (++it == n_it) { it = 0; ++head; }
@@ -528,6 +525,8 @@ packed_prepare_kernel(const View dout, const View o, const float* __restrict__ l
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += af[i] * bf[i];
       }
+    }
+    {
       uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (prow0 + r) * HD + part * 8);
       acc[0] = acc[1] = make_uint4(0, 0, 0, 0);
     }
@@ -540,12 +539,13 @@ packed_prepare_kernel(const View dout, const View o, const float* __restrict__ l
   }
 }
 
-// dq = round(scale * float32 copy), zero behind the last sequence.
+// dq = round(scale * float32 copy), zero behind the last sequence. The copy of a tile is
+// laid out [query / 4][head column][query % 4]: a thread takes 4 queries x 8 columns.
 template <int HD, int FMT>
 __global__ void __launch_bounds__(256)
 packed_finish_kernel(const BwdParams p) {
   constexpr int TPR = HD / 8;
-  constexpr int ROWS = 256 / TPR;
+  constexpr int QUADS = 256 / TPR;  // groups of 4 queries per round
   const int4 item = plan_item(p.plan, blockIdx.x);
   if (item.z < 0) return;
   const int head = blockIdx.y;
@@ -554,17 +554,29 @@ packed_finish_kernel(const BwdParams p) {
   const int tile0 = item.z > 0 ? (item.z - 1) * kTile : 0;
   const int rows = min(kTile, item.y - tile0);
   const int64_t prow0 = (int64_t)head * p.slots * kTile + (int64_t)item.w * kTile + tile0;
-  for (int r = threadIdx.x / TPR + blockIdx.z * ROWS; r < rows; r += ROWS * gridDim.z) {
-    uint4 pk = make_uint4(0, 0, 0, 0);
+  for (int qd = threadIdx.x / TPR + blockIdx.z * QUADS; qd * 4 < rows; qd += QUADS * gridDim.z) {
+    float v[4][8];
     if (item.z > 0) {
-      const float4* src = reinterpret_cast<const float4*>(p.dq_acc + (prow0 + r) * HD + part * 8);
-      const float4 a = __ldcs(src), b = __ldcs(src + 1);
-      pk.x = pack2<FMT>(a.x * p.scale, a.y * p.scale);
-      pk.y = pack2<FMT>(a.z * p.scale, a.w * p.scale);
-      pk.z = pack2<FMT>(b.x * p.scale, b.y * p.scale);
-      pk.w = pack2<FMT>(b.z * p.scale, b.w * p.scale);
+      const float4* src = reinterpret_cast<const float4*>(p.dq_acc + (prow0 + qd * 4) * HD) + part * 8;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float4 f = __ldcs(src + c);
+        v[0][c] = f.x; v[1][c] = f.y; v[2][c] = f.z; v[3][c] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[0][c] = v[1][c] = v[2][c] = v[3][c] = 0.f;
     }
-    *reinterpret_cast<uint4*>(view_row(p.dq, item.x + tile0 + r, head) + part * 16) = pk;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (qd * 4 + i < rows) {
+        uint4 pk;
+        pk.x = pack2<FMT>(v[i][0] * p.scale, v[i][1] * p.scale);
+        pk.y = pack2<FMT>(v[i][2] * p.scale, v[i][3] * p.scale);
+        pk.z = pack2<FMT>(v[i][4] * p.scale, v[i][5] * p.scale);
+        pk.w = pack2<FMT>(v[i][6] * p.scale, v[i][7] * p.scale);
+        *reinterpret_cast<uint4*>(view_row(p.dq, item.x + tile0 + qd * 4 + i, head) + part * 16) = pk;
+      }
   }
 }
 
