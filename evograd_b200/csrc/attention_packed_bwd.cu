@@ -5,29 +5,36 @@
 //
 // One pass over the visible tiles, five products per (key tile, query tile). A block
 // owns one key tile of one k/v head and walks the query tiles behind it, for every
-// query head of the group, in chunks of 64 queries:
+// query head of the group. A tile's two halves of 64 queries are two streams:
 //   S^T   = K Q_i^T                 [128 keys x 128 queries], once per tile
-//   dP^T  = V dO^T                  [128 keys x 64 queries]
+//   dP^T  = V dO^T                  [128 keys x 64 queries] per stream
 //   P^T, dS^T in registers, then 16 bits back into tensor memory over dP^T
 //   dV   += P^T dO,  dK += dS^T Q   (A from tensor memory)
-//   dQ^T  = K^T dS^T                [128 head columns x 64 queries]
-// dK and dV stay in tensor memory until the end (fixed order, no atomics). dQ^T also
-// belongs to other blocks' rows: four warps of their own add it to a float32 copy of
-// dQ (one 128-byte line per warp instruction), so dq can differ in the last bit from
-// run to run; a last kernel scales and rounds the copy.
+//   dQ^T  = K^T dS^T                [128 head columns x 64 queries], over P^T and dS^T
+// Each stream has eight compute warps and tensor-memory columns of its own, so that one
+// stream's exponentials and dS run under the other stream's products; with one set of
+// sixteen warps on one chunk after the other, the chain products -> warps -> products
+// took 6200 cycles per tile pair. dK and dV stay in tensor memory until the end (fixed
+// order, no atomics). dQ^T also belongs to other blocks' rows: four warps of their own
+// add it to a float32 copy of dQ, so dq can differ in the last bit from run to run; a
+// last kernel scales and rounds the copy.
 //
-// Tensor memory: S^T [0,128), dP^T / P^T / dS^T of the chunk [128,192), dQ^T of the
-// chunk [192,256), dV [256,256+HD), dK [384,384+HD). Shared memory: K, V, two dO and
-// two Q stages, two 16 KB dS^T chunks, row statistics (226 KB at head size 128).
-// At head size 64 the dQ^T product keeps its 128 rows: the A operand's second 64
-// columns are the V tile, which follows K in shared memory, and the rows they give
-// are not read (a 64-row product has another layout in tensor memory).
+// Order of the products for tile c (numbers in brackets: the stream):
+//   S(c+1)  dP(c)[1]  dV,dK(c)[0]  dQ(c)[0]  dV,dK(c)[1]  dP(c+1)[0]  dQ(c)[1]
+// The tensor pipe runs in order, so every wait of the issuing warp sits behind products
+// that hide it: dP of a stream has to wait until the stream's last dQ^T has been taken
+// out of the columns they share, and runs behind the other stream's dV, dK or the next
+// scores.
+//
+// Tensor memory: S^T [0,128), streams' dP^T / P^T / dS^T / dQ^T [128,192) and [192,256),
+// dV [256,256+HD), dK [384,384+HD). Shared memory: K, V, two dO and two Q stages, two
+// 16 KB dS^T halves, row statistics (226 KB at head size 128). At head size 64 the dQ^T
+// product keeps its 128 rows: the A operand's second 64 columns are the V tile, which
+// follows K in shared memory, and the rows they give are not read (a 64-row product has
+// another layout in tensor memory).
 //
 // Tiles start at the sequence's first token; rows of K, V, Q and dO behind its end are
 // other tokens and are zeroed in shared memory, and their statistics make P zero.
-//
-// Bound: the dependent chain products -> compute warps -> products through
-// single-buffered tensor memory, and the L2's float32 adders for dQ.
 #include "attention_bwd_parts.cuh"
 #include "packed.cuh"
 
@@ -42,9 +49,11 @@ using namespace attn;
 using namespace attn_bwd;
 using namespace packed;
 
-constexpr int kCG = 4;  // column groups of compute warps
-// TMA warp, MMA warp, 16 compute warps, 4 warps that take dQ^T out of tensor memory
-constexpr int kBwdThreads = 64 + 128 * kCG + 128;
+constexpr int kComputeWarps = 16;  // two streams of eight
+constexpr int kStreamWarps = 8;
+constexpr int kCG = 4;             // column groups of compute warps in the final stores
+// TMA warp, MMA warp, compute warps, 4 warps that take dQ^T out of tensor memory
+constexpr int kBwdThreads = 32 * (2 + kComputeWarps + 4);
 constexpr uint32_t kChunkBytes = 64 * 128 * 2;  // 64 queries x 128 keys of 16-bit dS^T
 constexpr uint32_t kStatBytes = 2048;
 
@@ -112,8 +121,6 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ CUtensorMap map_do, const BwdParams p) {
-  constexpr int CG = kCG;
-  constexpr int CPW = 64 / CG;  // query columns of a chunk per compute warp (16)
   // Key tile n - w of a sequence of n tiles: w query tiles to visit, heaviest first.
   int slot, bh;
   map_block(blockIdx.x, p.slots, p.units, p.head_group, slot, bh);
@@ -159,13 +166,13 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   uint64_t* do_empty = bs.bars + 7;  // [2]
   uint64_t* s_full = bs.bars + 9;
   uint64_t* x_free = bs.bars + 10;
-  uint64_t* dp_full = bs.bars + 11;   // [2] by chunk parity
-  uint64_t* pds_full = bs.bars + 13;  // [2] P^T / dS^T of the chunk are in Y
-  uint64_t* ds_full = bs.bars + 15;   // [2] dS^T of the chunk is in shared memory
-  uint64_t* dq_full = bs.bars + 17;   // [2] dQ^T of the chunk is in D
-  uint64_t* d_free = bs.bars + 19;    // [2] D has been read
+  uint64_t* dp_full = bs.bars + 11;   // [2] by stream, as all below
+  uint64_t* pds_full = bs.bars + 13;  // [2] P^T / dS^T are in Y
+  uint64_t* ds_full = bs.bars + 15;   // [2] dS^T is in shared memory
+  uint64_t* dq_full = bs.bars + 17;   // [2] dQ^T is in Y
+  uint64_t* d_free = bs.bars + 19;    // [2] dQ^T has been read
   uint64_t* done = bs.bars + 21;
-  const Roles r = roles();  // r.half is the warp's column group, 0 .. CG-1
+  const Roles r = roles();
   const float scale_log2 = p.scale * kLog2e;
 
   if (threadIdx.x == 0) {
@@ -174,10 +181,10 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1); mbar_init(q_empty + i, 1);
       mbar_init(do_full + i, 1); mbar_init(do_empty + i, 1);
-      mbar_init(dp_full + i, 1); mbar_init(pds_full + i, 4 * CG);
-      mbar_init(ds_full + i, 4 * CG); mbar_init(dq_full + i, 1); mbar_init(d_free + i, 4);
+      mbar_init(dp_full + i, 1); mbar_init(pds_full + i, kStreamWarps);
+      mbar_init(ds_full + i, kStreamWarps); mbar_init(dq_full + i, 1); mbar_init(d_free + i, 4);
     }
-    mbar_init(s_full, 1); mbar_init(x_free, 4 * CG);
+    mbar_init(s_full, 1); mbar_init(x_free, kComputeWarps);
     fence_mbar_init();
     prefetch_tensormap(&map_q); prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v); prefetch_tensormap(&map_do);
@@ -193,7 +200,7 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   constexpr uint32_t idesc_p = instr_desc_f16(FMT, 128, 64, 0, 0);
   constexpr uint32_t idesc_d = instr_desc_f16(FMT, 128, HD, 0, 1);
   constexpr uint32_t idesc_q = instr_desc_f16(FMT, 128, 64, 1, 1);
-  const uint32_t tX = tmem, tY = tmem + 128, tD = tmem + 192;
+  const uint32_t tX = tmem, tY0 = tmem + 128;  // stream b: tY0 + 64 b
   const uint32_t tDV = tmem + 256, tDK = tmem + 384;
 
   if (r.is_tma && r.lane == 0) {
@@ -231,43 +238,43 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     const bool lead = elect_one();
     const DescBase v_base = desc_base_kmajor(smem_u32(sV));
     const DescBase kt_base = desc_base_mnmajor(smem_u32(sK), kTile);
-    // dP^T of query chunk ch: B operand = rows [64 ch, 64 ch + 64) of a dO tile.
-    auto issue_dp = [&](int ch, uint32_t do_saddr) {
-      const DescBase da = desc_base_kmajor(do_saddr + ch * 64 * 128);
+    // dP^T of stream b: B operand = rows [64 b, 64 b + 64) of a dO tile.
+    auto issue_dp = [&](int b, uint32_t do_saddr) {
+      const DescBase da = desc_base_kmajor(do_saddr + b * 64 * 128);
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
         if (lead)
-          mma_ss(tY, desc_at(v_base, kstep_kmajor(kTile, ks)), desc_at(da, kstep_kmajor(kTile, ks)),
-                 idesc_p, ks > 0 ? 1u : 0u);
-      if (lead) mma_commit(dp_full + ch);
+          mma_ss(tY0 + 64 * b, desc_at(v_base, kstep_kmajor(kTile, ks)),
+                 desc_at(da, kstep_kmajor(kTile, ks)), idesc_p, ks > 0 ? 1u : 0u);
+      if (lead) mma_commit(dp_full + b);
     };
-    // Query k-step kk of the chunk (16 queries): P^T in Y columns [16 kk, 16 kk + 8),
+    // Query k-step kk of the stream (16 queries): P^T in its columns [16 kk, 16 kk + 8),
     // dS^T in the 8 columns behind it (the layout the compute warps write).
-    auto issue_dv = [&](int ch, uint32_t do_saddr, bool first) {
-      const DescBase dob = desc_base_mnmajor(do_saddr + ch * 64 * 128, kTile);
+    auto issue_dv = [&](int b, uint32_t do_saddr, bool first) {
+      const DescBase dob = desc_base_mnmajor(do_saddr + b * 64 * 128, kTile);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
         if (lead)
-          mma_ts(tDV, tY + kk * CPW, desc_at(dob, kstep_mnmajor(kk)), idesc_d,
+          mma_ts(tDV, tY0 + 64 * b + kk * 16, desc_at(dob, kstep_mnmajor(kk)), idesc_d,
                  (first && kk == 0) ? 0u : 1u);
     };
-    auto issue_dk = [&](int ch, uint32_t q_saddr, bool first) {
-      const DescBase qb = desc_base_mnmajor(q_saddr + ch * 64 * 128, kTile);
+    auto issue_dk = [&](int b, uint32_t q_saddr, bool first) {
+      const DescBase qb = desc_base_mnmajor(q_saddr + b * 64 * 128, kTile);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
         if (lead)
-          mma_ts(tDK, tY + kk * CPW + CPW / 2, desc_at(qb, kstep_mnmajor(kk)), idesc_d,
+          mma_ts(tDK, tY0 + 64 * b + kk * 16 + 8, desc_at(qb, kstep_mnmajor(kk)), idesc_d,
                  (first && kk == 0) ? 0u : 1u);
     };
-    // dQ^T of chunk ch: A = K^T (the K tile read MN-major), B = dS^T chunk.
-    auto issue_dq = [&](int ch) {
-      const DescBase dsb = desc_base_mnmajor(smem_u32(sDS) + ch * kChunkBytes, kTile);
+    // dQ^T of stream b over its P^T / dS^T: A = K^T (the K tile read MN-major), B = dS^T.
+    auto issue_dq = [&](int b) {
+      const DescBase dsb = desc_base_mnmajor(smem_u32(sDS) + b * kChunkBytes, kTile);
 #pragma unroll
       for (int ks = 0; ks < kTile / 16; ++ks)
         if (lead)
-          mma_ss(tD, desc_at(kt_base, kstep_mnmajor(ks)), desc_at(dsb, kstep_mnmajor(ks)), idesc_q,
-                 ks > 0 ? 1u : 0u);
-      if (lead) mma_commit(dq_full + ch);
+          mma_ss(tY0 + 64 * b, desc_at(kt_base, kstep_mnmajor(ks)), desc_at(dsb, kstep_mnmajor(ks)),
+                 idesc_q, ks > 0 ? 1u : 0u);
+      if (lead) mma_commit(dq_full + b);
     };
     // Query iteration `it` reads the sequence's last tile: its rows behind the end are zeroed.
     auto clear_tail = [&](uint8_t* tile, int it) {
@@ -287,6 +294,7 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     clear_tail(sDO0, 0);
     tc_fence_after_sync();
     issue_dp(0, smem_u32(sDO0));
+    issue_dp(1, smem_u32(sDO0));
     int it1 = 0;  // query tile of iteration c + 1
     for (int c = 0; c < n_git; ++c) {
       const int st = c & 1, st1 = st ^ 1;
@@ -294,21 +302,6 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
       const bool more = c + 1 < n_git;
       const uint32_t do_saddr = smem_u32(sDO0 + st * TB), q_saddr = smem_u32(sQ0 + st * TB);
       if (++it1 == n_it) it1 = 0;
-      // One wait on the critical path per chunk (P^T / dS^T are ready), with the
-      // waits that are normally satisfied long before ahead of it. dQ^T runs one
-      // chunk behind, so its operand and its place in D are ready by the time it is
-      // issued.
-      // chunk 0
-      if (c > 0) {
-        mbar_wait(d_free + 0, par ^ 1u, ctx, 826);
-        mbar_wait(ds_full + 1, par ^ 1u, ctx, 825);
-      }
-      mbar_wait(pds_full + 0, par, ctx, 824);
-      tc_fence_after_sync();
-      issue_dv(0, do_saddr, c == 0);
-      issue_dk(0, q_saddr, c == 0);
-      issue_dp(1, do_saddr);
-      if (c > 0) issue_dq(1);  // of tile c - 1
       if (more) {
         mbar_wait(q_full + st1, par1, ctx, 827);
         clear_tail(sQ0 + st1 * TB, it1);
@@ -317,50 +310,56 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
         issue_scores<HD>(lead, tX, smem_u32(sK), smem_u32(sQ0 + st1 * TB), idesc_s);
         if (lead) mma_commit(s_full);
       }
-      // chunk 1
-      if (c > 0) mbar_wait(d_free + 1, par ^ 1u, ctx, 835);
-      mbar_wait(ds_full + 0, par, ctx, 834);
-      if (more) {
-        mbar_wait(do_full + st1, par1, ctx, 833);
-        clear_tail(sDO0 + st1 * TB, it1);
+      if (c > 0) {
+        mbar_wait(d_free + 1, par ^ 1u, ctx, 826);
+        tc_fence_after_sync();
+        issue_dp(1, do_saddr);
       }
+      mbar_wait(pds_full + 0, par, ctx, 824);
+      tc_fence_after_sync();
+      issue_dv(0, do_saddr, c == 0);
+      issue_dk(0, q_saddr, c == 0);
+      mbar_wait(ds_full + 0, par, ctx, 825);
+      tc_fence_after_sync();
+      issue_dq(0);
       mbar_wait(pds_full + 1, par, ctx, 829);
       tc_fence_after_sync();
       issue_dv(1, do_saddr, false);
       if (lead) mma_commit(do_empty + st);
       issue_dk(1, q_saddr, false);
       if (lead) mma_commit(q_empty + st);
-      if (more) issue_dp(0, smem_u32(sDO0 + st1 * TB));
-      issue_dq(0);
-      __syncwarp();
-    }
-    {
-      const uint32_t last = (uint32_t)((n_git - 1) & 1);
-      mbar_wait(d_free + 0, last, ctx, 836);
-      mbar_wait(ds_full + 1, last, ctx, 837);
+      if (more) {
+        mbar_wait(do_full + st1, par1, ctx, 833);
+        clear_tail(sDO0 + st1 * TB, it1);
+        mbar_wait(d_free + 0, par, ctx, 835);
+        tc_fence_after_sync();
+        issue_dp(0, smem_u32(sDO0 + st1 * TB));
+      }
+      mbar_wait(ds_full + 1, par, ctx, 834);
       tc_fence_after_sync();
       issue_dq(1);
+      __syncwarp();
     }
     if (lead) mma_commit(done);
-  } else if (r.warp >= 2 + 4 * CG) {
-    // dQ^T of every chunk: this warp's 32 lanes (head columns) x 64 query columns of D,
-    // one 128-byte line of the float32 dQ copy per warp instruction.
+  } else if (r.warp >= 2 + kComputeWarps) {
+    // dQ^T of every half tile: this warp's 32 lanes (head columns) x 64 query columns,
+    // added to the float32 copy four queries at a time (16 bytes per lane, 512 per warp).
     const uint32_t lane_base = (uint32_t)(r.quarter * 32) << 16;
     int it = 0, head = bh * p.group;
     for (int c = 0; c < n_git; ++c) {
       const uint32_t par = (uint32_t)(c & 1);
       float* tile_dst = p.dq_acc + (head * P + prow0 + (int64_t)it * kTile) * HD + r.row * 4;
 #pragma unroll
-      for (int ch = 0; ch < 2; ++ch) {
-        mbar_wait(dq_full + ch, par, ctx, 841);
+      for (int b = 0; b < 2; ++b) {
+        mbar_wait(dq_full + b, par, ctx, 841);
         __syncwarp();
         tc_fence_after_sync();
         uint32_t acc[2][32];
-        tmem_ld(tD + lane_base, acc[0]);
-        tmem_ld(tD + lane_base + 32, acc[1]);
+        tmem_ld(tY0 + 64 * b + lane_base, acc[0]);
+        tmem_ld(tY0 + 64 * b + lane_base + 32, acc[1]);
         tmem_wait_ld();
-        warp_arrive(d_free + ch, r.lane);
-        float* dst = tile_dst + ch * 64 * HD;
+        warp_arrive(d_free + b, r.lane);
+        float* dst = tile_dst + b * 64 * HD;
         if (r.row < p.D) {
 #pragma unroll
           for (int j = 0; j < 64; j += 4)
@@ -373,118 +372,111 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   } else if (r.is_compute) {
     const uint32_t lane_base = (uint32_t)(r.quarter * 32) << 16;
     const int kv_pos = kv0 + r.row;
-    const int col0 = r.half * CPW;  // first query column inside a chunk of this warp
-    f32x2 p2[CPW / 2];  // P^T of the chunk that comes next, two query columns per element
-    uint32_t pp[CPW / 2];
+    const int b = (r.warp - 2) / kStreamWarps;               // stream
+    const int col0 = ((r.warp - 2) % kStreamWarps / 4) * 32;  // first query column inside its half tile
+    const uint32_t tY = tY0 + 64 * b + lane_base + col0;
     const f32x2 neg_scale2 = f2_splat(-scale_log2);
-    // P^T of one chunk from 16 columns of X, two columns per packed instruction:
-    // t = lse2 - s c, p = 2^-t. `diag`: queries before the key are masked. When
-    // `release` is set, X is handed back as soon as its columns are in registers.
-    auto exp_chunk = [&](uint32_t x_col, const float* lse_ptr, bool diag, int q_first, bool release) {
-      uint32_t sr[CPW];
-      tmem_ld(tX + lane_base + x_col, sr);
-      tmem_wait_ld();
-      if (release) warp_arrive(x_free, r.lane);
-      const float4* lse4 = reinterpret_cast<const float4*>(lse_ptr);
-#pragma unroll
-      for (int g = 0; g < CPW / 4; ++g) {
-        const float4 l4 = lse4[g];
-        const f32x2 t01 = f2_fma(f2_make(__uint_as_float(sr[4 * g]), __uint_as_float(sr[4 * g + 1])),
-                                 neg_scale2, f2_make(l4.x, l4.y));
-        const f32x2 t23 = f2_fma(f2_make(__uint_as_float(sr[4 * g + 2]), __uint_as_float(sr[4 * g + 3])),
-                                 neg_scale2, f2_make(l4.z, l4.w));
-        float t[4];
-        f2_split(t01, t[0], t[1]);
-        f2_split(t23, t[2], t[3]);
-        float pe[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) pe[e] = fast_exp2(-t[e]);
-        if (diag) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (q_first + 4 * g + e < kv_pos) pe[e] = 0.f;
-        }
-        p2[2 * g] = f2_make(pe[0], pe[1]);
-        p2[2 * g + 1] = f2_make(pe[2], pe[3]);
-        pp[2 * g] = pack2<FMT>(pe[0], pe[1]);
-        pp[2 * g + 1] = pack2<FMT>(pe[2], pe[3]);
-      }
-    };
+    const f32x2 minus_one2 = f2_splat(-1.0f);
     int it = 0;
-    // P^T of the very first chunk
-    mbar_wait(do_full + 0, 0, ctx, 842);
-    mbar_wait(s_full, 0, ctx, 843);
-    __syncwarp();
-    tc_fence_after_sync();
-    exp_chunk(col0, s_stat + col0, true, kv0 + col0, false);
     for (int c = 0; c < n_git; ++c) {
       const int st = c & 1;
       const uint32_t par = (uint32_t)(c & 1);
-      const float* stat = s_stat + st * 256;
-      const int q0 = (kvt + it) * kTile;
-      const int it1 = it + 1 == n_it ? 0 : it + 1;
-#pragma unroll
-      for (int ch = 0; ch < 2; ++ch) {
-        // dS^T of chunk (c, ch): into Y behind P^T, and into shared memory
-        mbar_wait(dp_full + ch, par, ctx, 844);
-        __syncwarp();
-        tc_fence_after_sync();
-        uint32_t dr[CPW];
-        tmem_ld(tY + lane_base + col0, dr);
+      const float* stat = s_stat + st * 256 + b * 64 + col0;
+      // P^T: t = lse2 - s c, p = 2^-t, two columns per packed instruction. On the first
+      // query tile, queries before the key are masked. S^T is handed back as soon as its
+      // columns are in registers.
+      f32x2 p2[16];
+      mbar_wait(do_full + st, (uint32_t)((c >> 1) & 1), ctx, 842);
+      mbar_wait(s_full, par, ctx, 843);
+      __syncwarp();
+      tc_fence_after_sync();
+      {
+        uint32_t sr[32];
+        tmem_ld(tX + lane_base + b * 64 + col0, sr);
         tmem_wait_ld();
-        const float4* del4 = reinterpret_cast<const float4*>(stat + 128 + ch * 64 + col0);
-        uint32_t dd[CPW / 2];
-        const f32x2 minus_one2 = f2_splat(-1.0f);
+        warp_arrive(x_free, r.lane);
+        const float4* lse4 = reinterpret_cast<const float4*>(stat);
 #pragma unroll
-        for (int g = 0; g < CPW / 4; ++g) {
+        for (int g = 0; g < 8; ++g) {
+          const float4 l4 = lse4[g];
+          const f32x2 t01 = f2_fma(f2_make(__uint_as_float(sr[4 * g]), __uint_as_float(sr[4 * g + 1])),
+                                   neg_scale2, f2_make(l4.x, l4.y));
+          const f32x2 t23 = f2_fma(f2_make(__uint_as_float(sr[4 * g + 2]), __uint_as_float(sr[4 * g + 3])),
+                                   neg_scale2, f2_make(l4.z, l4.w));
+          float t[4];
+          f2_split(t01, t[0], t[1]);
+          f2_split(t23, t[2], t[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[e] = fast_exp2(-t[e]);
+          p2[2 * g] = f2_make(t[0], t[1]);
+          p2[2 * g + 1] = f2_make(t[2], t[3]);
+        }
+      }
+      if (it == 0) {
+        const int q_first = kv0 + b * 64 + col0;
+#pragma unroll
+        for (int g = 0; g < 16; ++g) {
+          float lo, hi;
+          f2_split(p2[g], lo, hi);
+          if (q_first + 2 * g < kv_pos) lo = 0.f;
+          if (q_first + 2 * g + 1 < kv_pos) hi = 0.f;
+          p2[g] = f2_make(lo, hi);
+        }
+      }
+      // dS^T = P^T (dP^T - delta), 16 queries at a time; P^T and dS^T go back over dP^T
+      // first: the products that wait for them are the critical path.
+      mbar_wait(dp_full + b, par, ctx, 844);
+      __syncwarp();
+      tc_fence_after_sync();
+      uint32_t dd[2][8];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint32_t dr[16], pp[8];
+        tmem_ld(tY + 16 * k, dr);
+        tmem_wait_ld();
+        const float4* del4 = reinterpret_cast<const float4*>(stat + 128 + 16 * k);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
           const float4 d4 = del4[g];
-          // dS = P (dP - delta), two columns at a time; rounded to 16 bits as an operand
           const f32x2 a01 = f2_fma(f2_make(d4.x, d4.y), minus_one2,
                                    f2_make(__uint_as_float(dr[4 * g]), __uint_as_float(dr[4 * g + 1])));
           const f32x2 a23 = f2_fma(f2_make(d4.z, d4.w), minus_one2,
                                    f2_make(__uint_as_float(dr[4 * g + 2]), __uint_as_float(dr[4 * g + 3])));
-          float d[4];
-          f2_split(f2_mul(p2[2 * g], a01), d[0], d[1]);
-          f2_split(f2_mul(p2[2 * g + 1], a23), d[2], d[3]);
-          dd[2 * g] = pack2<FMT>(d[0], d[1]);
-          dd[2 * g + 1] = pack2<FMT>(d[2], d[3]);
+          float d[4], pe[4];
+          f2_split(f2_mul(p2[8 * k + 2 * g], a01), d[0], d[1]);
+          f2_split(f2_mul(p2[8 * k + 2 * g + 1], a23), d[2], d[3]);
+          f2_split(p2[8 * k + 2 * g], pe[0], pe[1]);
+          f2_split(p2[8 * k + 2 * g + 1], pe[2], pe[3]);
+          pp[2 * g] = pack2<FMT>(pe[0], pe[1]);
+          pp[2 * g + 1] = pack2<FMT>(pe[2], pe[3]);
+          dd[k][2 * g] = pack2<FMT>(d[0], d[1]);
+          dd[k][2 * g + 1] = pack2<FMT>(d[2], d[3]);
         }
-        // P^T / dS^T into Y first: the products that wait for them are the critical path.
-        tmem_st(tY + lane_base + col0, pp);
-        tmem_st(tY + lane_base + col0 + CPW / 2, dd);
-        tmem_wait_st();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (r.lane == 0) mbar_arrive(pds_full + ch);
-        if (c > 0) mbar_wait(dq_full + ch, par ^ 1u, ctx, 848);  // the buffer's last reader is done
-        {
-          // dS^T for the dQ^T product: row r.row (a key) of the chunk's [128 keys x 64
-          // queries] tile, 16-byte pieces 2g and 2g+1 of its 128 bytes, at their
-          // swizzled places.
-          uint8_t* row_ptr = sDS + ch * kChunkBytes + r.row * 128;
-          const int sw = r.row & 7;
-          *reinterpret_cast<uint4*>(row_ptr + (((2 * r.half) ^ sw) << 4)) =
-              make_uint4(dd[0], dd[1], dd[2], dd[3]);
-          *reinterpret_cast<uint4*>(row_ptr + (((2 * r.half + 1) ^ sw) << 4)) =
-              make_uint4(dd[4], dd[5], dd[6], dd[7]);
-        }
-        // P^T of the chunk after this one
-        if (ch == 0) {
-          exp_chunk(64 + col0, stat + 64 + col0, it == 0, q0 + 64 + col0, true);
-        } else if (c + 1 < n_git) {
-          mbar_wait(do_full + (st ^ 1), (uint32_t)(((c + 1) >> 1) & 1), ctx, 845);
-          mbar_wait(s_full, par ^ 1u, ctx, 846);
-          __syncwarp();
-          tc_fence_after_sync();
-          exp_chunk(col0, s_stat + (st ^ 1) * 256 + col0, it1 == 0, (kvt + it1) * kTile + col0, false);
-        }
-        // The tensor pipe reads the shared-memory copy of dS^T a whole chunk later: its
-        // proxy fence waits here, behind the exponentials.
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (r.lane == 0) mbar_arrive(ds_full + ch);
+        tmem_st(tY + 16 * k, pp);
+        tmem_st(tY + 16 * k + 8, dd[k]);
       }
-      it = it1;
+      tmem_wait_st();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (r.lane == 0) mbar_arrive(pds_full + b);
+      // dS^T for the dQ^T product: row r.row (a key) of the half's [128 keys x 64 queries]
+      // tile, four 16-byte pieces of its 128 bytes at their swizzled places. The buffer's
+      // last reader has finished: this dP^T was issued behind the last dQ^T.
+      {
+        uint8_t* row_ptr = sDS + b * kChunkBytes + r.row * 128;
+        const int sw = r.row & 7, piece = col0 / 8;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          *reinterpret_cast<uint4*>(row_ptr + (((piece + 2 * k) ^ sw) << 4)) =
+              make_uint4(dd[k][0], dd[k][1], dd[k][2], dd[k][3]);
+          *reinterpret_cast<uint4*>(row_ptr + (((piece + 2 * k + 1) ^ sw) << 4)) =
+              make_uint4(dd[k][4], dd[k][5], dd[k][6], dd[k][7]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (r.lane == 0) mbar_arrive(ds_full + b);
+      if (++it == n_it) it = 0;
     }
     mbar_wait(done, 0, ctx, 847);
     __syncwarp();
