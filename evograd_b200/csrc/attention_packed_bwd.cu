@@ -6,32 +6,33 @@
 // One pass over the visible tiles, five products per (key tile, query tile). A block
 // owns one key tile of one k/v head and walks the query tiles behind it, for every
 // query head of the group. A tile's two halves of 64 queries are two streams:
-//   S^T   = K Q_i^T                 [128 keys x 128 queries], once per tile
-//   dP^T  = V dO^T                  [128 keys x 64 queries] per stream
+//   S^T   = K Q^T,  dP^T = V dO^T   [128 keys x 64 queries], A from tensor memory
 //   P^T, dS^T in registers, then 16 bits back into tensor memory over dP^T
 //   dV   += P^T dO,  dK += dS^T Q   (A from tensor memory)
-//   dQ^T  = K^T dS^T                [128 head columns x 64 queries], over P^T and dS^T
-// Each stream has eight compute warps and tensor-memory columns of its own, so that one
-// stream's exponentials and dS run under the other stream's products; with one set of
-// sixteen warps on one chunk after the other, the chain products -> warps -> products
-// took 6200 cycles per tile pair. dK and dV stay in tensor memory until the end (fixed
-// order, no atomics). dQ^T also belongs to other blocks' rows: four warps of their own
-// add it to a float32 copy of dQ, so dq can differ in the last bit from run to run; a
-// last kernel scales and rounds the copy.
+//   dQ^T  = K^T dS^T                [128 head columns x 64 queries], A the K tile in shared
+// A stream's S^T, dP^T, P^T / dS^T and dQ^T follow one another in the same 64 columns of
+// tensor memory. Each stream has eight compute warps of its own, so one stream's
+// exponentials and dS run under the other stream's products. dK and dV stay in tensor
+// memory until the end (fixed order, no atomics). dQ^T also belongs to other blocks'
+// rows: four warps of their own send it to a float32 copy of dQ by asynchronous bulk
+// reductions, so dq can differ in the last bit from run to run; a last kernel scales and
+// rounds the copy.
+//
+// K and V are kept in tensor memory as well (64 columns each): a product of two
+// shared-memory operands with 64 columns needs 192 bytes a clock of the shared memory's
+// 128, and with both scores and dP^T formed that way the operand reads, not the tensor
+// pipe, set the time (416 KB per tile pair against 320 KB now).
 //
 // Order of the products for tile c (numbers in brackets: the stream):
-//   S(c+1)  dP(c)[1]  dV,dK(c)[0]  dQ(c)[0]  dV,dK(c)[1]  dP(c+1)[0]  dQ(c)[1]
-// The tensor pipe runs in order, so every wait of the issuing warp sits behind products
-// that hide it: dP of a stream has to wait until the stream's last dQ^T has been taken
-// out of the columns they share, and runs behind the other stream's dV, dK or the next
-// scores.
+//   S(c)[0]  dV,dK(c-1)[1]  dP(c)[0]  dQ(c-1)[1]  S(c)[1]  dV,dK(c)[0]  dP(c)[1]  dQ(c)[0]
+// The tensor pipe runs in order; the streams are half a tile apart, so what one of them
+// waits for runs behind the other's products.
 //
-// Tensor memory: S^T [0,128), streams' dP^T / P^T / dS^T / dQ^T [128,192) and [192,256),
-// dV [256,256+HD), dK [384,384+HD). Shared memory: K, V, two dO and two Q stages, two
-// 16 KB dS^T halves, row statistics (226 KB at head size 128). At head size 64 the dQ^T
-// product keeps its 128 rows: the A operand's second 64 columns are the V tile, which
-// follows K in shared memory, and the rows they give are not read (a 64-row product has
-// another layout in tensor memory).
+// Tensor memory: streams [0,64) and [64,128), K [128,192), V [192,256), dV [256,256+HD),
+// dK [384,384+HD). Shared memory: K, two dO and two Q stages, two 16 KB dS^T halves, row
+// statistics, 32 KB of float32 dQ on its way out (226 KB at head size 128). At head size 64 the dQ^T product keeps its 128
+// rows: the A operand's second 64 columns are whatever follows K in shared memory, and
+// the rows they give are not read (a 64-row product has another layout in tensor memory).
 //
 // Tiles start at the sequence's first token; rows of K, V, Q and dO behind its end are
 // other tokens and are zeroed in shared memory, and their statistics make P zero.
@@ -66,7 +67,7 @@ struct BwdParams {
   float* lse2;    // [Hq][slots * 128] log-sum-exp in log2 units, +inf behind a sequence
   float* delta;   // [Hq][slots * 128]
   float* dq_acc;  // [Hq][slots * 128][HD]
-  View dq, dk, dv;
+  View k, v, dq, dk, dv;
   int tokens, slots, units, head_group, group, D;
   float scale;
   long long wait_limit;
@@ -76,12 +77,19 @@ struct BwdParams {
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-__device__ __forceinline__ void red_add_f32x4(float* addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(addr),
-               "f"(__uint_as_float(a)), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)),
-               "f"(__uint_as_float(d))
+// float32 sums of a contiguous piece of shared memory into global memory, asynchronous
+// (both addresses 16-byte aligned, a multiple of 16 bytes), in the thread's bulk group.
+__device__ __forceinline__ void bulk_add_f32(float* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.reduce.async.bulk.global.shared::cta.bulk_group.add.f32 [%0], [%1], %2;" ::"l"(dst),
+               "r"(smem_u32(src)), "r"(bytes)
                : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+// All but the newest N groups of this thread have read their source / are complete.
+template <int N> __device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ uint8_t* view_row(const View& v, int64_t token, int head) {
   return reinterpret_cast<uint8_t*>(v.p) + (token * v.st + (int64_t)head * v.sh) * 2;
 }
@@ -119,7 +127,6 @@ template <int HD, int FMT>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_k,
-                       const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ CUtensorMap map_do, const BwdParams p) {
   // Key tile n - w of a sequence of n tiles: w query tiles to visit, heaviest first.
   int slot, bh;
@@ -154,40 +161,39 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     return;
   }
   uint8_t* sK = bs.smem;
-  uint8_t* sV = sK + TB;  // directly behind K (the dQ^T product of head size 64 reads on)
-  uint8_t* sDO0 = sV + TB;       // 2 stages
+  uint8_t* sDO0 = sK + TB;       // 2 stages
   uint8_t* sQ0 = sDO0 + 2 * TB;  // 2 stages
-  uint8_t* sDS = sQ0 + 2 * TB;   // 2 chunks of dS^T
-  float* s_stat = reinterpret_cast<float*>(sDS + 2 * kChunkBytes);  // [stage][lse2 | delta][128]
-  uint64_t* kv_full = bs.bars + 0;
-  uint64_t* q_full = bs.bars + 1;    // [2]
+  uint8_t* sDS = sQ0 + 2 * TB;   // dS^T of the streams
+  uint8_t* sDQ = sDS + 2 * kChunkBytes;  // float32 dQ on its way out, two pieces of 32 queries
+  float* s_stat = reinterpret_cast<float*>(sDQ + TB);  // [stage][lse2 | delta][128]
+  uint64_t* kv_full = bs.bars + 0;   // K in shared memory, K and V in tensor memory
+  uint64_t* q_full = bs.bars + 1;    // [2] by stage
   uint64_t* q_empty = bs.bars + 3;   // [2]
   uint64_t* do_full = bs.bars + 5;   // [2]
   uint64_t* do_empty = bs.bars + 7;  // [2]
-  uint64_t* s_full = bs.bars + 9;
-  uint64_t* x_free = bs.bars + 10;
-  uint64_t* dp_full = bs.bars + 11;   // [2] by stream, as all below
-  uint64_t* pds_full = bs.bars + 13;  // [2] P^T / dS^T are in Y
-  uint64_t* ds_full = bs.bars + 15;   // [2] dS^T is in shared memory
-  uint64_t* dq_full = bs.bars + 17;   // [2] dQ^T is in Y
-  uint64_t* d_free = bs.bars + 19;    // [2] dQ^T has been read
-  uint64_t* done = bs.bars + 21;
+  uint64_t* s_full = bs.bars + 9;     // [2] by stream, as all below
+  uint64_t* x_free = bs.bars + 11;    // [2] the scores have been read
+  uint64_t* dp_full = bs.bars + 13;   // [2]
+  uint64_t* pds_full = bs.bars + 15;  // [2] P^T / dS^T are in tensor memory
+  uint64_t* ds_full = bs.bars + 17;   // [2] dS^T is in shared memory
+  uint64_t* dq_full = bs.bars + 19;   // [2]
+  uint64_t* d_free = bs.bars + 21;    // [2] dQ^T has been read
+  uint64_t* done = bs.bars + 23;
   const Roles r = roles();
   const float scale_log2 = p.scale * kLog2e;
 
   if (threadIdx.x == 0) {
     *bs.abort_flag = 0;
-    mbar_init(kv_full, 1); mbar_init(done, 1);
+    mbar_init(kv_full, 1 + kComputeWarps); mbar_init(done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1); mbar_init(q_empty + i, 1);
       mbar_init(do_full + i, 1); mbar_init(do_empty + i, 1);
+      mbar_init(s_full + i, 1); mbar_init(x_free + i, kStreamWarps);
       mbar_init(dp_full + i, 1); mbar_init(pds_full + i, kStreamWarps);
       mbar_init(ds_full + i, kStreamWarps); mbar_init(dq_full + i, 1); mbar_init(d_free + i, 4);
     }
-    mbar_init(s_full, 1); mbar_init(x_free, kComputeWarps);
     fence_mbar_init();
-    prefetch_tensormap(&map_q); prefetch_tensormap(&map_k);
-    prefetch_tensormap(&map_v); prefetch_tensormap(&map_do);
+    prefetch_tensormap(&map_q); prefetch_tensormap(&map_k); prefetch_tensormap(&map_do);
   }
   __syncthreads();
   if (r.warp == 1) { tmem_alloc(bs.tmem_slot, 512); tmem_relinquish(); }
@@ -196,17 +202,16 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   tc_fence_after_sync();
   const uint32_t tmem = *bs.tmem_slot;
   const WaitCtx ctx{bs.abort_flag, &g_attn_packed_bwd_status, p.wait_limit};
-  constexpr uint32_t idesc_s = instr_desc_f16(FMT, 128, 128, 0, 0);
   constexpr uint32_t idesc_p = instr_desc_f16(FMT, 128, 64, 0, 0);
   constexpr uint32_t idesc_d = instr_desc_f16(FMT, 128, HD, 0, 1);
   constexpr uint32_t idesc_q = instr_desc_f16(FMT, 128, 64, 1, 1);
-  const uint32_t tX = tmem, tY0 = tmem + 128;  // stream b: tY0 + 64 b
+  const uint32_t tY0 = tmem;  // stream b: tY0 + 64 b
+  const uint32_t tK = tmem + 128, tV = tmem + 192;
   const uint32_t tDV = tmem + 256, tDK = tmem + 384;
 
   if (r.is_tma && r.lane == 0) {
-    mbar_expect_tx(kv_full, 2 * TB);
+    mbar_expect_tx(kv_full, TB);
     load_tile<HD>(sK, &map_k, seq0 + kv0, bh, kv_full);
-    load_tile<HD>(sV, &map_v, seq0 + kv0, bh, kv_full);
     int it = 0, head = bh * p.group, git = 0;
     for (; git < n_git; ++git) {
       const int st = git & 1;
@@ -236,17 +241,17 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     }
   } else if (r.is_mma) {
     const bool lead = elect_one();
-    const DescBase v_base = desc_base_kmajor(smem_u32(sV));
     const DescBase kt_base = desc_base_mnmajor(smem_u32(sK), kTile);
-    // dP^T of stream b: B operand = rows [64 b, 64 b + 64) of a dO tile.
-    auto issue_dp = [&](int b, uint32_t do_saddr) {
-      const DescBase da = desc_base_kmajor(do_saddr + b * 64 * 128);
+    // [128 keys x 64 queries] of stream b into its columns: A = K or V in tensor memory,
+    // B = rows [64 b, 64 b + 64) of a Q or dO tile.
+    auto issue_rows = [&](int b, uint32_t a_tmem, uint32_t tile_saddr, uint64_t* bar) {
+      const DescBase rows = desc_base_kmajor(tile_saddr + b * 64 * 128);
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
         if (lead)
-          mma_ss(tY0 + 64 * b, desc_at(v_base, kstep_kmajor(kTile, ks)),
-                 desc_at(da, kstep_kmajor(kTile, ks)), idesc_p, ks > 0 ? 1u : 0u);
-      if (lead) mma_commit(dp_full + b);
+          mma_ts(tY0 + 64 * b, a_tmem + 8 * ks, desc_at(rows, kstep_kmajor(kTile, ks)), idesc_p,
+                 ks > 0 ? 1u : 0u);
+      if (lead) mma_commit(bar + b);
     };
     // Query k-step kk of the stream (16 queries): P^T in its columns [16 kk, 16 kk + 8),
     // dS^T in the 8 columns behind it (the layout the compute warps write).
@@ -281,74 +286,75 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
       if (it == n_it - 1 && tail_rows < kTile) clear_tile_rows<HD>(tile, tail_rows, r.lane);
     };
     mbar_wait(kv_full, 0, ctx, 822);
-    if (kvt == last_tile && tail_rows < kTile) {
-      clear_tile_rows<HD>(sK, tail_rows, r.lane);
-      clear_tile_rows<HD>(sV, tail_rows, r.lane);
-    }
-    mbar_wait(q_full + 0, 0, ctx, 823);
-    clear_tail(sQ0, 0);
-    tc_fence_after_sync();
-    issue_scores<HD>(lead, tX, smem_u32(sK), smem_u32(sQ0), idesc_s);
-    if (lead) mma_commit(s_full);
-    mbar_wait(do_full + 0, 0, ctx, 832);
-    clear_tail(sDO0, 0);
-    tc_fence_after_sync();
-    issue_dp(0, smem_u32(sDO0));
-    issue_dp(1, smem_u32(sDO0));
-    int it1 = 0;  // query tile of iteration c + 1
-    for (int c = 0; c < n_git; ++c) {
-      const int st = c & 1, st1 = st ^ 1;
-      const uint32_t par = (uint32_t)(c & 1), par1 = (uint32_t)(((c + 1) >> 1) & 1);
-      const bool more = c + 1 < n_git;
-      const uint32_t do_saddr = smem_u32(sDO0 + st * TB), q_saddr = smem_u32(sQ0 + st * TB);
-      if (++it1 == n_it) it1 = 0;
-      if (more) {
-        mbar_wait(q_full + st1, par1, ctx, 827);
-        clear_tail(sQ0 + st1 * TB, it1);
-        mbar_wait(x_free, par, ctx, 828);
+    if (kvt == last_tile && tail_rows < kTile) clear_tile_rows<HD>(sK, tail_rows, r.lane);
+    int it = 0;  // query tile of iteration c
+    for (int c = 0; c <= n_git; ++c) {
+      const int st = c & 1;
+      const uint32_t par = (uint32_t)(c & 1), full = (uint32_t)((c >> 1) & 1);
+      const bool now = c < n_git, behind = c > 0;  // tile c; stream 1's second half of tile c - 1
+      uint8_t *q_tile = sQ0 + st * TB, *do_tile = sDO0 + st * TB;
+      const uint32_t q_saddr = smem_u32(q_tile), do_saddr = smem_u32(do_tile);
+      if (now) {
+        mbar_wait(q_full + st, full, ctx, 823);
+        clear_tail(q_tile, it);
+        if (behind) mbar_wait(d_free + 0, par ^ 1u, ctx, 835);
         tc_fence_after_sync();
-        issue_scores<HD>(lead, tX, smem_u32(sK), smem_u32(sQ0 + st1 * TB), idesc_s);
-        if (lead) mma_commit(s_full);
+        issue_rows(0, tK, q_saddr, s_full);
       }
-      if (c > 0) {
-        mbar_wait(d_free + 1, par ^ 1u, ctx, 826);
+      if (behind) {
+        mbar_wait(pds_full + 1, par ^ 1u, ctx, 829);
         tc_fence_after_sync();
-        issue_dp(1, do_saddr);
+        issue_dv(1, smem_u32(sDO0 + (st ^ 1) * TB), false);
+        if (lead) mma_commit(do_empty + (st ^ 1));
+        issue_dk(1, smem_u32(sQ0 + (st ^ 1) * TB), false);
+        if (lead) mma_commit(q_empty + (st ^ 1));
       }
-      mbar_wait(pds_full + 0, par, ctx, 824);
-      tc_fence_after_sync();
-      issue_dv(0, do_saddr, c == 0);
-      issue_dk(0, q_saddr, c == 0);
-      mbar_wait(ds_full + 0, par, ctx, 825);
-      tc_fence_after_sync();
-      issue_dq(0);
-      mbar_wait(pds_full + 1, par, ctx, 829);
-      tc_fence_after_sync();
-      issue_dv(1, do_saddr, false);
-      if (lead) mma_commit(do_empty + st);
-      issue_dk(1, q_saddr, false);
-      if (lead) mma_commit(q_empty + st);
-      if (more) {
-        mbar_wait(do_full + st1, par1, ctx, 833);
-        clear_tail(sDO0 + st1 * TB, it1);
-        mbar_wait(d_free + 0, par, ctx, 835);
+      if (now) {
+        mbar_wait(do_full + st, full, ctx, 832);
+        clear_tail(do_tile, it);
+        mbar_wait(x_free + 0, par, ctx, 828);
         tc_fence_after_sync();
-        issue_dp(0, smem_u32(sDO0 + st1 * TB));
+        issue_rows(0, tV, do_saddr, dp_full);
       }
-      mbar_wait(ds_full + 1, par, ctx, 834);
-      tc_fence_after_sync();
-      issue_dq(1);
+      if (behind) {
+        mbar_wait(ds_full + 1, par ^ 1u, ctx, 834);
+        tc_fence_after_sync();
+        issue_dq(1);
+      }
+      if (now) {
+        if (behind) {
+          mbar_wait(d_free + 1, par ^ 1u, ctx, 826);
+          tc_fence_after_sync();
+        }
+        issue_rows(1, tK, q_saddr, s_full);
+        mbar_wait(pds_full + 0, par, ctx, 824);
+        tc_fence_after_sync();
+        issue_dv(0, do_saddr, c == 0);
+        issue_dk(0, q_saddr, c == 0);
+        mbar_wait(x_free + 1, par, ctx, 833);
+        tc_fence_after_sync();
+        issue_rows(1, tV, do_saddr, dp_full);
+        mbar_wait(ds_full + 0, par, ctx, 825);
+        tc_fence_after_sync();
+        issue_dq(0);
+      }
+      if (++it == n_it) it = 0;
       __syncwarp();
     }
     if (lead) mma_commit(done);
   } else if (r.warp >= 2 + kComputeWarps) {
-    // dQ^T of every half tile: this warp's 32 lanes (head columns) x 64 query columns,
-    // added to the float32 copy four queries at a time (16 bytes per lane, 512 per warp).
+    // dQ^T of every half tile to the float32 copy, 32 queries at a time: out of tensor
+    // memory (a thread has one head column), into shared memory in the copy's layout, and
+    // on by an asynchronous bulk reduction, 16 KB each, one being written while the other
+    // is read. (Reductions issued by these threads, 64 lines each, held up every access of
+    // the SM to shared memory and mbarriers for about 1100 cycles per half tile.)
     const uint32_t lane_base = (uint32_t)(r.quarter * 32) << 16;
+    constexpr uint32_t kPiece = 32 * HD * 4;
+    const bool issuer = r.warp == 2 + kComputeWarps && r.lane == 0;
     int it = 0, head = bh * p.group;
     for (int c = 0; c < n_git; ++c) {
       const uint32_t par = (uint32_t)(c & 1);
-      float* tile_dst = p.dq_acc + (head * P + prow0 + (int64_t)it * kTile) * HD + r.row * 4;
+      float* tile_dst = p.dq_acc + (head * P + prow0 + (int64_t)it * kTile) * HD;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         mbar_wait(dq_full + b, par, ctx, 841);
@@ -359,16 +365,24 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
         tmem_ld(tY0 + 64 * b + lane_base + 32, acc[1]);
         tmem_wait_ld();
         warp_arrive(d_free + b, r.lane);
-        float* dst = tile_dst + b * 64 * HD;
-        if (r.row < p.D) {
 #pragma unroll
-          for (int j = 0; j < 64; j += 4)
-            red_add_f32x4(dst + j * HD, acc[j >> 5][j & 31], acc[j >> 5][(j & 31) + 1],
-                          acc[j >> 5][(j & 31) + 2], acc[j >> 5][(j & 31) + 3]);
+        for (int h = 0; h < 2; ++h) {
+          if (issuer) bulk_wait_read<1>();  // this piece's last reduction has read it
+          named_barrier_sync(1, 128);
+          if (r.row < HD) {
+            uint4* dst = reinterpret_cast<uint4*>(sDQ + h * kPiece) + r.row;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              dst[j * HD] = make_uint4(acc[h][4 * j], acc[h][4 * j + 1], acc[h][4 * j + 2], acc[h][4 * j + 3]);
+          }
+          fence_proxy_async_smem();
+          named_barrier_sync(1, 128);
+          if (issuer && !*ctx.abort_flag) bulk_add_f32(tile_dst + (b * 64 + h * 32) * HD, sDQ + h * kPiece, kPiece);
         }
       }
       if (++it == n_it) { it = 0; ++head; }
     }
+    if (issuer) bulk_wait_all();
   } else if (r.is_compute) {
     const uint32_t lane_base = (uint32_t)(r.quarter * 32) << 16;
     const int kv_pos = kv0 + r.row;
@@ -377,6 +391,26 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     const uint32_t tY = tY0 + 64 * b + lane_base + col0;
     const f32x2 neg_scale2 = f2_splat(-scale_log2);
     const f32x2 minus_one2 = f2_splat(-1.0f);
+    // Stream 0's warps put K, stream 1's V into tensor memory: a thread its key's row (half
+    // of it), two 16-bit elements per column, zero behind the sequence's end and behind D.
+    {
+      const View& src = b ? p.v : p.k;
+      const bool ok = kv_pos < L;
+      const uint8_t* g = view_row(src, seq0 + (ok ? kv_pos : 0), bh);
+      const int e0 = col0 / 32 * (HD / 2);  // first element
+      uint32_t w[HD / 4];
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (ok && e0 + 8 * i < p.D) x = *reinterpret_cast<const uint4*>(g + (e0 + 8 * i) * 2);
+        w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
+      }
+      const uint32_t dst = (b ? tV : tK) + lane_base + e0 / 2;
+#pragma unroll
+      for (int i = 0; i < HD / 64; ++i) tmem_st(dst + 16 * i, *reinterpret_cast<uint32_t(*)[16]>(&w[16 * i]));
+      tmem_wait_st();
+      warp_arrive(kv_full, r.lane);
+    }
     int it = 0;
     for (int c = 0; c < n_git; ++c) {
       const int st = c & 1;
@@ -387,14 +421,14 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
       // columns are in registers.
       f32x2 p2[16];
       mbar_wait(do_full + st, (uint32_t)((c >> 1) & 1), ctx, 842);
-      mbar_wait(s_full, par, ctx, 843);
+      mbar_wait(s_full + b, par, ctx, 843);
       __syncwarp();
       tc_fence_after_sync();
       {
         uint32_t sr[32];
-        tmem_ld(tX + lane_base + b * 64 + col0, sr);
+        tmem_ld(tY, sr);
         tmem_wait_ld();
-        warp_arrive(x_free, r.lane);
+        warp_arrive(x_free + b, r.lane);
         const float4* lse4 = reinterpret_cast<const float4*>(stat);
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
@@ -587,12 +621,10 @@ int read_packed_bwd_status(int reset) {
 const bool g_packed_bwd_registered = (register_device_status(read_packed_bwd_status), true);
 
 template <int HD, int FMT>
-int launch(const View& dout, const View& q, const View& k, const View& v, const View& o,
-           const float* lse, BwdParams& p, int64_t Hq, int64_t Hkv, cudaStream_t stream) {
-  CUtensorMap mq, mk, mv, mdo;
+int launch(const View& dout, const View& q, const View& o, const float* lse, BwdParams& p, int64_t Hq, int64_t Hkv, cudaStream_t stream) {
+  CUtensorMap mq, mk, mdo;
   if (!encode_view_map(&mq, q, FMT, p.D, p.tokens, Hq) ||
-      !encode_view_map(&mk, k, FMT, p.D, p.tokens, Hkv) ||
-      !encode_view_map(&mv, v, FMT, p.D, p.tokens, Hkv) ||
+      !encode_view_map(&mk, p.k, FMT, p.D, p.tokens, Hkv) ||
       !encode_view_map(&mdo, dout, FMT, p.D, p.tokens, Hq))
     return fail(EVG_ELAUNCH, "packed_attention_bwd: cuTensorMapEncodeTiled failed");
   size_t smem = bwd_tile_region<HD>() + kControlBytes + 1024;
@@ -609,7 +641,7 @@ int launch(const View& dout, const View& q, const View& k, const View& v, const 
   const dim3 rows_grid((unsigned)p.slots, (unsigned)Hq, (unsigned)parts);
   packed_prepare_kernel<HD, FMT><<<rows_grid, 256, 0, stream>>>(dout, o, lse, p);
   if (int rc = check_launch("packed_attention_bwd statistics")) return rc;
-  kern<<<(unsigned)((int64_t)p.slots * p.units), kBwdThreads, smem, stream>>>(mq, mk, mv, mdo, p);
+  kern<<<(unsigned)((int64_t)p.slots * p.units), kBwdThreads, smem, stream>>>(mq, mk, mdo, p);
   if (int rc = check_launch("packed_attention_bwd")) return rc;
   packed_finish_kernel<HD, FMT><<<rows_grid, 256, 0, stream>>>(p);
   return check_launch("packed_attention_bwd dq");
@@ -636,6 +668,8 @@ int launch_bwd(const View& dout, const View& q, const View& k, const View& v, co
   p.lse2 = (float*)workspace;
   p.delta = p.lse2 + rows;
   p.dq_acc = p.delta + rows;
+  p.k = k;
+  p.v = v;
   p.dq = dq;
   p.dk = dk;
   p.dv = dv;
@@ -646,10 +680,10 @@ int launch_bwd(const View& dout, const View& q, const View& k, const View& v, co
   p.scale = scale;
   p.wait_limit = wait_limit_cycles2();
   if (D > 64)
-    return fmt == 1 ? launch<128, 1>(dout, q, k, v, o, lse, p, Hq, Hkv, stream)
-                    : launch<128, 0>(dout, q, k, v, o, lse, p, Hq, Hkv, stream);
-  return fmt == 1 ? launch<64, 1>(dout, q, k, v, o, lse, p, Hq, Hkv, stream)
-                  : launch<64, 0>(dout, q, k, v, o, lse, p, Hq, Hkv, stream);
+    return fmt == 1 ? launch<128, 1>(dout, q, o, lse, p, Hq, Hkv, stream)
+                    : launch<128, 0>(dout, q, o, lse, p, Hq, Hkv, stream);
+  return fmt == 1 ? launch<64, 1>(dout, q, o, lse, p, Hq, Hkv, stream)
+                  : launch<64, 0>(dout, q, o, lse, p, Hq, Hkv, stream);
 }
 
 }  // namespace packed
