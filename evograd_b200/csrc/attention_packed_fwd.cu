@@ -4,10 +4,15 @@
 //   lse_i = log sum_j exp(s_ij)
 //
 // 320 threads per block: a TMA producer warp, a tcgen05 issuer warp and two groups
-// of four softmax warps, each group with a 128-row query tile of its own (TMEM:
-// S_A [0,128), S_B [128,256), O_A [256,256+HD), O_B [384,384+HD)), so one tile's
-// softmax runs while the other tile's products do. Per key tile j:
-//   O_A += P_A(j) V_j;  S_A(j+1) = Q_A K_{j+1}^T;  O_B += P_B(j) V_j;  S_B(j+1) = ...
+// of four softmax warps, each group with a 128-row query tile of its own, so one tile's
+// softmax runs while the other tile's products do. Keys come in tiles of 128 and are
+// worked through in halves of 64: each group has two score buffers, and while it turns
+// one half's scores into probabilities the other half's are being formed, so its warps
+// never wait for a product that waits for them (with one 128-key buffer per group the
+// chain scores -> softmax -> PV -> next scores took 3980 cycles per key tile). Per half g:
+//   O_A += P_A(g) V_g;  S_A(g+2) = Q_A K_{g+2}^T;  O_B += P_B(g) V_g;  S_B(g+2) = ...
+// TMEM: score buffers A [0,128), B [128,256) (P packed over the scores it came from),
+// O_A [256,256+HD), O_B [384,384+HD).
 //
 // The two query tiles of a block share their key tiles. Where the query heads of a
 // k/v head can be paired (an even group), they are the SAME positions of two heads:
@@ -19,8 +24,11 @@
 // tokens: as keys the causal mask drops them, as values they are zeroed in shared
 // memory (0 x infinity), as queries they are computed and not stored.
 //
-// Bound: the special-function unit and the tensor pipe together (one exponential per
-// visible pair and head; 4 HD flop).
+// Bound: the softmax warps' chain per half (TMEM load, maximum, 64 exponentials and their
+// packing, TMEM store: 1700-1900 cycles for the two warps of a scheduler, the special-
+// function unit busy for 1024 of them) and, in long runs, the power limit. Forming a
+// quarter or a third of the exponentials by a polynomial on the FMA pipe was 5-7 %
+// slower. 12001 + 2500 + 1000 + 883 tokens, 32/8 heads of 128: 1068 us, 1166 TFLOP/s.
 #include "packed.cuh"
 
 namespace evg {
@@ -46,6 +54,12 @@ struct FwdParams {
   long long wait_limit;
 };
 
+// Maximum of three (one instruction).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // 16-bit rows of one head set to zero, lse to -inf: tokens behind the last sequence.
 __device__ __forceinline__ void clear_rows(const FwdParams& p, int row0, int rows, int head) {
   const int vec = p.D / 8;
@@ -92,6 +106,10 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
   const bool b_active = n_kv[1] > 0;
   const int n_max = b_active ? n_kv[1] : n_kv[0];
   const int head_kv = head[0] / p.group;
+  // halves of 64 keys; a last tile of at most 64 tokens has one
+  const int tail_rows = L - last_tile * kTile;  // valid rows of the sequence's last tile
+  const int n_half[2] = {2 * n_kv[0] - (qt[0] == last_tile && tail_rows <= 64),
+                         b_active ? 2 * n_kv[1] - (qt[1] == last_tile && tail_rows <= 64) : 0};
 
   extern __shared__ uint8_t smem_raw[];
   constexpr uint32_t TB = tile_bytes<HD>();
@@ -104,9 +122,10 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
   uint64_t* k_empty = bs.bars + 3;  // [2]
   uint64_t* v_full = bs.bars + 5;   // [2]
   uint64_t* v_empty = bs.bars + 7;  // [2]
-  uint64_t* s_full = bs.bars + 9;   // [2] tile A, tile B
-  uint64_t* p_full = bs.bars + 11;  // [2]
-  uint64_t* o_done = bs.bars + 13;
+  uint64_t* s_full = bs.bars + 9;    // [tile A, tile B][half]
+  uint64_t* p_full = bs.bars + 13;   // [tile A, tile B][half]
+  uint64_t* pv_done = bs.bars + 17;  // [tile A, tile B]
+  uint64_t* o_done = bs.bars + 19;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -115,8 +134,9 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
     for (int i = 0; i < 2; ++i) {
       mbar_init(k_full + i, 1); mbar_init(k_empty + i, 1);
       mbar_init(v_full + i, 1); mbar_init(v_empty + i, 1);
-      mbar_init(s_full + i, 1); mbar_init(p_full + i, 4);
+      mbar_init(pv_done + i, 1);
     }
+    for (int i = 0; i < 4; ++i) { mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); }
     fence_mbar_init();
     prefetch_tensormap(&map_q); prefetch_tensormap(&map_k); prefetch_tensormap(&map_v);
   }
@@ -127,10 +147,8 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
   tc_fence_after_sync();
   const uint32_t tmem = *bs.tmem_slot;
   const WaitCtx ctx{bs.abort_flag, &g_attn_packed_fwd_status, p.wait_limit};
-  constexpr uint32_t idesc_s = instr_desc_f16(FMT, 128, 128, 0, 0);
+  constexpr uint32_t idesc_s = instr_desc_f16(FMT, 128, 64, 0, 0);
   constexpr uint32_t idesc_o = instr_desc_f16(FMT, 128, HD, 0, 1);
-  const uint32_t tS[2] = {tmem, tmem + 128};
-  const uint32_t tO[2] = {tmem + 256, tmem + 384};
 
   if (warp == 0) {
     if (lane == 0) {
@@ -161,45 +179,58 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
     }
   } else if (warp == 1) {
     const bool lead = elect_one();
-    const int tail_rows = L - last_tile * kTile;  // valid rows of the sequence's last tile
+    // Scores of half g of tile w (0: A, 1: B): keys [64 hf, 64 hf + 64) of a K tile.
+    auto issue_s = [&](int w, int hf, const uint8_t* q_tile, const uint8_t* k_tile) {
+      const DescBase qb = desc_base_kmajor(smem_u32(q_tile));
+      const DescBase kb = desc_base_kmajor(smem_u32(k_tile) + hf * 64 * 128);
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)
+        if (lead)
+          mma_ss(tmem + w * 128 + hf * 64, desc_at(qb, kstep_kmajor(kTile, ks)),
+                 desc_at(kb, kstep_kmajor(kTile, ks)), idesc_s, ks > 0 ? 1u : 0u);
+      if (lead) mma_commit(s_full + 2 * w + hf);
+    };
+    auto issue_pv = [&](int w, int hf, const uint8_t* v_tile, bool first) {
+      const DescBase vb = desc_base_mnmajor(smem_u32(v_tile) + hf * 64 * 128, kTile);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+        if (lead)
+          mma_ts(tmem + 256 + w * 128, tmem + w * 128 + hf * 64 + ks * 8, desc_at(vb, kstep_mnmajor(ks)),
+                 idesc_o, (first && ks == 0) ? 0u : 1u);
+      if (lead) mma_commit(pv_done + w);
+    };
     mbar_wait(q_full, 0, ctx, 803);
     mbar_wait(k_full + 0, 0, ctx, 804);
     tc_fence_after_sync();
-    issue_scores<HD>(lead, tS[0], smem_u32(sQ[0]), smem_u32(sK[0]), idesc_s);
-    if (lead) mma_commit(s_full + 0);
-    if (b_active) {
-      issue_scores<HD>(lead, tS[1], smem_u32(sQ[1]), smem_u32(sK[0]), idesc_s);
-      if (lead) mma_commit(s_full + 1);
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      if (hf < n_half[0]) issue_s(0, hf, sQ[0], sK[0]);
+      if (hf < n_half[1]) issue_s(1, hf, sQ[1], sK[0]);
     }
     if (lead) mma_commit(k_empty + 0);
     for (int j = 0; j < n_max; ++j) {
-      const int st = j & 1, st1 = (j + 1) & 1;
-      const uint32_t ph = j & 1;
+      const int st = j & 1, st1 = st ^ 1;
+      const uint32_t par = j & 1;
       mbar_wait(v_full + st, (j >> 1) & 1, ctx, 805);
       if (j == last_tile && tail_rows < kTile) clear_tile_rows<HD>(sV[st], tail_rows, lane);
-      if (j < n_kv[0]) {
-        mbar_wait(p_full + 0, ph, ctx, 806);
-        tc_fence_after_sync();
-        issue_accumulate(lead, tO[0], tS[0], smem_u32(sV[st]), idesc_o, j > 0);
-      }
-      if (j + 1 < n_max) {
-        mbar_wait(k_full + st1, ((j + 1) >> 1) & 1, ctx, 807);
-        tc_fence_after_sync();
-      }
-      if (j + 1 < n_kv[0]) {
-        issue_scores<HD>(lead, tS[0], smem_u32(sQ[0]), smem_u32(sK[st1]), idesc_s);
-        if (lead) mma_commit(s_full + 0);
-      }
-      if (b_active) {
-        mbar_wait(p_full + 1, ph, ctx, 808);
-        tc_fence_after_sync();
-        issue_accumulate(lead, tO[1], tS[1], smem_u32(sV[st]), idesc_o, j > 0);
+      if (j + 1 < n_max) mbar_wait(k_full + st1, ((j + 1) >> 1) & 1, ctx, 807);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int g = 2 * j + hf;
+        if (g < n_half[0]) {
+          mbar_wait(p_full + hf, par, ctx, 806);
+          tc_fence_after_sync();
+          issue_pv(0, hf, sV[st], g == 0);
+          if (g + 2 < n_half[0]) issue_s(0, hf, sQ[0], sK[st1]);
+        }
+        if (g < n_half[1]) {
+          mbar_wait(p_full + 2 + hf, par, ctx, 808);
+          tc_fence_after_sync();
+          issue_pv(1, hf, sV[st], g == 0);
+          if (g + 2 < n_half[1]) issue_s(1, hf, sQ[1], sK[st1]);
+        }
       }
       if (lead) mma_commit(v_empty + st);
-      if (b_active && j + 1 < n_kv[1]) {
-        issue_scores<HD>(lead, tS[1], smem_u32(sQ[1]), smem_u32(sK[st1]), idesc_s);
-        if (lead) mma_commit(s_full + 1);
-      }
       if (lead && j + 1 < n_max) mma_commit(k_empty + st1);
       __syncwarp();
     }
@@ -212,50 +243,46 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
     const int row = quarter * 32 + lane;
     const int my_tile = wg ? qt[1] : qt[0], my_head = wg ? head[1] : head[0];
     const int q_pos = my_tile * kTile + row;  // position inside the sequence
-    const int n_mine = wg ? n_kv[1] : n_kv[0];
-    const uint32_t tSw = tmem + wg * 128, tOw = tmem + 256 + wg * 128;
+    const int n_mine = wg ? n_half[1] : n_half[0];
+    const uint32_t tOw = tmem + 256 + wg * 128;
     const float scale_log2 = p.scale_log2;
     float m_run = -INFINITY, l_run = 0.f;
-    for (int j = 0; j < n_mine; ++j) {
-      mbar_wait(s_full + wg, j & 1, ctx, 809);
+    for (int g = 0; g < n_mine; ++g) {
+      const int hf = g & 1;
+      const uint32_t tSw = tmem + wg * 128 + hf * 64 + lane_base;
+      mbar_wait(s_full + 2 * wg + hf, (g >> 1) & 1, ctx, 809);
       __syncwarp();
       tc_fence_after_sync();
-      // Pass 1: row maximum. Columns [0, 64) stay in registers for pass 2, [64, 96)
-      // arrive in the same round trip to tensor memory and [96, 128) while the first
-      // maxima are formed; four partial maxima keep the dependent chains short.
-      const int kv0 = j * kTile;
-      const bool diag = (j == my_tile);
-      uint32_t keep[64], tmp[32];
-      tmem_ld32(tSw + lane_base, *reinterpret_cast<uint32_t(*)[32]>(&keep[0]));
-      tmem_ld32(tSw + lane_base + 32, *reinterpret_cast<uint32_t(*)[32]>(&keep[32]));
-      tmem_ld32(tSw + lane_base + 64, tmp);
+      const int kv0 = g * 64;
+      const bool diag = (g >> 1) == my_tile;
+      uint32_t sr[64];
+      tmem_ld32(tSw, *reinterpret_cast<uint32_t(*)[32]>(&sr[0]));
+      tmem_ld32(tSw + 32, *reinterpret_cast<uint32_t(*)[32]>(&sr[32]));
       tmem_wait_ld();
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      auto fold = [&](const uint32_t* v, int col0, int n) {
-        if (diag) {
+      // Four partial maxima keep the comparisons from forming one long dependent chain.
+      float mx4[4];
+      if (diag) {
 #pragma unroll
-          for (int i = 0; i < n; ++i) {
-            float t = __uint_as_float(v[i]);
-            if (kv0 + col0 + i > q_pos) t = -INFINITY;
-            mx4[i & 3] = fmaxf(mx4[i & 3], t);
-          }
-        } else {
+        for (int i = 0; i < 64; ++i)
+          if (kv0 + i > q_pos) sr[i] = __float_as_uint(-INFINITY);
+      }
 #pragma unroll
-          for (int i = 0; i < n; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(v[i]));
-        }
-      };
-      fold(tmp, 64, 32);
-      tmem_ld32(tSw + lane_base + 96, tmp);
-      fold(keep, 0, 64);
-      tmem_wait_ld();
-      fold(tmp, 96, 32);
+      for (int i = 0; i < 4; ++i) mx4[i] = fmaxf(__uint_as_float(sr[i]), __uint_as_float(sr[i + 4]));
+#pragma unroll
+      for (int i = 8; i < 64; i += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mx4[k] = max3(mx4[k], __uint_as_float(sr[i + k]), __uint_as_float(sr[i + k + 4]));
       // scale_log2 > 0, so scaling commutes with the maximum
       const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale_log2;
-      const bool grow = mx > m_run + kRescaleThreshold;  // always true on the first tile
+      const bool grow = mx > m_run + kRescaleThreshold;  // always true on the first half
       const float m_new = grow ? mx : m_run;
-      if (j > 0 && __any_sync(0xffffffffu, grow)) {
-        // Rescale this warp's rows of O (rows that did not grow use alpha = 1). The
-        // previous O += P V has completed: the scores just read were issued after it.
+      if (g > 0 && __any_sync(0xffffffffu, grow)) {
+        // Rescale this warp's rows of O (rows that did not grow use alpha = 1) once the
+        // half before this one has been added.
+        mbar_wait(pv_done + wg, (g - 1) & 1, ctx, 811);
+        __syncwarp();
+        tc_fence_after_sync();
         const float alpha = grow ? fast_exp2(m_run - m_new) : 1.0f;
         l_run *= alpha;
 #pragma unroll
@@ -269,40 +296,36 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
         }
       }
       m_run = m_new;
-      // Pass 2: probabilities. The packed P of chunk c (16 columns) lands in columns
-      // [16c, 16c+16), which belong to score chunks already consumed. P is rounded to
-      // 16 bits as the tensor cores' operand; its sum is taken before rounding.
-      const float neg_m = -m_run;
-      float ls4[4] = {0.f, 0.f, 0.f, 0.f};
-      auto probs = [&](const uint32_t* v, int c) {
+      // Probabilities: 64 score columns -> 32 packed columns over them. P is rounded to 16
+      // bits as the tensor cores' operand; its sum is taken before rounding. A masked score
+      // of -infinity gives zero.
+      const f32x2 neg_m2 = f2_splat(-m_run), scale2 = f2_splat(scale_log2);
+      f32x2 ls2[2] = {0ull, 0ull};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
         uint32_t pr[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          float p0 = fast_exp2(fmaf(__uint_as_float(v[2 * i]), scale_log2, neg_m));
-          float p1 = fast_exp2(fmaf(__uint_as_float(v[2 * i + 1]), scale_log2, neg_m));
-          if (diag) {
-            if (kv0 + c * 32 + 2 * i > q_pos) p0 = 0.f;
-            if (kv0 + c * 32 + 2 * i + 1 > q_pos) p1 = 0.f;
-          }
-          ls4[i & 3] += p0 + p1;
-          pr[i] = pack2<FMT>(p0, p1);
+          const f32x2 x = f2_fma(f2_make(__uint_as_float(sr[32 * c + 2 * i]), __uint_as_float(sr[32 * c + 2 * i + 1])),
+                                 scale2, neg_m2);
+          float lo, hi;
+          f2_split(x, lo, hi);
+          lo = fast_exp2(lo);
+          hi = fast_exp2(hi);
+          ls2[i & 1] = f2_add(ls2[i & 1], f2_make(lo, hi));
+          pr[i] = pack2<FMT>(lo, hi);
         }
-        tmem_st16(tSw + lane_base + c * 16, pr);
-      };
-      // columns [64, 128) come back from tensor memory under the exponentials of [0, 64)
-      uint32_t late[32];
-      tmem_ld32(tSw + lane_base + 64, late);
-      probs(&keep[0], 0);
-      tmem_ld32(tSw + lane_base + 96, tmp);
-      probs(&keep[32], 1);
-      tmem_wait_ld();
-      probs(late, 2);
-      probs(tmp, 3);
-      l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
+        tmem_st16(tSw + c * 16, pr);
+      }
+      {
+        float a0, a1;
+        f2_split(f2_add(ls2[0], ls2[1]), a0, a1);
+        l_run += a0 + a1;
+      }
       tmem_wait_st();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + wg);
+      if (lane == 0) mbar_arrive(p_full + 2 * wg + hf);
     }
     if (n_mine > 0) {
       mbar_wait(o_done, 0, ctx, 810);

@@ -42,6 +42,7 @@ bool encode_view_map(CUtensorMap* map, const View& v, int fmt, int64_t D, int64_
 namespace {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kSharedWeights = 4096;  // tables in shared memory up to half a million tokens
 
 // Exclusive prefix sum over the block; `total` is the sum (same in all threads).
 __device__ int block_exclusive_scan(int v, int* warp_sums, int& total) {
@@ -74,10 +75,13 @@ packed_plan_kernel(const int* __restrict__ cu, int n_seq, int tokens, int slots,
                    int* __restrict__ plan) {
   __shared__ int warp_sums[32];
   __shared__ int s_valid;
+  __shared__ int tables[2 * kSharedWeights];
   int4* items = reinterpret_cast<int4*>(plan + kPlanHeader);
-  int* at_least = plan + kPlanHeader + 4 * slots;  // [max_w + 2] sequences with >= w tiles
-  int* item0 = at_least + max_w + 2;               // [max_w + 2] first item of weight w
-  int* rank = item0 + max_w + 2;                   // [n_seq] position among sequences by falling tiles
+  int* scratch = plan + kPlanHeader + 4 * slots;
+  const bool small = max_w + 2 <= kSharedWeights;
+  int* at_least = small ? tables : scratch;  // [max_w + 2] sequences with >= w tiles
+  int* item0 = at_least + max_w + 2;         // [max_w + 2] first item of weight w
+  int* rank = scratch + 2 * (max_w + 2);     // [n_seq] place among the sequences of equally many tiles
   const int tid = threadIdx.x;
 
   // Offsets must start at 0, never fall and end inside the token axis; anything else
