@@ -115,7 +115,8 @@ packed_generic_fwd_kernel(const GenericParams p) {
   if (lane == 0) p.lse_out[(int64_t)h * p.tokens + seq0 + i] = m + logf(l);
 }
 
-// delta = do . o, and dq of its row:  dq_i = scale * sum_{j<=i} p_ij (do_i.v_j - delta_i) k_j
+// delta_i = sum_{j<=i} p_ij do_i.v_j (from its definition: o is rounded), and dq of the row:
+// dq_i = scale * sum_{j<=i} p_ij (do_i.v_j - delta_i) k_j
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32)
 packed_generic_dq_kernel(const GenericParams p) {
@@ -134,18 +135,19 @@ packed_generic_dq_kernel(const GenericParams p) {
   }
   const T* qr = row_ptr<T>(p.q, seq0 + i, h);
   const T* gr = row_ptr<T>(p.dout, seq0 + i, h);
-  const T* orow = row_ptr<T>(p.o, seq0 + i, h);
-  float s0 = 0.f;
   for (int d = lane; d < D; d += 32) {
     qs[d] = to_f32<T>(qr[d]);
     gs[d] = to_f32<T>(gr[d]);
-    s0 = fmaf(gs[d], to_f32<T>(orow[d]), s0);
   }
   __syncwarp();
-  const float delta_i = warp_sum(s0);
   const int64_t stat = (int64_t)h * p.tokens + seq0 + i;
-  if (lane == 0) p.delta[stat] = delta_i;
   const float lse_i = p.lse[stat];
+  float sum = 0.f;
+  for (int j = lane; j <= i; j += 32)
+    sum += expf(p.scale * dot_row<T>(qs, row_ptr<T>(p.k, seq0 + j, g), D) - lse_i) *
+           dot_row<T>(gs, row_ptr<T>(p.v, seq0 + j, g), D);
+  const float delta_i = warp_sum(sum);
+  if (lane == 0) p.delta[stat] = delta_i;
   float acc[kMaxDT];
 #pragma unroll
   for (int t = 0; t < kMaxDT; ++t) acc[t] = 0.f;

@@ -525,10 +525,24 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
 
 // Row statistics of every item's query tile: delta = do . o and the log-sum-exp in log2
 // units, padded rows +inf / 0, and the tile's rows of the float32 dQ copy cleared.
+// In sequences of a few tokens dS = P (dP - delta) is often a small difference, to which
+// the rounding of o to 16 bits would contribute up to percents (two tokens: 4 %); there
+// delta is summed from its definition, sum_j P_ij do_i . v_j.
 // A block takes 256 / (HD / 8) rows of one head.
+constexpr int kShortSequence = 8;
+template <int FMT> __device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
+  float af[8], bf[8], s = 0.f;
+  if constexpr (FMT == 1) { unpack<__nv_bfloat16>(a, af); unpack<__nv_bfloat16>(b, bf); }
+  else { unpack<__half>(a, af); unpack<__half>(b, bf); }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += af[i] * bf[i];
+  return s;
+}
+
 template <int HD, int FMT>
 __global__ void __launch_bounds__(256)
-packed_prepare_kernel(const View dout, const View o, const float* __restrict__ lse, const BwdParams p) {
+packed_prepare_kernel(const View dout, const View q, const View o, const float* __restrict__ lse,
+                      const BwdParams p) {
   constexpr int TPR = HD / 8;
   constexpr int ROWS = 256 / TPR;
   const int4 item = plan_item(p.plan, blockIdx.x);
@@ -538,29 +552,35 @@ packed_prepare_kernel(const View dout, const View o, const float* __restrict__ l
   const int tile0 = (item.z - 1) * kTile;
   const int64_t prow0 = (int64_t)head * p.slots * kTile + (int64_t)item.w * kTile + tile0;
   for (int r = threadIdx.x / TPR + blockIdx.z * ROWS; r < kTile; r += ROWS * gridDim.z) {
-    const bool ok = tile0 + r < item.y;
+    const bool ok = tile0 + r < item.y, mine = ok && part * 8 < p.D;
     const int64_t token = item.x + tile0 + r;
-    float s = 0.f;
-    if (ok) {
-      if (part * 8 < p.D) {
-        const uint4 a = ld_vec(view_row(dout, token, head) + part * 16);
-        const uint4 b = ld_vec(view_row(o, token, head) + part * 16);
-        float af[8], bf[8];
-        if constexpr (FMT == 1) { unpack<__nv_bfloat16>(a, af); unpack<__nv_bfloat16>(b, bf); }
-        else { unpack<__half>(a, af); unpack<__half>(b, bf); }
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    const uint4 g = mine ? ld_vec(view_row(dout, token, head) + part * 16) : none;
+    auto row_sum = [&](float v) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += af[i] * bf[i];
+      for (int off = TPR / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+      return v;
+    };
+    const float lse_row = ok ? lse[(int64_t)head * p.tokens + token] : 0.f;
+    float s = 0.f;
+    if (item.y <= kShortSequence) {
+      const uint4 qv = mine ? ld_vec(view_row(q, token, head) + part * 16) : none;
+      for (int j = 0; j < item.y; ++j) {
+        const bool seen = mine && j <= r;
+        const float qk = row_sum(seen ? dot8<FMT>(qv, ld_vec(view_row(p.k, item.x + j, head / p.group) + part * 16)) : 0.f);
+        const float gv = row_sum(seen ? dot8<FMT>(g, ld_vec(view_row(p.v, item.x + j, head / p.group) + part * 16)) : 0.f);
+        if (j <= r) s += expf(p.scale * qk - lse_row) * gv;
       }
+    } else {
+      s = row_sum(mine ? dot8<FMT>(g, ld_vec(view_row(o, token, head) + part * 16)) : 0.f);
     }
     {
       uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (prow0 + r) * HD + part * 8);
       acc[0] = acc[1] = make_uint4(0, 0, 0, 0);
     }
-#pragma unroll
-    for (int off = TPR / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
     if (part == 0) {
       p.delta[prow0 + r] = ok ? s : 0.f;
-      p.lse2[prow0 + r] = ok ? lse[(int64_t)head * p.tokens + token] * kLog2e : INFINITY;
+      p.lse2[prow0 + r] = ok ? lse_row * kLog2e : INFINITY;
     }
   }
 }
@@ -639,7 +659,7 @@ int launch(const View& dout, const View& q, const View& o, const float* lse, Bwd
   const int64_t want = (4 * (int64_t)device_info().sm_count + tiles - 1) / tiles;
   const int parts = (int)(want < 1 ? 1 : want > kMostParts ? kMostParts : want);
   const dim3 rows_grid((unsigned)p.slots, (unsigned)Hq, (unsigned)parts);
-  packed_prepare_kernel<HD, FMT><<<rows_grid, 256, 0, stream>>>(dout, o, lse, p);
+  packed_prepare_kernel<HD, FMT><<<rows_grid, 256, 0, stream>>>(dout, q, o, lse, p);
   if (int rc = check_launch("packed_attention_bwd statistics")) return rc;
   kern<<<(unsigned)((int64_t)p.slots * p.units), kBwdThreads, smem, stream>>>(mq, mk, mdo, p);
   if (int rc = check_launch("packed_attention_bwd")) return rc;
