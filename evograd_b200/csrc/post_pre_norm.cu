@@ -686,14 +686,33 @@ Shape pick_shape(int64_t C, size_t elem, bool aligned, int arrays, int one_vecto
 // Most blocks a backward launches, and with that partial rows.
 int most_blocks() { return device_info().sm_count * 8; }
 
-template <typename Kernel>
-int blocks_for(Kernel kernel, const Shape& s, int64_t rows, size_t smem) {
+// Blocks of a kernel that fit an SM. Asking takes the host about as long as a launch, so
+// a thread remembers its last answers (a fixed property of kernel, block and device).
+int occupancy(const void* kernel, int threads, size_t smem) {
+  struct Known {
+    const void* kernel;
+    int device, threads, blocks;
+    size_t smem;
+  };
+  static thread_local Known known[8] = {};
+  static thread_local unsigned next = 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  for (const Known& k : known)
+    if (k.kernel == kernel && k.device == dev && k.threads == threads && k.smem == smem) return k.blocks;
   int occ = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, s.threads, smem) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, threads, smem) != cudaSuccess) {
     cudaGetLastError();
     occ = 1;
   }
   if (occ < 1) occ = 1;
+  known[next++ % 8] = Known{kernel, dev, threads, occ, smem};
+  return occ;
+}
+
+template <typename Kernel>
+int blocks_for(Kernel kernel, const Shape& s, int64_t rows, size_t smem) {
+  const int occ = occupancy((const void*)kernel, s.threads, smem);
   int64_t n = (int64_t)device_info().sm_count * occ;
   const int64_t per = !s.any && s.mode == kWarp ? s.threads / 32 : 1;
   const int64_t need = (rows + per - 1) / per;

@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+from array import array
 
 import torch
 
@@ -971,27 +972,24 @@ def _dense(t) -> bool:
 
 
 def _grad_list(grads, what):
-    """The tensors as a list, their device and dtype enums. One pass per property over the
-    whole list: a model has hundreds of them and the kernels take microseconds."""
+    """The tensors as a list, their device, dtype enums, addresses and element counts. One
+    pass per property over the whole list: a model has hundreds of tensors and the kernels
+    take microseconds."""
     grads = list(grads)
     if not grads:
         raise ValueError(f"{what}: no tensors")
-    if not all([isinstance(t, torch.Tensor) for t in grads]):
-        raise TypeError(f"{what}: expected tensors")
-    devices = {t.device for t in grads}
-    dev = grads[0].device
-    if len(devices) != 1 or dev.type != "cuda":
-        _require_cuda(*grads)
+    dev = _require_cuda(*grads)
     try:
         codes = [_DTYPES[t.dtype] for t in grads]
     except KeyError as e:
         raise TypeError(f"unsupported dtype {e.args[0]}; expected float32/float16/bfloat16") from None
-    if not all([t.is_contiguous() for t in grads]):
+    plain = [t.is_contiguous() for t in grads]
+    if not all(plain):
         for i, t in enumerate(grads):
-            if not _dense(t):
+            if not plain[i] and not _dense(t):
                 raise ValueError(f"{what}: tensor {i} has gaps or repeated elements "
                                  f"(strides {tuple(t.stride())})")
-    return grads, dev, codes
+    return grads, dev, codes, plain, [t.data_ptr() for t in grads], [t.numel() for t in grads]
 
 
 @functools.lru_cache(maxsize=256)
@@ -999,51 +997,52 @@ def _clip_bytes(count: int) -> int:
     return lib.evg_clip_grads_workspace_bytes(count)
 
 
-def _clip_call(grads, dev, codes, ptrs, out_ptrs, max_norm, clip):
-    n = len(grads)
+def _clip_call(dev, codes, ptrs, out_ptrs, numel, max_norm, clip):
+    n = len(ptrs)
     norm = torch.empty((), device=dev, dtype=torch.float32)
-    words = ctypes.c_int64 * n
     ws_bytes = _clip_bytes(n)
     ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-    _enqueue(dev, "evg_clip_grads", words(*ptrs), None if out_ptrs is None else words(*out_ptrs),
-             words(*[t.numel() for t in grads]), (ctypes.c_int * n)(*codes), n, float(max_norm),
-             1 if clip else 0, norm.data_ptr(), ws.data_ptr(), ws_bytes)
+    # host arrays, read before the call returns
+    aptr, asize, akind = array("Q", ptrs), array("q", numel), array("i", codes)
+    aout = None if out_ptrs is None else array("Q", out_ptrs)
+    _enqueue(dev, "evg_clip_grads", aptr.buffer_info()[0], None if aout is None else aout.buffer_info()[0],
+             asize.buffer_info()[0], akind.buffer_info()[0], n, float(max_norm), 1 if clip else 0,
+             norm.data_ptr(), ws.data_ptr(), ws_bytes)
     return norm
 
 
 def grad_norm(grads) -> torch.Tensor:
     """2-norm over all elements of all tensors (float32 / float16 / bfloat16, mixed), as a
     float32 scalar on their device."""
-    grads, dev, codes = _grad_list(grads, "grad_norm")
-    return _clip_call(grads, dev, codes, [t.data_ptr() for t in grads], None, 0.0, False)
+    _, dev, codes, _, ptrs, numel = _grad_list(grads, "grad_norm")
+    return _clip_call(dev, codes, ptrs, None, numel, 0.0, False)
 
 
 def clip_grad_norm(grads, max_norm: float, outs=None) -> torch.Tensor:
     """Scale all tensors by ``min(1, max_norm / (norm + 1e-6))`` with ``norm`` their global
-    2-norm, in place or into ``outs`` (same shapes, types and strides; not overlapping the
-    gradients unless it is them). Returns the norm before clipping, a float32 scalar on the
-    device; nothing is read back. A norm that is not finite scales as the formula says
-    (infinite: finite elements to zero; NaN: everything to NaN). The same tensor must not
-    be listed twice."""
-    grads, dev, codes = _grad_list(grads, "clip_grad_norm")
+    2-norm, in place or into ``outs`` (per gradient a tensor of its type with as many
+    elements in the same memory order, which must not overlap the gradients unless it is
+    them). Returns the norm before clipping, a float32 scalar on the device; nothing is
+    read back. A norm that is not finite scales as the formula says (infinite: finite
+    elements to zero; NaN: everything to NaN). The same tensor must not be listed twice."""
+    grads, dev, codes, plain, ptrs, numel = _grad_list(grads, "clip_grad_norm")
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    ptrs = [t.data_ptr() for t in grads]
     out_ptrs = None
     if outs is not None:
-        outs, odev, ocodes = _grad_list(outs, "clip_grad_norm outs")
+        outs, odev, ocodes, oplain, out_ptrs, onumel = _grad_list(outs, "clip_grad_norm outs")
         if odev != dev:
             raise RuntimeError(f"tensors on different devices: {dev} and {odev}")
-        if ocodes != codes or [t.shape for t in outs] != [t.shape for t in grads] or \
-                [t.stride() for t in outs] != [t.stride() for t in grads]:
-            raise ValueError("outs must have the shapes, dtypes and strides of their gradients")
-        out_ptrs = [t.data_ptr() for t in outs]
+        if ocodes != codes or onumel != numel or oplain != plain or (not all(plain) and any(
+                not c and (o.shape != t.shape or o.stride() != t.stride())
+                for o, t, c in zip(outs, grads, plain))):
+            raise ValueError("outs must have the types, sizes and memory order of their gradients")
     written = out_ptrs or ptrs
     # (an empty tensor has no address of its own)
     if len(set(written)) != len(written) and \
-            len({p for p, t in zip(written, grads) if t.numel()}) != sum([1 for t in grads if t.numel()]):
+            len({p for p, n in zip(written, numel) if n}) != sum(1 for n in numel if n):
         raise ValueError("clip_grad_norm: the same tensor is listed twice")
-    return _clip_call(grads, dev, codes, ptrs, out_ptrs, max_norm, True)
+    return _clip_call(dev, codes, ptrs, out_ptrs, numel, max_norm, True)
 
 
 # ------------------------------------------------------------- evoattention
