@@ -16,7 +16,9 @@
 // memory until the end (fixed order, no atomics). dQ^T also belongs to other blocks'
 // rows: four warps of their own send it to a float32 copy of dQ by asynchronous bulk
 // reductions, so dq can differ in the last bit from run to run; a last kernel scales and
-// rounds the copy.
+// rounds the copy. A sequence's first query tile meets one key tile only: its dQ is rounded
+// and written at once and has no float32 copy (128 sequences of 128 tokens, 32/8 heads:
+// 368 us with one).
 //
 // K and V are kept in tensor memory as well (64 columns each): a product of two
 // shared-memory operands with 64 columns needs 192 bytes a clock of the shared memory's
@@ -369,7 +371,17 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
         for (int h = 0; h < 2; ++h) {
           if (issuer) bulk_wait_read<1>();  // this piece's last reduction has read it
           named_barrier_sync(1, 128);
-          if (r.row < HD) {
+          const bool whole = kvt + it == 0;
+          if (whole) {
+            // A sequence's first query tile gets its whole dQ here: rounded, as 16-bit rows
+            // [query][head column], 256 contiguous bytes per query on the way out.
+            uint16_t* dst = reinterpret_cast<uint16_t*>(sDQ + h * kPiece) + r.row;
+            if (r.row < HD) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                dst[j * HD] = (uint16_t)pack2<FMT>(__uint_as_float(acc[h][j]) * p.scale, 0.f);
+            }
+          } else if (r.row < HD) {
             uint4* dst = reinterpret_cast<uint4*>(sDQ + h * kPiece) + r.row;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -377,7 +389,19 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
           }
           fence_proxy_async_smem();
           named_barrier_sync(1, 128);
-          if (issuer && !*ctx.abort_flag) bulk_add_f32(tile_dst + (b * 64 + h * 32) * HD, sDQ + h * kPiece, kPiece);
+          if (whole) {
+            constexpr int TPR = HD / 8;
+            const int t = threadIdx.x & 127, part = t % TPR;
+            const uint4* src = reinterpret_cast<const uint4*>(sDQ + h * kPiece) + t;
+#pragma unroll
+            for (int u = 0; u < 32 * TPR / 128; ++u) {
+              const int query = b * 64 + h * 32 + t / TPR + u * (128 / TPR);
+              if (query < L && part * 8 < p.D)
+                reinterpret_cast<uint4*>(view_row(p.dq, seq0 + query, head))[part] = src[u * 128];
+            }
+          } else if (issuer && !*ctx.abort_flag) {
+            bulk_add_f32(tile_dst + (b * 64 + h * 32) * HD, sDQ + h * kPiece, kPiece);
+          }
         }
       }
       if (++it == n_it) { it = 0; ++head; }
@@ -524,7 +548,8 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
 }
 
 // Row statistics of every item's query tile: delta = do . o and the log-sum-exp in log2
-// units, padded rows +inf / 0, and the tile's rows of the float32 dQ copy cleared.
+// units, padded rows +inf / 0, and the tile's rows of the float32 dQ copy cleared (a
+// sequence's first tile has none).
 // In sequences of a few tokens dS = P (dP - delta) is often a small difference, to which
 // the rounding of o to 16 bits would contribute up to percents (two tokens: 4 %); there
 // delta is summed from its definition, sum_j P_ij do_i . v_j.
@@ -574,7 +599,7 @@ packed_prepare_kernel(const View dout, const View q, const View o, const float* 
     } else {
       s = row_sum(mine ? dot8<FMT>(g, ld_vec(view_row(o, token, head) + part * 16)) : 0.f);
     }
-    {
+    if (tile0 > 0) {
       uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (prow0 + r) * HD + part * 8);
       acc[0] = acc[1] = make_uint4(0, 0, 0, 0);
     }
@@ -593,7 +618,7 @@ packed_finish_kernel(const BwdParams p) {
   constexpr int TPR = HD / 8;
   constexpr int QUADS = 256 / TPR;  // groups of 4 queries per round
   const int4 item = plan_item(p.plan, blockIdx.x);
-  if (item.z < 0) return;
+  if (item.z < 0 || item.z == 1) return;  // first tiles are written by the products' kernel
   const int head = blockIdx.y;
   const int part = threadIdx.x % TPR;
   if (part * 8 >= p.D) return;
