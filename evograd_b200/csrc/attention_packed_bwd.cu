@@ -16,9 +16,10 @@
 // memory until the end (fixed order, no atomics). dQ^T also belongs to other blocks'
 // rows: four warps of their own send it to a float32 copy of dQ by asynchronous bulk
 // reductions, so dq can differ in the last bit from run to run; a last kernel scales and
-// rounds the copy. A sequence's first query tile meets one key tile only: its dQ is rounded
-// and written at once and has no float32 copy (128 sequences of 128 tokens, 32/8 heads:
-// 368 us with one).
+// rounds the copy. A sequence of one tile has no float32 copy, its dQ is rounded and written
+// at once (128 sequences of 128 tokens, 32/8 heads of 128: 367 -> 283 us; doing the same
+// for the first tile of longer sequences, whose other blocks wait meanwhile, was 5 % slower
+// on 16 sequences of 1 to 900 tokens).
 //
 // K and V are kept in tensor memory as well (64 columns each): a product of two
 // shared-memory operands with 64 columns needs 192 bytes a clock of the shared memory's
@@ -96,32 +97,37 @@ __device__ __forceinline__ uint8_t* view_row(const View& v, int64_t token, int h
   return reinterpret_cast<uint8_t*>(v.p) + (token * v.st + (int64_t)head * v.sh) * 2;
 }
 
-// Rows of a [128 x HD] float32 accumulator in tensor memory -> 16-bit rows of a View;
-// the column groups of compute warps take HD / kCG columns each.
+// A [128 x HD] float32 accumulator in tensor memory -> 16-bit rows of a tile in shared
+// memory, 16-byte pieces XORed with the row (the compute warps; column groups of HD / kCG).
 template <int HD, int FMT>
-__device__ __forceinline__ void store_view_rows(uint32_t t_acc, const View& out, int head, int seq0,
-                                                int row0, int L, int D, float scale, const Roles& r) {
+__device__ __forceinline__ void accumulator_to_tile(uint32_t t_acc, uint8_t* tile, float scale, const Roles& r) {
   constexpr int CW = HD / kCG;  // 32 or 16 columns per warp
-  const uint32_t lane_base = (uint32_t)(r.quarter * 32) << 16;
-  const int row = row0 + r.row;
-  const bool ok = row < L;
-  uint8_t* dst = view_row(out, seq0 + (ok ? row : 0), head);
   const int col = r.half * CW;
   uint32_t acc[CW];
   __syncwarp();
-  tmem_ld(t_acc + lane_base + col, acc);
+  tmem_ld(t_acc + ((uint32_t)(r.quarter * 32) << 16) + col, acc);
   tmem_wait_ld();
-  if (!ok) return;
 #pragma unroll
   for (int v = 0; v < CW / 8; ++v) {
-    if (col + v * 8 < D) {
-      uint4 pk;
-      pk.x = pack2<FMT>(__uint_as_float(acc[8 * v + 0]) * scale, __uint_as_float(acc[8 * v + 1]) * scale);
-      pk.y = pack2<FMT>(__uint_as_float(acc[8 * v + 2]) * scale, __uint_as_float(acc[8 * v + 3]) * scale);
-      pk.z = pack2<FMT>(__uint_as_float(acc[8 * v + 4]) * scale, __uint_as_float(acc[8 * v + 5]) * scale);
-      pk.w = pack2<FMT>(__uint_as_float(acc[8 * v + 6]) * scale, __uint_as_float(acc[8 * v + 7]) * scale);
-      *reinterpret_cast<uint4*>(dst + (col + v * 8) * 2) = pk;
-    }
+    uint4 pk;
+    pk.x = pack2<FMT>(__uint_as_float(acc[8 * v + 0]) * scale, __uint_as_float(acc[8 * v + 1]) * scale);
+    pk.y = pack2<FMT>(__uint_as_float(acc[8 * v + 2]) * scale, __uint_as_float(acc[8 * v + 3]) * scale);
+    pk.z = pack2<FMT>(__uint_as_float(acc[8 * v + 4]) * scale, __uint_as_float(acc[8 * v + 5]) * scale);
+    pk.w = pack2<FMT>(__uint_as_float(acc[8 * v + 6]) * scale, __uint_as_float(acc[8 * v + 7]) * scale);
+    reinterpret_cast<uint4*>(tile)[r.row * (HD / 8) + ((col / 8 + v) ^ (r.row & 7))] = pk;
+  }
+}
+// That tile's rows inside the sequence -> a View, whole rows at a time (`t`: 0 .. 511).
+template <int HD>
+__device__ __forceinline__ void tile_to_view(const uint8_t* tile, const View& out, int head, int seq0,
+                                             int row0, int L, int D, int t) {
+  constexpr int TPR = HD / 8;
+#pragma unroll
+  for (int i = t; i < kTile * TPR; i += 32 * kComputeWarps) {
+    const int row = i / TPR, piece = i % TPR;
+    if (row0 + row < L && piece * 8 < D)
+      reinterpret_cast<uint4*>(view_row(out, seq0 + row0 + row, head))[piece] =
+          reinterpret_cast<const uint4*>(tile)[row * TPR + (piece ^ (row & 7))];
   }
 }
 
@@ -129,6 +135,7 @@ template <int HD, int FMT>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ CUtensorMap map_do, const BwdParams p) {
   // Key tile n - w of a sequence of n tiles: w query tiles to visit, heaviest first.
   int slot, bh;
@@ -168,7 +175,7 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   uint8_t* sDS = sQ0 + 2 * TB;   // dS^T of the streams
   uint8_t* sDQ = sDS + 2 * kChunkBytes;  // float32 dQ on its way out, two pieces of 32 queries
   float* s_stat = reinterpret_cast<float*>(sDQ + TB);  // [stage][lse2 | delta][128]
-  uint64_t* kv_full = bs.bars + 0;   // K in shared memory, K and V in tensor memory
+  uint64_t* kv_full = bs.bars + 0;   // K and V in tensor memory
   uint64_t* q_full = bs.bars + 1;    // [2] by stage
   uint64_t* q_empty = bs.bars + 3;   // [2]
   uint64_t* do_full = bs.bars + 5;   // [2]
@@ -180,13 +187,13 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   uint64_t* ds_full = bs.bars + 17;   // [2] dS^T is in shared memory
   uint64_t* dq_full = bs.bars + 19;   // [2]
   uint64_t* d_free = bs.bars + 21;    // [2] dQ^T has been read
-  uint64_t* done = bs.bars + 23;
+  uint64_t* done = bs.bars + 23;      // K and V in shared memory; then: all products finished
   const Roles r = roles();
   const float scale_log2 = p.scale * kLog2e;
 
   if (threadIdx.x == 0) {
     *bs.abort_flag = 0;
-    mbar_init(kv_full, 1 + kComputeWarps); mbar_init(done, 1);
+    mbar_init(kv_full, kComputeWarps); mbar_init(done, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1); mbar_init(q_empty + i, 1);
       mbar_init(do_full + i, 1); mbar_init(do_empty + i, 1);
@@ -195,7 +202,8 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
       mbar_init(ds_full + i, kStreamWarps); mbar_init(dq_full + i, 1); mbar_init(d_free + i, 4);
     }
     fence_mbar_init();
-    prefetch_tensormap(&map_q); prefetch_tensormap(&map_k); prefetch_tensormap(&map_do);
+    prefetch_tensormap(&map_q); prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v); prefetch_tensormap(&map_do);
   }
   __syncthreads();
   if (r.warp == 1) { tmem_alloc(bs.tmem_slot, 512); tmem_relinquish(); }
@@ -212,8 +220,9 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   const uint32_t tDV = tmem + 256, tDK = tmem + 384;
 
   if (r.is_tma && r.lane == 0) {
-    mbar_expect_tx(kv_full, TB);
-    load_tile<HD>(sK, &map_k, seq0 + kv0, bh, kv_full);
+    mbar_expect_tx(done, 2 * TB);
+    load_tile<HD>(sK, &map_k, seq0 + kv0, bh, done);
+    load_tile<HD>(sDS, &map_v, seq0 + kv0, bh, done);  // V only passes through
     int it = 0, head = bh * p.group, git = 0;
     for (; git < n_git; ++git) {
       const int st = git & 1;
@@ -235,7 +244,7 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     if (*ctx.abort_flag) {
       // Let the copies still in flight land before the block returns: each of
       // these waits gives up after the same cycle budget.
-      mbar_drain(kv_full, 0, p.wait_limit);
+      mbar_drain(done, 0, p.wait_limit);
       for (int g = git > 2 ? git - 2 : 0; g < git; ++g) {
         mbar_drain(q_full + (g & 1), (uint32_t)((g >> 1) & 1), p.wait_limit);
         mbar_drain(do_full + (g & 1), (uint32_t)((g >> 1) & 1), p.wait_limit);
@@ -367,40 +376,34 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
         tmem_ld(tY0 + 64 * b + lane_base + 32, acc[1]);
         tmem_wait_ld();
         warp_arrive(d_free + b, r.lane);
+        if (last_tile == 0) {
+          // A sequence of one tile gets its whole dQ here: rounded and written at once, 64
+          // contiguous bytes per warp and query.
+          if (r.row < p.D) {
+            uint8_t* dst = view_row(p.dq, seq0 + b * 64, head) + r.row * 2;
+            const int n = L - b * 64;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (issuer) bulk_wait_read<1>();  // this piece's last reduction has read it
-          named_barrier_sync(1, 128);
-          const bool whole = kvt + it == 0;
-          if (whole) {
-            // A sequence's first query tile gets its whole dQ here: rounded, as 16-bit rows
-            // [query][head column], 256 contiguous bytes per query on the way out.
-            uint16_t* dst = reinterpret_cast<uint16_t*>(sDQ + h * kPiece) + r.row;
-            if (r.row < HD) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                dst[j * HD] = (uint16_t)pack2<FMT>(__uint_as_float(acc[h][j]) * p.scale, 0.f);
+            for (int j = 0; j < 64; ++j) {
+              if (j < n)
+                *reinterpret_cast<uint16_t*>(dst) =
+                    (uint16_t)pack2<FMT>(__uint_as_float(acc[j >> 5][j & 31]) * p.scale, 0.f);
+              dst += p.dq.st * 2;
             }
-          } else if (r.row < HD) {
-            uint4* dst = reinterpret_cast<uint4*>(sDQ + h * kPiece) + r.row;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              dst[j * HD] = make_uint4(acc[h][4 * j], acc[h][4 * j + 1], acc[h][4 * j + 2], acc[h][4 * j + 3]);
           }
-          fence_proxy_async_smem();
-          named_barrier_sync(1, 128);
-          if (whole) {
-            constexpr int TPR = HD / 8;
-            const int t = threadIdx.x & 127, part = t % TPR;
-            const uint4* src = reinterpret_cast<const uint4*>(sDQ + h * kPiece) + t;
+        } else {
 #pragma unroll
-            for (int u = 0; u < 32 * TPR / 128; ++u) {
-              const int query = b * 64 + h * 32 + t / TPR + u * (128 / TPR);
-              if (query < L && part * 8 < p.D)
-                reinterpret_cast<uint4*>(view_row(p.dq, seq0 + query, head))[part] = src[u * 128];
+          for (int h = 0; h < 2; ++h) {
+            if (issuer) bulk_wait_read<1>();  // this piece's last reduction has read it
+            named_barrier_sync(1, 128);
+            if (r.row < HD) {
+              uint4* dst = reinterpret_cast<uint4*>(sDQ + h * kPiece) + r.row;
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                dst[j * HD] = make_uint4(acc[h][4 * j], acc[h][4 * j + 1], acc[h][4 * j + 2], acc[h][4 * j + 3]);
             }
-          } else if (issuer && !*ctx.abort_flag) {
-            bulk_add_f32(tile_dst + (b * 64 + h * 32) * HD, sDQ + h * kPiece, kPiece);
+            fence_proxy_async_smem();
+            named_barrier_sync(1, 128);
+            if (issuer && !*ctx.abort_flag) bulk_add_f32(tile_dst + (b * 64 + h * 32) * HD, sDQ + h * kPiece, kPiece);
           }
         }
       }
@@ -416,22 +419,26 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     const f32x2 neg_scale2 = f2_splat(-scale_log2);
     const f32x2 minus_one2 = f2_splat(-1.0f);
     // Stream 0's warps put K, stream 1's V into tensor memory: a thread its key's row (half
-    // of it), two 16-bit elements per column, zero behind the sequence's end and behind D.
+    // of it), two 16-bit elements per column, zero behind the sequence's end. (Read from
+    // global memory row by row this took 8500 cycles per block.)
     {
-      const View& src = b ? p.v : p.k;
+      mbar_wait(done, 0, ctx, 849);
+      const uint8_t* src = (b ? sDS : sK) + r.row * 128;
       const bool ok = kv_pos < L;
-      const uint8_t* g = view_row(src, seq0 + (ok ? kv_pos : 0), bh);
-      const int e0 = col0 / 32 * (HD / 2);  // first element
-      uint32_t w[HD / 4];
+      constexpr int PW = HD / 16;  // 16-byte pieces per warp, all in one 64-column atom
+      const int piece0 = (col0 / 32) * PW;
+      uint32_t w[4 * PW];
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (ok && e0 + 8 * i < p.D) x = *reinterpret_cast<const uint4*>(g + (e0 + 8 * i) * 2);
+      for (int i = 0; i < PW; ++i) {
+        const int piece = piece0 + i;
+        const uint4 x = ok ? *reinterpret_cast<const uint4*>(src + (piece >> 3) * (kTile * 128) +
+                                                             (((piece & 7) ^ (r.row & 7)) << 4))
+                           : make_uint4(0, 0, 0, 0);
         w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
       }
-      const uint32_t dst = (b ? tV : tK) + lane_base + e0 / 2;
+      const uint32_t dst = (b ? tV : tK) + lane_base + piece0 * 4;
 #pragma unroll
-      for (int i = 0; i < HD / 64; ++i) tmem_st(dst + 16 * i, *reinterpret_cast<uint32_t(*)[16]>(&w[16 * i]));
+      for (int i = 0; i < PW / 4; ++i) tmem_st(dst + 16 * i, *reinterpret_cast<uint32_t(*)[16]>(&w[16 * i]));
       tmem_wait_st();
       warp_arrive(kv_full, r.lane);
     }
@@ -536,11 +543,16 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
       if (r.lane == 0) mbar_arrive(ds_full + b);
       if (++it == n_it) it = 0;
     }
-    mbar_wait(done, 0, ctx, 847);
+    // dV and dK through the dO stages, which no product reads any more
+    mbar_wait(done, 1, ctx, 847);
     __syncwarp();
     tc_fence_after_sync();
-    store_view_rows<HD, FMT>(tDV, p.dv, bh, seq0, kv0, L, p.D, 1.0f, r);
-    store_view_rows<HD, FMT>(tDK, p.dk, bh, seq0, kv0, L, p.D, p.scale, r);
+    accumulator_to_tile<HD, FMT>(tDV, sDO0, 1.0f, r);
+    accumulator_to_tile<HD, FMT>(tDK, sDO0 + TB, p.scale, r);
+    named_barrier_sync(2, 32 * kComputeWarps);
+    const int t = (r.warp - 2) * 32 + r.lane;
+    tile_to_view<HD>(sDO0, p.dv, bh, seq0, kv0, L, p.D, t);
+    tile_to_view<HD>(sDO0 + TB, p.dk, bh, seq0, kv0, L, p.D, t);
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -549,7 +561,7 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
 
 // Row statistics of every item's query tile: delta = do . o and the log-sum-exp in log2
 // units, padded rows +inf / 0, and the tile's rows of the float32 dQ copy cleared (a
-// sequence's first tile has none).
+// sequence of one tile has none).
 // In sequences of a few tokens dS = P (dP - delta) is often a small difference, to which
 // the rounding of o to 16 bits would contribute up to percents (two tokens: 4 %); there
 // delta is summed from its definition, sum_j P_ij do_i . v_j.
@@ -599,7 +611,7 @@ packed_prepare_kernel(const View dout, const View q, const View o, const float* 
     } else {
       s = row_sum(mine ? dot8<FMT>(g, ld_vec(view_row(o, token, head) + part * 16)) : 0.f);
     }
-    if (tile0 > 0) {
+    if (item.y > kTile) {
       uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (prow0 + r) * HD + part * 8);
       acc[0] = acc[1] = make_uint4(0, 0, 0, 0);
     }
@@ -618,7 +630,7 @@ packed_finish_kernel(const BwdParams p) {
   constexpr int TPR = HD / 8;
   constexpr int QUADS = 256 / TPR;  // groups of 4 queries per round
   const int4 item = plan_item(p.plan, blockIdx.x);
-  if (item.z < 0 || item.z == 1) return;  // first tiles are written by the products' kernel
+  if (item.z < 0 || (item.z > 0 && item.y <= kTile)) return;  // one tile: written by the products' kernel
   const int head = blockIdx.y;
   const int part = threadIdx.x % TPR;
   if (part * 8 >= p.D) return;
@@ -667,9 +679,10 @@ const bool g_packed_bwd_registered = (register_device_status(read_packed_bwd_sta
 
 template <int HD, int FMT>
 int launch(const View& dout, const View& q, const View& o, const float* lse, BwdParams& p, int64_t Hq, int64_t Hkv, cudaStream_t stream) {
-  CUtensorMap mq, mk, mdo;
+  CUtensorMap mq, mk, mv, mdo;
   if (!encode_view_map(&mq, q, FMT, p.D, p.tokens, Hq) ||
       !encode_view_map(&mk, p.k, FMT, p.D, p.tokens, Hkv) ||
+      !encode_view_map(&mv, p.v, FMT, p.D, p.tokens, Hkv) ||
       !encode_view_map(&mdo, dout, FMT, p.D, p.tokens, Hq))
     return fail(EVG_ELAUNCH, "packed_attention_bwd: cuTensorMapEncodeTiled failed");
   size_t smem = bwd_tile_region<HD>() + kControlBytes + 1024;
@@ -686,7 +699,7 @@ int launch(const View& dout, const View& q, const View& o, const float* lse, Bwd
   const dim3 rows_grid((unsigned)p.slots, (unsigned)Hq, (unsigned)parts);
   packed_prepare_kernel<HD, FMT><<<rows_grid, 256, 0, stream>>>(dout, q, o, lse, p);
   if (int rc = check_launch("packed_attention_bwd statistics")) return rc;
-  kern<<<(unsigned)((int64_t)p.slots * p.units), kBwdThreads, smem, stream>>>(mq, mk, mdo, p);
+  kern<<<(unsigned)((int64_t)p.slots * p.units), kBwdThreads, smem, stream>>>(mq, mk, mv, mdo, p);
   if (int rc = check_launch("packed_attention_bwd")) return rc;
   packed_finish_kernel<HD, FMT><<<rows_grid, 256, 0, stream>>>(p);
   return check_launch("packed_attention_bwd dq");
