@@ -18,9 +18,10 @@
 // (6.2 TB/s), backward 136 us (5.9 TB/s with its column sums).
 //
 // A row belongs to one warp (up to 64 16-byte vectors) or to one block whose threads
-// hold V vectors each and whose next rows come through a shared-memory ring; blocks are persistent, a thread keeps its columns for all its
-// rows, so the weights and the column sums stay in registers. Column sums leave as one
-// float32 partial row per block and are added by a second kernel in a fixed order.
+// hold V vectors each and whose next rows come through a shared-memory ring; blocks are
+// persistent, a thread keeps its columns for all its rows, so the weights and the column
+// sums stay in registers. Column sums leave as one float32 partial row per block and are
+// added by a second kernel in a fixed order.
 #include "evg_common.cuh"
 #include "sm100_umma.cuh"
 
@@ -256,6 +257,7 @@ post_pre_fwd_kernel(const NormArgs a) {
   const int64_t stride = MODE == kWarp ? (int64_t)gridDim.x * (blockDim.x / 32) : gridDim.x;
   int64_t row = MODE == kWarp ? (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
   if (threadIdx.x < 64) scratch[threadIdx.x] = 0.f;
+  if constexpr (MODE == kDirect) __syncthreads();  // the ring's start has one
   Rows<NA, MODE> in;
   in.base[0] = (const uint8_t*)a.x;
   in.base[1] = (const uint8_t*)a.h;
