@@ -3,21 +3,24 @@
 //   s_ij = scale q_i . k_j (j <= i, same sequence),  o_i = sum_j softmax_j(s_ij) v_j,
 //   lse_i = log sum_j exp(s_ij)
 //
-// 320 threads per block: a TMA producer warp, a tcgen05 issuer warp and two groups
-// of four softmax warps, each group with a 128-row query tile of its own, so one tile's
-// softmax runs while the other tile's products do. Keys come in tiles of 128 and are
-// worked through in halves of 64: each group has two score buffers, and while it turns
-// one half's scores into probabilities the other half's are being formed, so its warps
-// never wait for a product that waits for them (with one 128-key buffer per group the
-// chain scores -> softmax -> PV -> next scores took 3980 cycles per key tile). Per half g:
+// A TMA producer warp, a tcgen05 issuer warp and one or two groups of four softmax warps,
+// each group with a 128-row query tile of its own, so one tile's softmax runs while the
+// other's products do: two groups share a block's key tiles, or two blocks of one group
+// share the SM (the rule is at launch_fwd). Keys come in tiles of 128 and are worked
+// through in halves of 64: each group has two score buffers, and while it turns one half's
+// scores into probabilities the other half's are being formed, so its warps never wait for
+// a product that waits for them (with one 128-key buffer per group the chain
+// scores -> softmax -> PV -> next scores took 3980 cycles per key tile). Per half g:
 //   O_A += P_A(g) V_g;  S_A(g+2) = Q_A K_{g+2}^T;  O_B += P_B(g) V_g;  S_B(g+2) = ...
-// TMEM: score buffers A [0,128), B [128,256) (P packed over the scores it came from),
-// O_A [256,256+HD), O_B [384,384+HD).
+// TMEM of G groups: score buffers [128 w, 128 w + 128) of group w (P packed over the scores
+// it came from), O [128 G + 128 w, 128 G + 128 w + HD).
 //
-// The two query tiles of a block share their key tiles. Where the query heads of a
-// k/v head can be paired (an even group), they are the SAME positions of two heads:
-// both tiles are equally long and a sequence of one tile still fills both groups.
-// Otherwise they are two neighbouring tiles of one head.
+// Where the query heads of a k/v head can be paired (an even group), a block's two tiles
+// are the SAME positions of two heads: both are equally long and a sequence of one tile
+// still fills both groups. Otherwise they are two neighbouring tiles of one head.
+//
+// O leaves through shared memory as whole rows: with a thread writing its own row, 128
+// sequences of 128 tokens (32/8 heads of 128) took 143 us, now 134.
 //
 // Tiles start at the sequence's first token (a TMA coordinate along the token axis
 // has no alignment rule). The last tile's rows behind the sequence's end are other
@@ -41,7 +44,12 @@ using namespace umma;
 using namespace attn;
 using namespace packed;
 
-constexpr int kFwdThreads = 320;
+// TILES query tiles per block: 2, or 1 with two blocks on an SM.
+constexpr int fwd_threads(int tiles) { return 64 + 128 * tiles; }
+// Stages of the K and V rings. One tile per block at head size 128 has room for one: the
+// other block's work covers the wait.
+template <int HD, int TILES> __host__ __device__ constexpr int fwd_stages() { return TILES == 1 && HD == 128 ? 1 : 2; }
+template <int HD, int TILES> __host__ __device__ constexpr int fwd_smem_tiles() { return TILES + 2 * fwd_stages<HD, TILES>(); }
 
 struct FwdParams {
   const int* plan;
@@ -49,7 +57,7 @@ struct FwdParams {
   int64_t o_st, o_sh;
   float* lse;
   int tokens, slots, units, head_group, group, D;
-  int pair_heads;  // the block's two tiles are two heads (else two neighbouring tiles)
+  int pair_heads;  // two tiles: of two heads (else two neighbouring tiles of one)
   float scale_log2;
   long long wait_limit;
 };
@@ -64,17 +72,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 __device__ __forceinline__ void clear_rows(const FwdParams& p, int row0, int rows, int head) {
   const int vec = p.D / 8;
   uint8_t* o = reinterpret_cast<uint8_t*>(p.o);
-  for (int i = threadIdx.x; i < rows * vec; i += kFwdThreads) {
+  for (int i = threadIdx.x; i < rows * vec; i += blockDim.x) {
     const int r = i / vec, c = i % vec;
     *reinterpret_cast<uint4*>(o + ((int64_t)(row0 + r) * p.o_st + (int64_t)head * p.o_sh + c * 8) * 2) =
         make_uint4(0, 0, 0, 0);
   }
-  for (int r = threadIdx.x; r < rows; r += kFwdThreads)
+  for (int r = threadIdx.x; r < rows; r += blockDim.x)
     p.lse[(int64_t)head * p.tokens + row0 + r] = -INFINITY;
 }
 
-template <int HD, int FMT>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+template <int HD, int FMT, int TILES>
+__global__ void __launch_bounds__(fwd_threads(TILES), 3 - TILES)
 attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const FwdParams p) {
@@ -82,18 +90,22 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
   map_block(blockIdx.x, p.slots, p.units, p.head_group, slot, unit);
   const int4 item = plan_item(p.plan, slot);
   if (item.z < 0) return;  // unused slot
-  const int head[2] = {p.pair_heads ? 2 * unit : unit, p.pair_heads ? 2 * unit + 1 : unit};
+  constexpr bool kTwo = TILES == 2;
+  constexpr int KST = fwd_stages<HD, TILES>();
+  const bool pair_heads = kTwo && p.pair_heads;
+  const int head[2] = {pair_heads ? 2 * unit : unit, pair_heads ? 2 * unit + 1 : unit};
   const int seq0 = item.x, L = item.y;
   if (item.z == 0) {
     clear_rows(p, seq0, L, head[0]);
-    if (p.pair_heads) clear_rows(p, seq0, L, head[1]);
+    if (pair_heads) clear_rows(p, seq0, L, head[1]);
     return;
   }
   const int last_tile = (L - 1) / kTile;
   int qt[2], n_kv[2];
-  if (p.pair_heads) {
+  if (pair_heads || !kTwo) {
     qt[0] = qt[1] = item.z - 1;
-    n_kv[0] = n_kv[1] = item.z;
+    n_kv[0] = item.z;
+    n_kv[1] = kTwo ? item.z : 0;
   } else {
     // an item of odd weight whose successor exists is that item's tile A
     const int t = item.z - 1;
@@ -103,7 +115,7 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
     n_kv[0] = qt[0] + 1;
     n_kv[1] = (t & 1) ? qt[1] + 1 : 0;
   }
-  const bool b_active = n_kv[1] > 0;
+  const bool b_active = kTwo && n_kv[1] > 0;
   const int n_max = b_active ? n_kv[1] : n_kv[0];
   const int head_kv = head[0] / p.group;
   // halves of 64 keys; a last tile of at most 64 tokens has one
@@ -113,10 +125,10 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
 
   extern __shared__ uint8_t smem_raw[];
   constexpr uint32_t TB = tile_bytes<HD>();
-  BlockSetup bs = carve(smem_raw, 6 * TB);
-  uint8_t* sQ[2] = {bs.smem, bs.smem + TB};
-  uint8_t* sK[2] = {bs.smem + 2 * TB, bs.smem + 3 * TB};
-  uint8_t* sV[2] = {bs.smem + 4 * TB, bs.smem + 5 * TB};
+  BlockSetup bs = carve(smem_raw, fwd_smem_tiles<HD, TILES>() * TB);
+  uint8_t* sQ[2] = {bs.smem, bs.smem + (TILES - 1) * TB};
+  uint8_t* sK = bs.smem + TILES * TB;  // [KST]
+  uint8_t* sV = sK + KST * TB;         // [KST]
   uint64_t* q_full = bs.bars + 0;
   uint64_t* k_full = bs.bars + 1;   // [2]
   uint64_t* k_empty = bs.bars + 3;  // [2]
@@ -141,7 +153,7 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
     prefetch_tensormap(&map_q); prefetch_tensormap(&map_k); prefetch_tensormap(&map_v);
   }
   __syncthreads();
-  if (warp == 1) { tmem_alloc(bs.tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 1) { tmem_alloc(bs.tmem_slot, 256 * TILES); tmem_relinquish(); }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -157,23 +169,24 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
       if (b_active) load_tile<HD>(sQ[1], &map_q, seq0 + qt[1] * kTile, head[1], q_full);
       int j = 0;
       for (; j < n_max; ++j) {
-        const int st = j & 1;
-        if (j >= 2) mbar_wait(k_empty + st, ((j >> 1) - 1) & 1, ctx, 801);
+        const int st = j % KST;
+        const uint32_t reuse = (uint32_t)((j / KST - 1) & 1);
+        if (j >= KST) mbar_wait(k_empty + st, reuse, ctx, 801);
         if (*ctx.abort_flag) break;  // no new copies after a timeout
         mbar_expect_tx(k_full + st, TB);
-        load_tile<HD>(sK[st], &map_k, seq0 + j * kTile, head_kv, k_full + st);
-        if (j >= 2) mbar_wait(v_empty + st, ((j >> 1) - 1) & 1, ctx, 802);
+        load_tile<HD>(sK + st * TB, &map_k, seq0 + j * kTile, head_kv, k_full + st);
+        if (j >= KST) mbar_wait(v_empty + st, reuse, ctx, 802);
         if (!*ctx.abort_flag) {
           mbar_expect_tx(v_full + st, TB);
-          load_tile<HD>(sV[st], &map_v, seq0 + j * kTile, head_kv, v_full + st);
+          load_tile<HD>(sV + st * TB, &map_v, seq0 + j * kTile, head_kv, v_full + st);
         }
       }
       if (*ctx.abort_flag) {
         // let the copies still in flight land before the block returns
         mbar_drain(q_full, 0, p.wait_limit);
-        for (int g = j > 2 ? j - 2 : 0; g < j; ++g) {
-          mbar_drain(k_full + (g & 1), (uint32_t)((g >> 1) & 1), p.wait_limit);
-          mbar_drain(v_full + (g & 1), (uint32_t)((g >> 1) & 1), p.wait_limit);
+        for (int g = j > KST ? j - KST : 0; g < j; ++g) {
+          mbar_drain(k_full + g % KST, (uint32_t)((g / KST) & 1), p.wait_limit);
+          mbar_drain(v_full + g % KST, (uint32_t)((g / KST) & 1), p.wait_limit);
         }
       }
     }
@@ -195,7 +208,7 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
         if (lead)
-          mma_ts(tmem + 256 + w * 128, tmem + w * 128 + hf * 64 + ks * 8, desc_at(vb, kstep_mnmajor(ks)),
+          mma_ts(tmem + TILES * 128 + w * 128, tmem + w * 128 + hf * 64 + ks * 8, desc_at(vb, kstep_mnmajor(ks)),
                  idesc_o, (first && ks == 0) ? 0u : 1u);
       if (lead) mma_commit(pv_done + w);
     };
@@ -204,30 +217,35 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
     tc_fence_after_sync();
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      if (hf < n_half[0]) issue_s(0, hf, sQ[0], sK[0]);
-      if (hf < n_half[1]) issue_s(1, hf, sQ[1], sK[0]);
+      if (hf < n_half[0]) issue_s(0, hf, sQ[0], sK);
+      if (kTwo && hf < n_half[1]) issue_s(1, hf, sQ[1], sK);
     }
     if (lead) mma_commit(k_empty + 0);
     for (int j = 0; j < n_max; ++j) {
-      const int st = j & 1, st1 = st ^ 1;
+      const int st = j % KST, st1 = (j + 1) % KST;
       const uint32_t par = j & 1;
-      mbar_wait(v_full + st, (j >> 1) & 1, ctx, 805);
-      if (j == last_tile && tail_rows < kTile) clear_tile_rows<HD>(sV[st], tail_rows, lane);
-      if (j + 1 < n_max) mbar_wait(k_full + st1, ((j + 1) >> 1) & 1, ctx, 807);
+      uint8_t* v_tile = sV + st * TB;
+      const uint8_t* k_next = sK + st1 * TB;
+      mbar_wait(v_full + st, (uint32_t)((j / KST) & 1), ctx, 805);
+      if (j == last_tile && tail_rows < kTile) clear_tile_rows<HD>(v_tile, tail_rows, lane);
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int g = 2 * j + hf;
         if (g < n_half[0]) {
           mbar_wait(p_full + hf, par, ctx, 806);
           tc_fence_after_sync();
-          issue_pv(0, hf, sV[st], g == 0);
-          if (g + 2 < n_half[0]) issue_s(0, hf, sQ[0], sK[st1]);
+          issue_pv(0, hf, v_tile, g == 0);
         }
-        if (g < n_half[1]) {
+        if (hf == 0 && j + 1 < n_max) {
+          mbar_wait(k_full + st1, (uint32_t)(((j + 1) / KST) & 1), ctx, 807);
+          tc_fence_after_sync();
+        }
+        if (g + 2 < n_half[0]) issue_s(0, hf, sQ[0], k_next);
+        if (kTwo && g < n_half[1]) {
           mbar_wait(p_full + 2 + hf, par, ctx, 808);
           tc_fence_after_sync();
-          issue_pv(1, hf, sV[st], g == 0);
-          if (g + 2 < n_half[1]) issue_s(1, hf, sQ[1], sK[st1]);
+          issue_pv(1, hf, v_tile, g == 0);
+          if (g + 2 < n_half[1]) issue_s(1, hf, sQ[1], k_next);
         }
       }
       if (lead) mma_commit(v_empty + st);
@@ -237,14 +255,14 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
     if (lead) mma_commit(o_done);
   } else {
     // ---- softmax warps: one query row per thread
-    const int wg = (warp - 2) >> 2;  // 0: tile A, 1: tile B
+    const int wg = kTwo ? (warp - 2) >> 2 : 0;  // 0: tile A, 1: tile B
     const int quarter = warp & 3;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int row = quarter * 32 + lane;
     const int my_tile = wg ? qt[1] : qt[0], my_head = wg ? head[1] : head[0];
     const int q_pos = my_tile * kTile + row;  // position inside the sequence
     const int n_mine = wg ? n_half[1] : n_half[0];
-    const uint32_t tOw = tmem + 256 + wg * 128;
+    const uint32_t tOw = tmem + TILES * 128 + wg * 128;
     const float scale_log2 = p.scale_log2;
     float m_run = -INFINITY, l_run = 0.f;
     for (int g = 0; g < n_mine; ++g) {
@@ -331,35 +349,45 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
       mbar_wait(o_done, 0, ctx, 810);
       __syncwarp();
       tc_fence_after_sync();
+      // O through the group's Q tile in shared memory (no product reads it any more), so that
+      // whole rows leave: 16-byte pieces XORed with the row on the way in.
       const float inv_l = 1.0f / l_run;
-      const bool row_ok = q_pos < L;
-      const int64_t token = seq0 + (row_ok ? q_pos : 0);
-      uint8_t* orow_g = reinterpret_cast<uint8_t*>(p.o) + (token * p.o_st + (int64_t)my_head * p.o_sh) * 2;
+      constexpr int TPR = HD / 8;
+      uint4* tile = reinterpret_cast<uint4*>(wg ? sQ[1] : sQ[0]);
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t orow[32];
         tmem_ld32(tOw + lane_base + c * 32, orow);
         tmem_wait_ld();
-        if (row_ok) {
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            if (c * 32 + v * 8 < p.D) {
-              uint4 pk;
-              pk.x = pack2<FMT>(__uint_as_float(orow[8 * v + 0]) * inv_l, __uint_as_float(orow[8 * v + 1]) * inv_l);
-              pk.y = pack2<FMT>(__uint_as_float(orow[8 * v + 2]) * inv_l, __uint_as_float(orow[8 * v + 3]) * inv_l);
-              pk.z = pack2<FMT>(__uint_as_float(orow[8 * v + 4]) * inv_l, __uint_as_float(orow[8 * v + 5]) * inv_l);
-              pk.w = pack2<FMT>(__uint_as_float(orow[8 * v + 6]) * inv_l, __uint_as_float(orow[8 * v + 7]) * inv_l);
-              *reinterpret_cast<uint4*>(orow_g + (c * 32 + v * 8) * 2) = pk;
-            }
-          }
+        for (int v = 0; v < 4; ++v) {
+          uint4 pk;
+          pk.x = pack2<FMT>(__uint_as_float(orow[8 * v + 0]) * inv_l, __uint_as_float(orow[8 * v + 1]) * inv_l);
+          pk.y = pack2<FMT>(__uint_as_float(orow[8 * v + 2]) * inv_l, __uint_as_float(orow[8 * v + 3]) * inv_l);
+          pk.z = pack2<FMT>(__uint_as_float(orow[8 * v + 4]) * inv_l, __uint_as_float(orow[8 * v + 5]) * inv_l);
+          pk.w = pack2<FMT>(__uint_as_float(orow[8 * v + 6]) * inv_l, __uint_as_float(orow[8 * v + 7]) * inv_l);
+          tile[row * TPR + ((c * 4 + v) ^ (row & 7))] = pk;
         }
       }
+      const bool row_ok = q_pos < L;
+      const int64_t token = seq0 + (row_ok ? q_pos : 0);
       if (row_ok) p.lse[(int64_t)my_head * p.tokens + token] = (m_run + log2f(l_run)) * kLn2;
+      named_barrier_sync(1 + wg, 128);
+      uint8_t* out = reinterpret_cast<uint8_t*>(p.o) +
+                     ((int64_t)(seq0 + my_tile * kTile) * p.o_st + (int64_t)my_head * p.o_sh) * 2;
+      const int rows = min(kTile, L - my_tile * kTile);
+#pragma unroll
+      for (int i = (int)((threadIdx.x - 64) & 127); i < kTile * TPR; i += 128) {
+        const int orow = i / TPR, piece = i % TPR;
+        if (orow < rows && piece * 8 < p.D)
+          *reinterpret_cast<uint4*>(out + (int64_t)orow * p.o_st * 2 + piece * 16) =
+              tile[orow * TPR + (piece ^ (orow & 7))];
+      }
     }
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (warp == 1) tmem_dealloc(tmem, 256 * TILES);
 }
 
 int read_packed_fwd_status(int reset) {
@@ -376,7 +404,7 @@ int read_packed_fwd_status(int reset) {
 }
 const bool g_packed_fwd_registered = (register_device_status(read_packed_fwd_status), true);
 
-template <int HD, int FMT>
+template <int HD, int FMT, int TILES>
 int launch(const View& q, const View& k, const View& v, const FwdParams& p, int64_t Hq, int64_t Hkv,
            cudaStream_t stream) {
   CUtensorMap mq, mk, mv;
@@ -384,15 +412,21 @@ int launch(const View& q, const View& k, const View& v, const FwdParams& p, int6
       !encode_view_map(&mk, k, FMT, p.D, p.tokens, Hkv) ||
       !encode_view_map(&mv, v, FMT, p.D, p.tokens, Hkv))
     return fail(EVG_ELAUNCH, "packed_attention_fwd: cuTensorMapEncodeTiled failed");
-  const size_t smem = 6 * tile_bytes<HD>() + kControlBytes + 1024;
-  auto kern = attn_packed_fwd_kernel<HD, FMT>;
+  const size_t smem = fwd_smem_tiles<HD, TILES>() * tile_bytes<HD>() + kControlBytes + 1024;
+  auto kern = attn_packed_fwd_kernel<HD, FMT, TILES>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
       cudaSuccess) {
     cudaGetLastError();
     return fail(EVG_ELAUNCH, "packed_attention_fwd: cannot reserve %zu bytes of shared memory", smem);
   }
-  kern<<<(unsigned)((int64_t)p.slots * p.units), kFwdThreads, smem, stream>>>(mq, mk, mv, p);
+  kern<<<(unsigned)((int64_t)p.slots * p.units), fwd_threads(TILES), smem, stream>>>(mq, mk, mv, p);
   return check_launch("packed_attention_fwd");
+}
+template <int HD, int FMT>
+int launch_tiles(const View& q, const View& k, const View& v, const FwdParams& p, int tiles, int64_t Hq,
+                 int64_t Hkv, cudaStream_t stream) {
+  return tiles == 1 ? launch<HD, FMT, 1>(q, k, v, p, Hq, Hkv, stream)
+                    : launch<HD, FMT, 2>(q, k, v, p, Hq, Hkv, stream);
 }
 
 }  // namespace
@@ -413,14 +447,26 @@ int launch_fwd(const View& q, const View& k, const View& v, const View& o, float
   p.group = (int)(Hq / Hkv);
   p.D = (int)D;
   p.pair_heads = p.group % 2 == 0;
-  p.units = (int)(p.pair_heads ? Hq / 2 : Hq);
+  // Two query tiles per block share their key tiles; with one, two blocks run on an SM and
+  // nothing is idle that has no second tile. Measured, one | two, 16384 tokens:
+  //   head size 64: one at every length (16/16 heads: 128 tokens a sequence 64 | 98 us, 1024
+  //   88 | 102, 16384 729 | 822; 8/2 heads: 128 26 | 26, 1024 41 | 47, 16384 365 | 414)
+  //   128, even group (32/8): 1 token 981 | 1208, 64 97 | 102, 512 156 | 154,
+  //   2048 307 | 300, 16384 1912 | 1720
+  //   128, odd group (9/3), where the second tile is the sequence's next: 64 28 | 46,
+  //   512 50 | 58, 2048 107 | 109, 4096 190 | 187, 16384 706 | 651
+  const int64_t two_from = p.pair_heads ? 256 : 4096;  // tokens per sequence
+  const int tiles = D <= 64 || tokens < two_from * sequences ? 1 : 2;
+  p.units = (int)(tiles == 2 && p.pair_heads ? Hq / 2 : Hq);
   p.head_group = head_group_for((int64_t)p.slots * p.units, p.units);
   p.scale_log2 = scale * kLog2e;
   const int t = tune("attention.wait_limit");
   p.wait_limit = t > 0 ? (long long)t * 1000000ll : 2000000000ll;
   if (D > 64)
-    return fmt == 1 ? launch<128, 1>(q, k, v, p, Hq, Hkv, stream) : launch<128, 0>(q, k, v, p, Hq, Hkv, stream);
-  return fmt == 1 ? launch<64, 1>(q, k, v, p, Hq, Hkv, stream) : launch<64, 0>(q, k, v, p, Hq, Hkv, stream);
+    return fmt == 1 ? launch_tiles<128, 1>(q, k, v, p, tiles, Hq, Hkv, stream)
+                    : launch_tiles<128, 0>(q, k, v, p, tiles, Hq, Hkv, stream);
+  return fmt == 1 ? launch_tiles<64, 1>(q, k, v, p, tiles, Hq, Hkv, stream)
+                  : launch_tiles<64, 0>(q, k, v, p, tiles, Hq, Hkv, stream);
 }
 
 }  // namespace packed
