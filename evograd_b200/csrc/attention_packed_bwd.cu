@@ -16,10 +16,7 @@
 // memory until the end (fixed order, no atomics). dQ^T also belongs to other blocks'
 // rows: four warps of their own send it to a float32 copy of dQ by asynchronous bulk
 // reductions, so dq can differ in the last bit from run to run; a last kernel scales and
-// rounds the copy. A sequence of one tile has no float32 copy, its dQ is rounded and written
-// at once (128 sequences of 128 tokens, 32/8 heads of 128: 367 -> 283 us; doing the same
-// for the first tile of longer sequences, whose other blocks wait meanwhile, was 5 % slower
-// on 16 sequences of 1 to 900 tokens).
+// rounds the copy. The first query tile of a short sequence skips the copy (whole_dq).
 //
 // K and V are kept in tensor memory as well (64 columns each): a product of two
 // shared-memory operands with 64 columns needs 192 bytes a clock of the shared memory's
@@ -33,8 +30,8 @@
 //
 // Tensor memory: streams [0,64) and [64,128), K [128,192), V [192,256), dV [256,256+HD),
 // dK [384,384+HD). Shared memory: K, two dO and two Q stages, two 16 KB dS^T halves, row
-// statistics, 32 KB of float32 dQ on its way out (226 KB at head size 128). At head size 64 the dQ^T product keeps its 128
-// rows: the A operand's second 64 columns are whatever follows K in shared memory, and
+// statistics, 32 KB of float32 dQ on its way out (226 KB at head size 128). At head size 64
+// the dQ^T product keeps its 128 rows: the A operand's second 64 columns are whatever follows K in shared memory, and
 // the rows they give are not read (a 64-row product has another layout in tensor memory).
 //
 // Tiles start at the sequence's first token; rows of K, V, Q and dO behind its end are
@@ -60,6 +57,13 @@ constexpr int kCG = 4;             // column groups of compute warps in the fina
 constexpr int kBwdThreads = 32 * (2 + kComputeWarps + 4);
 constexpr uint32_t kChunkBytes = 64 * 128 * 2;  // 64 queries x 128 keys of 16-bit dS^T
 constexpr uint32_t kStatBytes = 2048;
+
+// Sequences whose first query tile, to which one block alone contributes, gets its dQ rounded
+// and written by that block instead of a float32 copy. Spared traffic against longer turns of
+// the four warps that do it (32/8 heads of 128, 16384 tokens, without | with: 64 tokens a
+// sequence 224 | 190 us, 128 278 | 247, 256 384 | 337, 512 473 | 453, 1024 584 | 616,
+// 2048 886 | 893; 5096 tokens in sequences of 1 to 900, forward and backward, 235 | 227).
+__device__ __forceinline__ bool whole_dq(int L) { return L <= 4 * kTile; }
 
 template <int HD> __host__ __device__ constexpr uint32_t bwd_tile_region() {
   return 6 * tile_bytes<HD>() + 2 * kChunkBytes + kStatBytes;
@@ -376,18 +380,29 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
         tmem_ld(tY0 + 64 * b + lane_base + 32, acc[1]);
         tmem_wait_ld();
         warp_arrive(d_free + b, r.lane);
-        if (last_tile == 0) {
-          // A sequence of one tile gets its whole dQ here: rounded and written at once, 64
-          // contiguous bytes per warp and query.
-          if (r.row < p.D) {
-            uint8_t* dst = view_row(p.dq, seq0 + b * 64, head) + r.row * 2;
-            const int n = L - b * 64;
+        if (kvt == 0 && it == 0 && whole_dq(L)) {
+          // All of these rows' dQ: rounded, through the same pieces of shared memory, and
+          // written as whole rows.
+          constexpr int TPR = HD / 8;
 #pragma unroll
-            for (int j = 0; j < 64; ++j) {
-              if (j < n)
-                *reinterpret_cast<uint16_t*>(dst) =
-                    (uint16_t)pack2<FMT>(__uint_as_float(acc[j >> 5][j & 31]) * p.scale, 0.f);
-              dst += p.dq.st * 2;
+          for (int h = 0; h < 2; ++h) {
+            if (issuer) bulk_wait_read<0>();  // earlier reductions have read both pieces
+            named_barrier_sync(1, 128);
+            uint8_t* piece = sDQ + h * kPiece;
+            if (r.row < HD) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                reinterpret_cast<uint16_t*>(piece)[j * HD + r.row] =
+                    (uint16_t)pack2<FMT>(__uint_as_float(acc[h][j]) * p.scale, 0.f);
+            }
+            named_barrier_sync(1, 128);
+            const int first = b * 64 + h * 32;
+#pragma unroll
+            for (int k = 0; k < 32 * TPR / 128; ++k) {
+              const int i = r.row + 128 * k, row = i / TPR, col = i % TPR;
+              if (first + row < L && col * 8 < p.D)
+                reinterpret_cast<uint4*>(view_row(p.dq, seq0 + first + row, head))[col] =
+                    reinterpret_cast<const uint4*>(piece)[i];
             }
           }
         } else {
@@ -560,8 +575,8 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
 }
 
 // Row statistics of every item's query tile: delta = do . o and the log-sum-exp in log2
-// units, padded rows +inf / 0, and the tile's rows of the float32 dQ copy cleared (a
-// sequence of one tile has none).
+// units, padded rows +inf / 0, and the tile's rows of the float32 dQ copy cleared
+// (where the copy is used).
 // In sequences of a few tokens dS = P (dP - delta) is often a small difference, to which
 // the rounding of o to 16 bits would contribute up to percents (two tokens: 4 %); there
 // delta is summed from its definition, sum_j P_ij do_i . v_j.
@@ -611,7 +626,7 @@ packed_prepare_kernel(const View dout, const View q, const View o, const float* 
     } else {
       s = row_sum(mine ? dot8<FMT>(g, ld_vec(view_row(o, token, head) + part * 16)) : 0.f);
     }
-    if (item.y > kTile) {
+    if (item.z > 1 || !whole_dq(item.y)) {
       uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (prow0 + r) * HD + part * 8);
       acc[0] = acc[1] = make_uint4(0, 0, 0, 0);
     }
@@ -630,7 +645,7 @@ packed_finish_kernel(const BwdParams p) {
   constexpr int TPR = HD / 8;
   constexpr int QUADS = 256 / TPR;  // groups of 4 queries per round
   const int4 item = plan_item(p.plan, blockIdx.x);
-  if (item.z < 0 || (item.z > 0 && item.y <= kTile)) return;  // one tile: written by the products' kernel
+  if (item.z < 0 || (item.z == 1 && whole_dq(item.y))) return;  // written by the products' kernel
   const int head = blockIdx.y;
   const int part = threadIdx.x % TPR;
   if (part * 8 >= p.D) return;
