@@ -128,6 +128,7 @@ packed_generic_dq_kernel(const GenericParams p) {
   int i;
   if (!my_row(item, i)) return;
   const int64_t seq0 = item.x;
+  const float ds_scale = item.y > 1 ? p.scale : 0.f;  // a lone token's dS is zero
   T* out = row_ptr<T>(p.dq, seq0 + i, h);
   if (item.z == 0) {
     for (int d = lane; d < D; d += 32) out[d] = from_f32<T>(0.f);
@@ -172,7 +173,7 @@ packed_generic_dq_kernel(const GenericParams p) {
 #pragma unroll
   for (int t = 0; t < kMaxDT; ++t) {
     const int d = lane + 32 * t;
-    if (d < D) out[d] = from_f32<T>(acc[t] * p.scale);
+    if (d < D) out[d] = from_f32<T>(acc[t] * ds_scale);
   }
 }
 
@@ -206,6 +207,7 @@ packed_generic_dkdv_kernel(const GenericParams p) {
 #pragma unroll
   for (int t = 0; t < kMaxDT; ++t) ak[t] = av[t] = 0.f;
   const int L = item.y;
+  const float ds_scale = L > 1 ? p.scale : 0.f;  // a lone token's dS is zero
   for (int h = g * p.group; h < (g + 1) * p.group; ++h) {
     for (int i0 = j; i0 < L; i0 += 32) {
       const int i = i0 + lane;
@@ -235,7 +237,7 @@ packed_generic_dkdv_kernel(const GenericParams p) {
   for (int t = 0; t < kMaxDT; ++t) {
     const int d = lane + 32 * t;
     if (d < D) {
-      dk[d] = from_f32<T>(ak[t] * p.scale);
+      dk[d] = from_f32<T>(ak[t] * ds_scale);
       dv[d] = from_f32<T>(av[t]);
     }
   }

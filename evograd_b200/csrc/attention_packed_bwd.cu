@@ -10,29 +10,43 @@
 //   P^T, dS^T in registers, then 16 bits back into tensor memory over dP^T
 //   dV   += P^T dO,  dK += dS^T Q   (A from tensor memory)
 //   dQ^T  = K^T dS^T                [128 head columns x 64 queries], A the K tile in shared
-// A stream's S^T, dP^T, P^T / dS^T and dQ^T follow one another in the same 64 columns of
-// tensor memory. Each stream has eight compute warps of its own, so one stream's
-// exponentials and dS run under the other stream's products. dK and dV stay in tensor
-// memory until the end (fixed order, no atomics). dQ^T also belongs to other blocks'
-// rows: four warps of their own send it to a float32 copy of dQ by asynchronous bulk
-// reductions, so dq can differ in the last bit from run to run; a last kernel scales and
-// rounds the copy. The first query tile of a short sequence skips the copy (whole_dq).
+// Each stream has eight compute warps of its own, so one stream's exponentials and dS run
+// under the other stream's products. dK and dV stay in tensor memory until the end (fixed
+// order, no atomics). dQ^T also belongs to other blocks' rows: four warps of their own send
+// it to a float32 copy of dQ by asynchronous bulk reductions, so dq can differ in the last
+// bit from run to run; a last kernel scales and rounds the copy. Only one block contributes
+// to a sequence's first query tile: it rounds and writes those rows at once (32/8 heads of
+// 128, 16384 tokens: sequences of 128 tokens 367 -> 240 us, of 512 473 -> 437, of 1024
+// 584 -> 577).
 //
-// K and V are kept in tensor memory as well (64 columns each): a product of two
+// K and V are kept in tensor memory as well (HD / 2 columns each): a product of two
 // shared-memory operands with 64 columns needs 192 bytes a clock of the shared memory's
-// 128, and with both scores and dP^T formed that way the operand reads, not the tensor
-// pipe, set the time (416 KB per tile pair against 320 KB now).
+// 128 (50 cycles measured, 35 with A in tensor memory), and with both scores and dP^T formed
+// that way the operand reads, not the tensor pipe, set the time (416 KB per tile pair
+// against 320 KB now, head size 128).
 //
-// Order of the products for tile c (numbers in brackets: the stream):
+// Head size 128: a stream's S^T, dP^T, P^T / dS^T and dQ^T follow one another in the same 64
+// columns of tensor memory. Order of the products for tile c (in brackets the stream):
 //   S(c)[0]  dV,dK(c-1)[1]  dP(c)[0]  dQ(c-1)[1]  S(c)[1]  dV,dK(c)[0]  dP(c)[1]  dQ(c)[0]
 // The tensor pipe runs in order; the streams are half a tile apart, so what one of them
 // waits for runs behind the other's products.
+// Tensor memory: streams [0,64) and [64,128), K [128,192), V [192,256), dV [256,384),
+// dK [384,512). Shared memory: K, two dO and two Q stages, two 16 KB dS^T halves, row
+// statistics, 32 KB of dQ on its way out (226 KB). What the rest costs: without the bulk
+// reductions 16384 tokens in sequences of 4096 take 14 % less time, with a quarter of the
+// dV and dK products 8 % less, with an eighth of the dQ products 10 % less.
 //
-// Tensor memory: streams [0,64) and [64,128), K [128,192), V [192,256), dV [256,256+HD),
-// dK [384,384+HD). Shared memory: K, two dO and two Q stages, two 16 KB dS^T halves, row
-// statistics, 32 KB of float32 dQ on its way out (226 KB at head size 128). At head size 64
-// the dQ^T product keeps its 128 rows: the A operand's second 64 columns are whatever follows K in shared memory, and
-// the rows they give are not read (a 64-row product has another layout in tensor memory).
+// Head size 64 leaves room for more: scores, dP^T and the streams' common dQ^T have columns
+// of their own, three stages of Q and dO, and a stream's next S^T and dP^T are formed behind
+// its dV and dK of this tile; per half tile
+//   S(c+1)[b]  dV,dK(c)[b]  dP(c+1)[b]  dQ(c)[b]
+// (16/16 heads, 16384 tokens in sequences of 4096: 600 -> 546 us with one 16 KB piece of dQ
+// per half; what is left is spread over the dQ warps' turns, 12 %, and waits: no single part
+// taken out brings more than 4 %).
+// Tensor memory: S^T [0,128), dP^T [128,256), K [256,288), V [288,320), dV [320,384),
+// dK [384,448), dQ^T [448,512). The dQ^T product keeps its 128 rows: the A operand's second
+// 64 columns are whatever follows K in shared memory, and the rows they give are not read
+// (a 64-row product has another layout in tensor memory).
 //
 // Tiles start at the sequence's first token; rows of K, V, Q and dO behind its end are
 // other tokens and are zeroed in shared memory, and their statistics make P zero.
@@ -56,17 +70,12 @@ constexpr int kCG = 4;             // column groups of compute warps in the fina
 // TMA warp, MMA warp, compute warps, 4 warps that take dQ^T out of tensor memory
 constexpr int kBwdThreads = 32 * (2 + kComputeWarps + 4);
 constexpr uint32_t kChunkBytes = 64 * 128 * 2;  // 64 queries x 128 keys of 16-bit dS^T
-constexpr uint32_t kStatBytes = 2048;
-
-// Sequences whose first query tile, to which one block alone contributes, gets its dQ rounded
-// and written by that block instead of a float32 copy. Spared traffic against longer turns of
-// the four warps that do it (32/8 heads of 128, 16384 tokens, without | with: 64 tokens a
-// sequence 224 | 190 us, 128 278 | 247, 256 384 | 337, 512 473 | 453, 1024 584 | 616,
-// 2048 886 | 893; 5096 tokens in sequences of 1 to 900, forward and backward, 235 | 227).
-__device__ __forceinline__ bool whole_dq(int L) { return L <= 4 * kTile; }
+constexpr uint32_t kDqBytes = 32768;          // float32 dQ on its way out
+// Stages of Q and dO, with their rows' statistics.
+template <int HD> __host__ __device__ constexpr int bwd_stages() { return HD == 64 ? 3 : 2; }
 
 template <int HD> __host__ __device__ constexpr uint32_t bwd_tile_region() {
-  return 6 * tile_bytes<HD>() + 2 * kChunkBytes + kStatBytes;
+  return (1 + 2 * bwd_stages<HD>()) * tile_bytes<HD>() + kDqBytes + 2 * kChunkBytes + 1024 * bwd_stages<HD>() + 128;
 }
 
 struct BwdParams {
@@ -168,39 +177,46 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   constexpr uint32_t TB = tile_bytes<HD>();
   constexpr uint32_t kRegion = bwd_tile_region<HD>();
+  constexpr int NST = bwd_stages<HD>();
+  constexpr bool kSplit = HD == 64;
   BlockSetup bs = carve(smem_raw, kRegion);
   if ((uint32_t)(bs.smem - smem_raw) + kRegion + (uint32_t)kControlBytes > p.smem_bytes) {
     if (threadIdx.x == 0) atomicCAS(&g_attn_packed_bwd_status, 0, 899);
     return;
   }
   uint8_t* sK = bs.smem;
-  uint8_t* sDO0 = sK + TB;       // 2 stages
-  uint8_t* sQ0 = sDO0 + 2 * TB;  // 2 stages
-  uint8_t* sDS = sQ0 + 2 * TB;   // dS^T of the streams
-  uint8_t* sDQ = sDS + 2 * kChunkBytes;  // float32 dQ on its way out, two pieces of 32 queries
-  float* s_stat = reinterpret_cast<float*>(sDQ + TB);  // [stage][lse2 | delta][128]
+  uint8_t* sDO0 = sK + TB;         // [NST]
+  uint8_t* sQ0 = sDO0 + NST * TB;  // [NST]
+  uint8_t* sDS = sQ0 + NST * TB;   // dS^T of the streams
+  uint8_t* sDQ = sDS + 2 * kChunkBytes;  // float32 dQ on its way out
+  float* s_stat = reinterpret_cast<float*>(sDQ + kDqBytes);  // [NST][lse2 | delta][128]
   uint64_t* kv_full = bs.bars + 0;   // K and V in tensor memory
-  uint64_t* q_full = bs.bars + 1;    // [2] by stage
-  uint64_t* q_empty = bs.bars + 3;   // [2]
-  uint64_t* do_full = bs.bars + 5;   // [2]
-  uint64_t* do_empty = bs.bars + 7;  // [2]
-  uint64_t* s_full = bs.bars + 9;     // [2] by stream, as all below
-  uint64_t* x_free = bs.bars + 11;    // [2] the scores have been read
-  uint64_t* dp_full = bs.bars + 13;   // [2]
-  uint64_t* pds_full = bs.bars + 15;  // [2] P^T / dS^T are in tensor memory
-  uint64_t* ds_full = bs.bars + 17;   // [2] dS^T is in shared memory
-  uint64_t* dq_full = bs.bars + 19;   // [2]
-  uint64_t* d_free = bs.bars + 21;    // [2] dQ^T has been read
-  uint64_t* done = bs.bars + 23;      // K and V in shared memory; then: all products finished
+  uint64_t* done = bs.bars + 1;      // K and V in shared memory; then: all products finished
+  uint64_t* s_full = bs.bars + 2;    // [2] by stream, as those below
+  uint64_t* x_free = bs.bars + 4;    // [2] the scores have been read
+  uint64_t* dp_full = bs.bars + 6;   // [2]
+  uint64_t* pds_full = bs.bars + 8;  // [2] P^T / dS^T are in tensor memory
+  uint64_t* ds_full = bs.bars + 10;  // [2] dS^T is in shared memory
+  uint64_t* dq_full = bs.bars + 12;  // [2]
+  uint64_t* d_free = bs.bars + 14;   // [2] dQ^T has been read
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(s_stat + NST * 256);  // [NST] by stage, as those below
+  uint64_t* q_empty = q_full + NST;
+  uint64_t* do_full = q_empty + NST;
+  uint64_t* do_empty = do_full + NST;
   const Roles r = roles();
   const float scale_log2 = p.scale * kLog2e;
+  // A lone token's probability is one whatever its score: its dS is zero, and only rounding
+  // noise of dP - delta stands in the accumulators.
+  const float ds_scale = L > 1 ? p.scale : 0.f;
 
   if (threadIdx.x == 0) {
     *bs.abort_flag = 0;
     mbar_init(kv_full, kComputeWarps); mbar_init(done, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NST; ++i) {
       mbar_init(q_full + i, 1); mbar_init(q_empty + i, 1);
       mbar_init(do_full + i, 1); mbar_init(do_empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1); mbar_init(x_free + i, kStreamWarps);
       mbar_init(dp_full + i, 1); mbar_init(pds_full + i, kStreamWarps);
       mbar_init(ds_full + i, kStreamWarps); mbar_init(dq_full + i, 1); mbar_init(d_free + i, 4);
@@ -219,9 +235,12 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   constexpr uint32_t idesc_p = instr_desc_f16(FMT, 128, 64, 0, 0);
   constexpr uint32_t idesc_d = instr_desc_f16(FMT, 128, HD, 0, 1);
   constexpr uint32_t idesc_q = instr_desc_f16(FMT, 128, 64, 1, 1);
-  const uint32_t tY0 = tmem;  // stream b: tY0 + 64 b
-  const uint32_t tK = tmem + 128, tV = tmem + 192;
-  const uint32_t tDV = tmem + 256, tDK = tmem + 384;
+  // stream b: scores at tS0 + 64 b, all that follows them at tY0 + 64 b
+  const uint32_t tS0 = tmem, tY0 = kSplit ? tmem + 128 : tmem;
+  const uint32_t tK = kSplit ? tmem + 256 : tmem + 128, tV = tK + HD / 2;
+  const uint32_t tDV = tV + HD / 2, tDK = tDV + HD;
+  const uint32_t tDQ0 = kSplit ? tDK + HD : tY0;  // + kDQ b
+  constexpr uint32_t kDQ = kSplit ? 0 : 64;
 
   if (r.is_tma && r.lane == 0) {
     mbar_expect_tx(done, 2 * TB);
@@ -229,13 +248,14 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     load_tile<HD>(sDS, &map_v, seq0 + kv0, bh, done);  // V only passes through
     int it = 0, head = bh * p.group, git = 0;
     for (; git < n_git; ++git) {
-      const int st = git & 1;
+      const int st = git % NST;
+      const uint32_t reuse = (uint32_t)((git / NST - 1) & 1);
       const int q0 = seq0 + (kvt + it) * kTile;
-      if (git >= 2) mbar_wait(q_empty + st, ((git >> 1) - 1) & 1, ctx, 821);
+      if (git >= NST) mbar_wait(q_empty + st, reuse, ctx, 821);
       if (*ctx.abort_flag) break;  // no new copies after a timeout
       mbar_expect_tx(q_full + st, TB);
       load_tile<HD>(sQ0 + st * TB, &map_q, q0, head, q_full + st);
-      if (git >= 2) mbar_wait(do_empty + st, ((git >> 1) - 1) & 1, ctx, 831);
+      if (git >= NST) mbar_wait(do_empty + st, reuse, ctx, 831);
       if (!*ctx.abort_flag) {
         const int64_t prow = head * P + prow0 + (int64_t)it * kTile;
         mbar_expect_tx(do_full + st, TB + 1024);
@@ -249,9 +269,9 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
       // Let the copies still in flight land before the block returns: each of
       // these waits gives up after the same cycle budget.
       mbar_drain(done, 0, p.wait_limit);
-      for (int g = git > 2 ? git - 2 : 0; g < git; ++g) {
-        mbar_drain(q_full + (g & 1), (uint32_t)((g >> 1) & 1), p.wait_limit);
-        mbar_drain(do_full + (g & 1), (uint32_t)((g >> 1) & 1), p.wait_limit);
+      for (int g = git > NST ? git - NST : 0; g < git; ++g) {
+        mbar_drain(q_full + g % NST, (uint32_t)((g / NST) & 1), p.wait_limit);
+        mbar_drain(do_full + g % NST, (uint32_t)((g / NST) & 1), p.wait_limit);
       }
     }
   } else if (r.is_mma) {
@@ -259,12 +279,12 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     const DescBase kt_base = desc_base_mnmajor(smem_u32(sK), kTile);
     // [128 keys x 64 queries] of stream b into its columns: A = K or V in tensor memory,
     // B = rows [64 b, 64 b + 64) of a Q or dO tile.
-    auto issue_rows = [&](int b, uint32_t a_tmem, uint32_t tile_saddr, uint64_t* bar) {
+    auto issue_rows = [&](int b, uint32_t dst, uint32_t a_tmem, uint32_t tile_saddr, uint64_t* bar) {
       const DescBase rows = desc_base_kmajor(tile_saddr + b * 64 * 128);
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
         if (lead)
-          mma_ts(tY0 + 64 * b, a_tmem + 8 * ks, desc_at(rows, kstep_kmajor(kTile, ks)), idesc_p,
+          mma_ts(dst + 64 * b, a_tmem + 8 * ks, desc_at(rows, kstep_kmajor(kTile, ks)), idesc_p,
                  ks > 0 ? 1u : 0u);
       if (lead) mma_commit(bar + b);
     };
@@ -292,7 +312,7 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
 #pragma unroll
       for (int ks = 0; ks < kTile / 16; ++ks)
         if (lead)
-          mma_ss(tY0 + 64 * b, desc_at(kt_base, kstep_mnmajor(ks)), desc_at(dsb, kstep_mnmajor(ks)),
+          mma_ss(tDQ0 + kDQ * b, desc_at(kt_base, kstep_mnmajor(ks)), desc_at(dsb, kstep_mnmajor(ks)),
                  idesc_q, ks > 0 ? 1u : 0u);
       if (lead) mma_commit(dq_full + b);
     };
@@ -302,69 +322,127 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     };
     mbar_wait(kv_full, 0, ctx, 822);
     if (kvt == last_tile && tail_rows < kTile) clear_tile_rows<HD>(sK, tail_rows, r.lane);
-    int it = 0;  // query tile of iteration c
-    for (int c = 0; c <= n_git; ++c) {
-      const int st = c & 1;
-      const uint32_t par = (uint32_t)(c & 1), full = (uint32_t)((c >> 1) & 1);
-      const bool now = c < n_git, behind = c > 0;  // tile c; stream 1's second half of tile c - 1
-      uint8_t *q_tile = sQ0 + st * TB, *do_tile = sDO0 + st * TB;
-      const uint32_t q_saddr = smem_u32(q_tile), do_saddr = smem_u32(do_tile);
-      if (now) {
-        mbar_wait(q_full + st, full, ctx, 823);
-        clear_tail(q_tile, it);
-        if (behind) mbar_wait(d_free + 0, par ^ 1u, ctx, 835);
-        tc_fence_after_sync();
-        issue_rows(0, tK, q_saddr, s_full);
-      }
-      if (behind) {
-        mbar_wait(pds_full + 1, par ^ 1u, ctx, 829);
-        tc_fence_after_sync();
-        issue_dv(1, smem_u32(sDO0 + (st ^ 1) * TB), false);
-        if (lead) mma_commit(do_empty + (st ^ 1));
-        issue_dk(1, smem_u32(sQ0 + (st ^ 1) * TB), false);
-        if (lead) mma_commit(q_empty + (st ^ 1));
-      }
-      if (now) {
-        mbar_wait(do_full + st, full, ctx, 832);
-        clear_tail(do_tile, it);
-        mbar_wait(x_free + 0, par, ctx, 828);
-        tc_fence_after_sync();
-        issue_rows(0, tV, do_saddr, dp_full);
-      }
-      if (behind) {
-        mbar_wait(ds_full + 1, par ^ 1u, ctx, 834);
-        tc_fence_after_sync();
-        issue_dq(1);
-      }
-      if (now) {
-        if (behind) {
-          mbar_wait(d_free + 1, par ^ 1u, ctx, 826);
+    if constexpr (kSplit) {
+      // Stage and parity of tile c's operands.
+      auto stage = [&](int c) { return c % NST; };
+      auto turn = [&](int c) { return (uint32_t)((c / NST) & 1); };
+      auto q_at = [&](int c) { return sQ0 + stage(c) * TB; };
+      auto do_at = [&](int c) { return sDO0 + stage(c) * TB; };
+      mbar_wait(q_full, 0, ctx, 823);
+      clear_tail(sQ0, 0);
+      tc_fence_after_sync();
+      issue_rows(0, tS0, tK, smem_u32(sQ0), s_full);
+      issue_rows(1, tS0, tK, smem_u32(sQ0), s_full);
+      mbar_wait(do_full, 0, ctx, 832);
+      clear_tail(sDO0, 0);
+      tc_fence_after_sync();
+      issue_rows(0, tY0, tV, smem_u32(sDO0), dp_full);
+      issue_rows(1, tY0, tV, smem_u32(sDO0), dp_full);
+      int it = 0;
+      for (int c = 0; c < n_git; ++c) {
+        const uint32_t par = (uint32_t)(c & 1);
+        const bool more = c + 1 < n_git;
+        const int it_next = it + 1 == n_it ? 0 : it + 1;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          if (more) {
+            if (b == 0) {
+              mbar_wait(q_full + stage(c + 1), turn(c + 1), ctx, 823);
+              clear_tail(q_at(c + 1), it_next);
+            }
+            mbar_wait(x_free + b, par, ctx, 828);
+            tc_fence_after_sync();
+            issue_rows(b, tS0, tK, smem_u32(q_at(c + 1)), s_full);
+          }
+          mbar_wait(pds_full + b, par, ctx, 824);
           tc_fence_after_sync();
+          issue_dv(b, smem_u32(do_at(c)), b == 0 && c == 0);
+          if (b && lead) mma_commit(do_empty + stage(c));
+          issue_dk(b, smem_u32(q_at(c)), b == 0 && c == 0);
+          if (b && lead) mma_commit(q_empty + stage(c));
+          if (more) {
+            if (b == 0) {
+              mbar_wait(do_full + stage(c + 1), turn(c + 1), ctx, 832);
+              clear_tail(do_at(c + 1), it_next);
+              tc_fence_after_sync();
+            }
+            issue_rows(b, tY0, tV, smem_u32(do_at(c + 1)), dp_full);
+          }
+          mbar_wait(ds_full + b, par, ctx, 825);
+          if (b) mbar_wait(d_free + 0, par, ctx, 835);
+          else if (c > 0) mbar_wait(d_free + 1, par ^ 1u, ctx, 826);
+          tc_fence_after_sync();
+          issue_dq(b);
         }
-        issue_rows(1, tK, q_saddr, s_full);
-        mbar_wait(pds_full + 0, par, ctx, 824);
-        tc_fence_after_sync();
-        issue_dv(0, do_saddr, c == 0);
-        issue_dk(0, q_saddr, c == 0);
-        mbar_wait(x_free + 1, par, ctx, 833);
-        tc_fence_after_sync();
-        issue_rows(1, tV, do_saddr, dp_full);
-        mbar_wait(ds_full + 0, par, ctx, 825);
-        tc_fence_after_sync();
-        issue_dq(0);
+        it = it_next;
+        __syncwarp();
       }
-      if (++it == n_it) it = 0;
-      __syncwarp();
+    } else {
+      int it = 0;  // query tile of iteration c
+      for (int c = 0; c <= n_git; ++c) {
+        const int st = c & 1;
+        const uint32_t par = (uint32_t)(c & 1), full = (uint32_t)((c >> 1) & 1);
+        const bool now = c < n_git, behind = c > 0;  // tile c; stream 1's second half of tile c - 1
+        uint8_t *q_tile = sQ0 + st * TB, *do_tile = sDO0 + st * TB;
+        const uint32_t q_saddr = smem_u32(q_tile), do_saddr = smem_u32(do_tile);
+        if (now) {
+          mbar_wait(q_full + st, full, ctx, 823);
+          clear_tail(q_tile, it);
+          if (behind) mbar_wait(d_free + 0, par ^ 1u, ctx, 835);
+          tc_fence_after_sync();
+          issue_rows(0, tS0, tK, q_saddr, s_full);
+        }
+        if (behind) {
+          mbar_wait(pds_full + 1, par ^ 1u, ctx, 829);
+          tc_fence_after_sync();
+          issue_dv(1, smem_u32(sDO0 + (st ^ 1) * TB), false);
+          if (lead) mma_commit(do_empty + (st ^ 1));
+          issue_dk(1, smem_u32(sQ0 + (st ^ 1) * TB), false);
+          if (lead) mma_commit(q_empty + (st ^ 1));
+        }
+        if (now) {
+          mbar_wait(do_full + st, full, ctx, 832);
+          clear_tail(do_tile, it);
+          mbar_wait(x_free + 0, par, ctx, 828);
+          tc_fence_after_sync();
+          issue_rows(0, tY0, tV, do_saddr, dp_full);
+        }
+        if (behind) {
+          mbar_wait(ds_full + 1, par ^ 1u, ctx, 834);
+          tc_fence_after_sync();
+          issue_dq(1);
+        }
+        if (now) {
+          if (behind) {
+            mbar_wait(d_free + 1, par ^ 1u, ctx, 826);
+            tc_fence_after_sync();
+          }
+          issue_rows(1, tS0, tK, q_saddr, s_full);
+          mbar_wait(pds_full + 0, par, ctx, 824);
+          tc_fence_after_sync();
+          issue_dv(0, do_saddr, c == 0);
+          issue_dk(0, q_saddr, c == 0);
+          mbar_wait(x_free + 1, par, ctx, 833);
+          tc_fence_after_sync();
+          issue_rows(1, tY0, tV, do_saddr, dp_full);
+          mbar_wait(ds_full + 0, par, ctx, 825);
+          tc_fence_after_sync();
+          issue_dq(0);
+        }
+        if (++it == n_it) it = 0;
+        __syncwarp();
+      }
     }
     if (lead) mma_commit(done);
   } else if (r.warp >= 2 + kComputeWarps) {
-    // dQ^T of every half tile to the float32 copy, 32 queries at a time: out of tensor
-    // memory (a thread has one head column), into shared memory in the copy's layout, and
-    // on by an asynchronous bulk reduction, 16 KB each, one being written while the other
-    // is read. (Reductions issued by these threads, 64 lines each, held up every access of
-    // the SM to shared memory and mbarriers for about 1100 cycles per half tile.)
+    // dQ^T of every half tile to the float32 copy: out of tensor memory (a thread has one
+    // head column), into shared memory in the copy's layout, and on by an asynchronous bulk
+    // reduction, 16 KB at a time, one piece being written while the other is read.
+    // (Reductions issued by these threads, 64 lines each, held up every access of the SM to
+    // shared memory and mbarriers for about 1100 cycles per half tile.)
     const uint32_t lane_base = (uint32_t)(r.quarter * 32) << 16;
-    constexpr uint32_t kPiece = 32 * HD * 4;
+    constexpr uint32_t kPiece = kDqBytes / 2;
+    constexpr int kRows = kPiece / (HD * 4);  // queries: half of a half tile, or all of it
     const bool issuer = r.warp == 2 + kComputeWarps && r.lane == 0;
     int it = 0, head = bh * p.group;
     for (int c = 0; c < n_git; ++c) {
@@ -376,49 +454,48 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
         __syncwarp();
         tc_fence_after_sync();
         uint32_t acc[2][32];
-        tmem_ld(tY0 + 64 * b + lane_base, acc[0]);
-        tmem_ld(tY0 + 64 * b + lane_base + 32, acc[1]);
+        tmem_ld(tDQ0 + kDQ * b + lane_base, acc[0]);
+        tmem_ld(tDQ0 + kDQ * b + lane_base + 32, acc[1]);
         tmem_wait_ld();
         warp_arrive(d_free + b, r.lane);
-        if (kvt == 0 && it == 0 && whole_dq(L)) {
-          // All of these rows' dQ: rounded, through the same pieces of shared memory, and
-          // written as whole rows.
+        if (kvt == 0 && it == 0) {
+          // A sequence's first query tile gets its whole dQ here: rounded, through the same
+          // shared memory, and written as whole rows.
           constexpr int TPR = HD / 8;
+          if (issuer) bulk_wait_read<0>();  // earlier reductions have read it
+          named_barrier_sync(1, 128);
+          if (r.row < HD) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (issuer) bulk_wait_read<0>();  // earlier reductions have read both pieces
-            named_barrier_sync(1, 128);
-            uint8_t* piece = sDQ + h * kPiece;
-            if (r.row < HD) {
+            for (int j = 0; j < 64; ++j)
+              reinterpret_cast<uint16_t*>(sDQ)[j * HD + r.row] =
+                  (uint16_t)pack2<FMT>(__uint_as_float(acc[j >> 5][j & 31]) * ds_scale, 0.f);
+          }
+          named_barrier_sync(1, 128);
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                reinterpret_cast<uint16_t*>(piece)[j * HD + r.row] =
-                    (uint16_t)pack2<FMT>(__uint_as_float(acc[h][j]) * p.scale, 0.f);
-            }
-            named_barrier_sync(1, 128);
-            const int first = b * 64 + h * 32;
-#pragma unroll
-            for (int k = 0; k < 32 * TPR / 128; ++k) {
-              const int i = r.row + 128 * k, row = i / TPR, col = i % TPR;
-              if (first + row < L && col * 8 < p.D)
-                reinterpret_cast<uint4*>(view_row(p.dq, seq0 + first + row, head))[col] =
-                    reinterpret_cast<const uint4*>(piece)[i];
-            }
+          for (int k = 0; k < 64 * TPR / 128; ++k) {
+            const int i = r.row + 128 * k, row = b * 64 + i / TPR, col = i % TPR;
+            if (row < L && col * 8 < p.D)
+              reinterpret_cast<uint4*>(view_row(p.dq, seq0 + row, head))[col] =
+                  reinterpret_cast<const uint4*>(sDQ)[i];
           }
         } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < 64 / kRows; ++h) {
+            uint8_t* piece = sDQ + (HD == 64 ? b : h) * kPiece;
             if (issuer) bulk_wait_read<1>();  // this piece's last reduction has read it
             named_barrier_sync(1, 128);
             if (r.row < HD) {
-              uint4* dst = reinterpret_cast<uint4*>(sDQ + h * kPiece) + r.row;
+              uint4* dst = reinterpret_cast<uint4*>(piece) + r.row;
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                dst[j * HD] = make_uint4(acc[h][4 * j], acc[h][4 * j + 1], acc[h][4 * j + 2], acc[h][4 * j + 3]);
+              for (int j = 0; j < kRows / 4; ++j) {
+                const int q = h * kRows + 4 * j;
+                dst[j * HD] = make_uint4(acc[q >> 5][q & 31], acc[q >> 5][(q & 31) + 1], acc[q >> 5][(q & 31) + 2],
+                                         acc[q >> 5][(q & 31) + 3]);
+              }
             }
             fence_proxy_async_smem();
             named_barrier_sync(1, 128);
-            if (issuer && !*ctx.abort_flag) bulk_add_f32(tile_dst + (b * 64 + h * 32) * HD, sDQ + h * kPiece, kPiece);
+            if (issuer && !*ctx.abort_flag) bulk_add_f32(tile_dst + (b * 64 + h * kRows) * HD, piece, kPiece);
           }
         }
       }
@@ -459,20 +536,20 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     }
     int it = 0;
     for (int c = 0; c < n_git; ++c) {
-      const int st = c & 1;
+      const int st = c % NST;
       const uint32_t par = (uint32_t)(c & 1);
       const float* stat = s_stat + st * 256 + b * 64 + col0;
       // P^T: t = lse2 - s c, p = 2^-t, two columns per packed instruction. On the first
       // query tile, queries before the key are masked. S^T is handed back as soon as its
       // columns are in registers.
       f32x2 p2[16];
-      mbar_wait(do_full + st, (uint32_t)((c >> 1) & 1), ctx, 842);
+      mbar_wait(do_full + st, (uint32_t)((c / NST) & 1), ctx, 842);
       mbar_wait(s_full + b, par, ctx, 843);
       __syncwarp();
       tc_fence_after_sync();
       {
         uint32_t sr[32];
-        tmem_ld(tY, sr);
+        tmem_ld(tS0 + 64 * b + lane_base + col0, sr);
         tmem_wait_ld();
         warp_arrive(x_free + b, r.lane);
         const float4* lse4 = reinterpret_cast<const float4*>(stat);
@@ -541,8 +618,10 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
       if (r.lane == 0) mbar_arrive(pds_full + b);
       // dS^T for the dQ^T product: row r.row (a key) of the half's [128 keys x 64 queries]
       // tile, four 16-byte pieces of its 128 bytes at their swizzled places. The buffer's
-      // last reader has finished: this dP^T was issued behind the last dQ^T.
+      // last reader, the last dQ^T, has to be finished (at head size 128 this dP^T waited
+      // for it).
       {
+        if (kSplit && c > 0) mbar_wait(dq_full + b, par ^ 1u, ctx, 846);
         uint8_t* row_ptr = sDS + b * kChunkBytes + r.row * 128;
         const int sw = r.row & 7, piece = col0 / 8;
 #pragma unroll
@@ -563,7 +642,7 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     __syncwarp();
     tc_fence_after_sync();
     accumulator_to_tile<HD, FMT>(tDV, sDO0, 1.0f, r);
-    accumulator_to_tile<HD, FMT>(tDK, sDO0 + TB, p.scale, r);
+    accumulator_to_tile<HD, FMT>(tDK, sDO0 + TB, ds_scale, r);
     named_barrier_sync(2, 32 * kComputeWarps);
     const int t = (r.warp - 2) * 32 + r.lane;
     tile_to_view<HD>(sDO0, p.dv, bh, seq0, kv0, L, p.D, t);
@@ -626,7 +705,7 @@ packed_prepare_kernel(const View dout, const View q, const View o, const float* 
     } else {
       s = row_sum(mine ? dot8<FMT>(g, ld_vec(view_row(o, token, head) + part * 16)) : 0.f);
     }
-    if (item.z > 1 || !whole_dq(item.y)) {
+    if (item.z > 1) {
       uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (prow0 + r) * HD + part * 8);
       acc[0] = acc[1] = make_uint4(0, 0, 0, 0);
     }
@@ -645,7 +724,7 @@ packed_finish_kernel(const BwdParams p) {
   constexpr int TPR = HD / 8;
   constexpr int QUADS = 256 / TPR;  // groups of 4 queries per round
   const int4 item = plan_item(p.plan, blockIdx.x);
-  if (item.z < 0 || (item.z == 1 && whole_dq(item.y))) return;  // written by the products' kernel
+  if (item.z < 0 || item.z == 1) return;  // first tiles: written by the products' kernel
   const int head = blockIdx.y;
   const int part = threadIdx.x % TPR;
   if (part * 8 >= p.D) return;

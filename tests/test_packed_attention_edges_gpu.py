@@ -119,6 +119,17 @@ def test_scale_and_single_tokens():
     assert rel(dv, want) <= 2.0 ** -8
 
 
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(4, 2, 128, "bf16"), (2, 2, 64, "fp16"), (2, 1, 16, "fp32")])
+def test_lone_tokens_have_no_score_gradient(hq, hkv, d, dtype):
+    """One key's probability is one whatever its score: dq and dk are zero, not noise."""
+    q, k, v, do, cu = make([1, 5, 1, 1], 2, hq, hkv, d, dtype)
+    _, _, dq, dk, dv = run(q, k, v, do, cu)
+    for row in (0, 6, 7):
+        assert not bool(dq[row].any()) and not bool(dk[row].any())
+        assert bool(dv[row].any())
+    assert bool(dq[1:6].any()) and bool(dk[1:6].any())
+
+
 def test_invalid_offsets_make_a_plan_without_sequences():
     from evograd_b200 import ops
 
