@@ -507,16 +507,198 @@ post_pre_bwd_kernel(const NormArgs a) {
   }
 }
 
-// ------------------------------------------------- any width, any alignment
-// One block per row, three passes over the row (the later ones from L2); the column sums
-// of the backward live in the block's own partial row.
-constexpr int kAnyThreads = 256;
-
+// ------------------------------------------- rows off the 16-byte boundaries
+// Element by element, but each element once: a row's elements stay in its threads' registers
+// as in the kernels above (columns lane, lane + W, ..., K of them), so a warp still reads
+// and writes contiguous memory. Elements and weights behind the row's end are zeros, which
+// add nothing to any sum.
 template <typename T>
 __device__ __forceinline__ float gate_at(const NormArgs& a, int gate, int64_t row, int64_t c) {
   const T* g = (const T*)a.gate;
   return gate == kNone ? 1.f : to_f32<T>(g[gate == kChannel ? c : gate == kToken ? row : row * a.C + c]);
 }
+// *p, or zero (a predicated load: as a branch per element, the loads of a row would wait for
+// one another).
+template <typename T> __device__ __forceinline__ float ld_if(const T* p, bool on) {
+  if constexpr (sizeof(T) == 2) {
+    unsigned short r;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b16 %0, 0;\n\t@p ld.global.b16 %0, [%1];\n\t}"
+                 : "=h"(r) : "l"(p), "r"((int)on));
+    return to_f32<T>(*reinterpret_cast<T*>(&r));
+  } else {
+    float r;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}"
+                 : "=f"(r) : "l"(p), "r"((int)on));
+    return r;
+  }
+}
+__host__ __device__ constexpr int ragged_threads(int W) { return W == 32 ? 256 : W; }
+
+template <typename T, int K, int W>
+__global__ void __launch_bounds__(ragged_threads(W), K <= 12 ? 1024 / ragged_threads(W) : 1)
+post_pre_fwd_ragged_kernel(const NormArgs a, int gate) {
+  constexpr int MODE = W == 32 ? kWarp : kDirect;
+  __shared__ __align__(16) float scratch[2 * 32];
+  int phase = 0;
+  const int lane = threadIdx.x % W;
+  const int left = (int)a.C - lane;  // column lane + k W exists while k W < left
+  const int64_t stride = (int64_t)gridDim.x * (ragged_threads(W) / W);
+  int64_t row = (int64_t)blockIdx.x * (ragged_threads(W) / W) + threadIdx.x / W;
+  if (threadIdx.x < 64) scratch[threadIdx.x] = 0.f;
+  if constexpr (MODE == kDirect) __syncthreads();
+  float wp[K], wn[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    wp[k] = ld_if((const T*)a.w_post + lane + k * W, k * W < left);
+    wn[k] = ld_if((const T*)a.w_pre + lane + k * W, k * W < left);
+    if (gate == kChannel) wp[k] *= ld_if((const T*)a.gate + lane + k * W, k * W < left);
+  }
+  for (; row < a.rows; row += stride) {
+    const int64_t at = row * a.C + lane;
+    const T *x = (const T*)a.x + at, *res = (const T*)a.h + at;
+    float v[K], h[K], acc = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = ld_if(x + k * W, k * W < left);
+      h[k] = ld_if(res + k * W, k * W < left);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) acc = fmaf(v[k], v[k], acc);
+    const float r1 = rsqrtf(fmaf(row_sum<MODE>(acc, scratch, phase), a.inv_c, a.eps));
+    const float scale = r1 * a.alpha * (gate == kToken ? gate_at<T>(a, gate, row, 0) : 1.f);
+    if (gate == kFull) {
+      const T* g = (const T*)a.gate + at;
+#pragma unroll
+      for (int k = 0; k < K; ++k) v[k] *= ld_if(g + k * W, k * W < left);
+    }
+    acc = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      h[k] = fmaf(v[k] * wp[k], scale, h[k]);
+      acc = fmaf(h[k], h[k], acc);
+    }
+    T *ho = (T*)a.h_out + at, *y = (T*)a.y + at;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (k * W < left) ho[k * W] = from_f32<T>(h[k]);
+    const float r2 = rsqrtf(fmaf(row_sum<MODE>(acc, scratch, phase), a.inv_c, a.eps));
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (k * W < left) y[k * W] = from_f32<T>(h[k] * r2 * wn[k]);
+    if (lane == 0) {
+      a.rstd_post[row] = r1;
+      a.rstd_pre[row] = r2;
+    }
+  }
+}
+
+template <typename T, int K, int W>
+__global__ void __launch_bounds__(ragged_threads(W), K == 8 ? 512 / ragged_threads(W) : 1)
+post_pre_bwd_ragged_kernel(const NormArgs a, int gate) {
+  constexpr int MODE = W == 32 ? kWarp : kDirect;
+  extern __shared__ float fold[];  // kWarp: one partial row, [2][C]
+  __shared__ __align__(16) float scratch[2 * 64];
+  int phase = 0;
+  const int C = (int)a.C, lane = threadIdx.x % W;
+  const int left = C - lane;  // column lane + k W exists while k W < left
+  const int64_t stride = (int64_t)gridDim.x * (ragged_threads(W) / W);
+  int64_t row = (int64_t)blockIdx.x * (ragged_threads(W) / W) + threadIdx.x / W;
+  for (int i = threadIdx.x; i < 128; i += blockDim.x) scratch[i] = 0.f;
+  __syncthreads();
+  float wp[K], wn[K], spost[K], spre[K];  // wp: times a channel's gate
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    wp[k] = ld_if((const T*)a.w_post + lane + k * W, k * W < left);
+    wn[k] = ld_if((const T*)a.w_pre + lane + k * W, k * W < left);
+    if (gate == kChannel) wp[k] *= ld_if((const T*)a.gate + lane + k * W, k * W < left);
+    spost[k] = spre[k] = 0.f;
+  }
+  for (; row < a.rows; row += stride) {
+    const int64_t at = row * C + lane;
+    const T *x = (const T*)a.x + at, *hs = (const T*)a.h + at, *g = (const T*)a.gate + at;
+    const T *dy = (const T*)a.dy + at, *dh = (const T*)a.dh_in + at;
+    const float r1 = a.rstd_post[row], r2 = a.rstd_pre[row];
+    const float gt = gate == kToken ? gate_at<T>(a, gate, row, 0) : 1.f;
+    float t[K], h[K], d[K], v[K], s[3] = {0.f, 0.f, 0.f};  // t h'hat; (dh' + rstd2 t) w x; h'hat w x
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      t[k] = ld_if(dy + k * W, k * W < left);
+      h[k] = ld_if(hs + k * W, k * W < left);
+      d[k] = ld_if(dh + k * W, k * W < left);
+      v[k] = ld_if(x + k * W, k * W < left);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      h[k] *= r2;
+      spre[k] = fmaf(t[k], h[k], spre[k]);
+      t[k] *= wn[k];
+      float wx = wp[k] * v[k];
+      if (gate == kFull) wx *= ld_if(g + k * W, k * W < left);
+      s[0] = fmaf(t[k], h[k], s[0]);
+      s[1] = fmaf(fmaf(t[k], r2, d[k]), wx, s[1]);
+      s[2] = fmaf(h[k], wx, s[2]);
+    }
+    row_sum3<MODE>(s, scratch, phase);
+    const float k1 = -r2 * s[0] * a.inv_c;        // -rstd2 c1
+    const float sum = fmaf(k1, s[2], s[1]) * r1;  // sum U xhat
+    const float ku = r1 * a.alpha * gt, kx = -r1 * ku * sum * a.inv_c;
+    if (gate == kToken && lane == 0) ((T*)a.dgate)[row] = from_f32<T>(a.alpha * sum);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float G = fmaf(t[k], r2, fmaf(h[k], k1, d[k]));
+      float q = G * v[k], U = G * wp[k];
+      if (gate == kFull) {
+        const float gk = ld_if(g + k * W, k * W < left);
+        t[k] = q * wp[k] * ku;  // dgate
+        q *= gk;
+        U *= gk;
+      }
+      spost[k] = fmaf(q, ku, spost[k]);
+      d[k] = G;
+      v[k] = fmaf(U, ku, v[k] * kx);
+    }
+    T *dho = (T*)a.dh_out + at, *dx = (T*)a.dx + at, *dg = (T*)a.dgate + at;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (k * W < left) {
+        dho[k * W] = from_f32<T>(d[k]);
+        dx[k * W] = from_f32<T>(v[k]);
+        if (gate == kFull) dg[k * W] = from_f32<T>(t[k]);
+      }
+  }
+  float* pre = a.partial + (int64_t)blockIdx.x * C;
+  float* post = a.partial + ((int64_t)gridDim.x + blockIdx.x) * C;
+  if constexpr (MODE != kWarp) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (k * W < left) {
+        pre[lane + k * W] = spre[k];
+        post[lane + k * W] = spost[k];
+      }
+  } else {
+    for (int wi = 0; wi < ragged_threads(W) / 32; ++wi) {  // the warps' rows in warp order
+      if ((int)threadIdx.x / 32 == wi) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (k * W < left) {
+            const int c = lane + k * W;
+            fold[c] = wi ? fold[c] + spre[k] : spre[k];
+            fold[C + c] = wi ? fold[C + c] + spost[k] : spost[k];
+          }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < C; c += blockDim.x) {
+      pre[c] = fold[c];
+      post[c] = fold[C + c];
+    }
+  }
+}
+
+// ------------------------------------------------------------- any width
+// One block per row, three passes over the row (the later ones from L2); the column sums
+// of the backward live in the block's own partial row.
+constexpr int kAnyThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kAnyThreads)
@@ -652,20 +834,32 @@ int read_post_pre_status(int reset) {
 const bool g_post_pre_registered = (register_device_status(read_post_pre_status), true);
 
 struct Shape {
-  bool any;  // the kernels without vectors
-  int mode, V, threads, stages;
+  enum { kVectors, kRagged, kAny } kind;
+  int mode, V, threads, stages;  // V: vectors per thread, elements for kRagged
 };
-// One vector per thread up to `one_vector_most` vectors, two up to 1024, four above: the
-// forward (few registers) runs best with the most threads, the backward with half of them
-// and twice the work between its barriers ([16384, 4096] bf16: 87 against 96 us with two
-// vectors forward, 136 against 158 us with one vector backward); a warp per row up to 64 vectors; rows of more than 2048
-// vectors, or off a 16-byte boundary, take the kernels without vectors. `arrays`: rows
-// read per row.
-Shape pick_shape(int64_t C, size_t elem, bool aligned, int arrays, int one_vector_most) {
+// One vector per thread up to 512 (forward) or 256 vectors (backward), two up to 1024, four
+// above: the forward (few registers) runs best with the most threads, the backward with half
+// of them and twice the work between its barriers ([16384, 4096] bf16: 87 against 96 us with
+// two vectors forward, 136 against 158 us with one vector backward); a warp per row up to 64
+// vectors. Rows off a 16-byte boundary take the ragged kernels up to 8192 elements, a warp
+// per row up to 256, 8, 12 or 16 elements per thread (16384 rows of bf16 forward + backward,
+// against the kernels that read the row three times: 201 columns 138 -> 34 us, 1001
+// 284 -> 105, 4098 961 -> 526, 6001 1668 -> 648, 8001 2418 -> 1204; with one shape of 16
+// elements from 4097 on, 4098 took 894); all wider rows the kernels for any width.
+// `arrays`: rows read per row.
+Shape pick_shape(int64_t C, size_t elem, bool aligned, int arrays, bool backward) {
+  const int one_vector_most = backward ? 256 : 512;
   Shape s{};
-  s.threads = kAnyThreads;
   if (!aligned || (C * elem) % 16 != 0 || C * elem / 16 > 2048) {
-    s.any = true;
+    const int W = C <= 256 ? 32 : C <= 1024 ? 128 : C <= 2048 ? 256 : 512;
+    s.mode = W == 32 ? kWarp : kDirect;
+    s.V = C <= 8 * W ? 8 : C <= 12 * W ? 12 : 16;
+    s.threads = ragged_threads(W);
+    s.kind = Shape::kRagged;
+    if (C > 8192) {
+      s.kind = Shape::kAny;
+      s.threads = kAnyThreads;
+    }
     return s;
   }
   const int nvec = (int)(C * elem / 16);
@@ -716,7 +910,7 @@ template <typename Kernel>
 int blocks_for(Kernel kernel, const Shape& s, int64_t rows, size_t smem) {
   const int occ = occupancy((const void*)kernel, s.threads, smem);
   int64_t n = (int64_t)device_info().sm_count * occ;
-  const int64_t per = !s.any && s.mode == kWarp ? s.threads / 32 : 1;
+  const int64_t per = s.kind != Shape::kAny && s.mode == kWarp ? s.threads / 32 : 1;
   const int64_t need = (rows + per - 1) / per;
   if (n > need) n = need;
   if (n > most_blocks()) n = most_blocks();
@@ -765,7 +959,19 @@ int launch_bwd(const NormArgs& a, int gate, const Shape& s, cudaStream_t st, int
 
 template <typename T>
 int run_fwd(const NormArgs& a, int gate, const Shape& s, cudaStream_t st) {
-  if (s.any) {
+  if (s.kind == Shape::kRagged) {
+    auto run = [&](auto kernel) {
+      kernel<<<blocks_for(kernel, s, a.rows, 0), s.threads, 0, st>>>(a, gate);
+      return check_launch("post_pre_norm_fwd");
+    };
+    return s.mode == kWarp    ? run(post_pre_fwd_ragged_kernel<T, 8, 32>)
+           : s.threads == 128 ? run(post_pre_fwd_ragged_kernel<T, 8, 128>)
+           : s.threads == 256 ? run(post_pre_fwd_ragged_kernel<T, 8, 256>)
+           : s.V == 8         ? run(post_pre_fwd_ragged_kernel<T, 8, 512>)
+           : s.V == 12        ? run(post_pre_fwd_ragged_kernel<T, 12, 512>)
+                              : run(post_pre_fwd_ragged_kernel<T, 16, 512>);
+  }
+  if (s.kind == Shape::kAny) {
     post_pre_fwd_any_kernel<T><<<blocks_for(post_pre_fwd_any_kernel<T>, s, a.rows, 0), s.threads, 0, st>>>(a, gate);
     return check_launch("post_pre_norm_fwd");
   }
@@ -776,7 +982,21 @@ int run_fwd(const NormArgs& a, int gate, const Shape& s, cudaStream_t st) {
 
 template <typename T>
 int run_bwd_rows(const NormArgs& a, int gate, const Shape& s, cudaStream_t st, int& blocks) {
-  if (s.any) {
+  if (s.kind == Shape::kRagged) {
+    auto run = [&](auto kernel) {
+      const size_t smem = s.mode == kWarp ? 2 * a.C * sizeof(float) : 0;
+      blocks = blocks_for(kernel, s, a.rows, smem);
+      kernel<<<blocks, s.threads, smem, st>>>(a, gate);
+      return check_launch("post_pre_norm_bwd");
+    };
+    return s.mode == kWarp    ? run(post_pre_bwd_ragged_kernel<T, 8, 32>)
+           : s.threads == 128 ? run(post_pre_bwd_ragged_kernel<T, 8, 128>)
+           : s.threads == 256 ? run(post_pre_bwd_ragged_kernel<T, 8, 256>)
+           : s.V == 8         ? run(post_pre_bwd_ragged_kernel<T, 8, 512>)
+           : s.V == 12        ? run(post_pre_bwd_ragged_kernel<T, 12, 512>)
+                              : run(post_pre_bwd_ragged_kernel<T, 16, 512>);
+  }
+  if (s.kind == Shape::kAny) {
     blocks = blocks_for(post_pre_bwd_any_kernel<T>, s, a.rows, 0);
     post_pre_bwd_any_kernel<T><<<blocks, s.threads, 0, st>>>(a, gate);
     return check_launch("post_pre_norm_bwd");
@@ -819,7 +1039,7 @@ extern "C" int evg_post_pre_norm_fwd(const void* x, const void* h, const void* w
   bool aligned = true;
   for (const void* p : {x, h, w_post, w_pre, (const void*)h_out, (const void*)y}) aligned = aligned && aligned16(p);
   if (gate_kind == kChannel || gate_kind == kFull) aligned = aligned && aligned16(gate);
-  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned, gate_kind == kFull ? 3 : 2, 512);
+  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned, gate_kind == kFull ? 3 : 2, false);
   a.stages = s.stages;
   return EVG_DISPATCH_DTYPE(dtype, [&] { return run_fwd<T>(a, gate_kind, s, (cudaStream_t)stream); });
 }
@@ -857,7 +1077,7 @@ extern "C" int evg_post_pre_norm_bwd(const void* dy, const void* dh, const void*
   for (const void* p : {dy, dh, x, h_out, w_post, w_pre, (const void*)dx, (const void*)dres}) aligned = aligned && aligned16(p);
   if (gate_kind == kChannel) aligned = aligned && aligned16(gate);
   if (gate_kind == kFull) aligned = aligned && aligned16(gate) && aligned16(dgate);
-  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned, gate_kind == kFull ? 5 : 4, 256);
+  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned, gate_kind == kFull ? 5 : 4, true);
   a.stages = s.stages;
   cudaStream_t st = (cudaStream_t)stream;
   return EVG_DISPATCH_DTYPE(dtype, [&] {

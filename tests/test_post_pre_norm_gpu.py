@@ -62,6 +62,17 @@ def test_against_float64(rows, cols, gate, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("dtype,rows,cols", [
+    ("bf16", 5000, 1), ("fp32", 9, 255), ("bf16", 2500, 201), ("fp16", 300, 257), ("fp32", 1200, 1001),
+    ("bf16", 700, 1500), ("fp16", 400, 2047), ("bf16", 333, 2049), ("fp32", 150, 4095), ("bf16", 300, 4097),
+    ("fp32", 64, 6001), ("fp16", 170, 6145), ("bf16", 151, 8191), ("bf16", 3, 8193)])
+def test_rows_off_the_vector_boundary(dtype, rows, cols, gate):
+    """Each shape of the element-wise kernels, below and above its limits."""
+    check(make(rows, cols, gate, dtype), 0.5, dtype)
+
+
+@pytest.mark.gpu
 def test_bits_do_not_change_between_runs():
     t = make(3001, 2048, "channel", "bf16")
     a, b = check(t, 0.22, "bf16"), check(t, 0.22, "bf16")
