@@ -2,7 +2,8 @@
 // tensor-core kernels do not take (float32, head sizes that are no multiple of eight
 // or above 128, views that are not 16-byte aligned). One warp owns one row: a query
 // row in the forward and in dQ, a key row in dK/dV; every sum has a fixed order.
-// These are the small correctness shapes; nothing here is tuned for speed.
+// They are for small shapes: bound by the chain product -> softmax -> sum of 32 rows at a
+// time, about 4.6 us per 32 keys forward, far from any unit's rate.
 #include <cmath>
 
 #include "packed.cuh"
@@ -21,8 +22,7 @@ int64_t bwd_workspace_bytes(int64_t tokens, int64_t sequences, int64_t Hq, int64
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kMaxDT = 8;  // head size <= 256
+constexpr int kWarps = 8;
 
 struct GenericParams {
   const int* plan;
@@ -48,67 +48,120 @@ template <typename T>
 __device__ __forceinline__ T* row_ptr(const View& v, int64_t token, int head) {
   return reinterpret_cast<T*>(v.p) + token * v.st + (int64_t)head * v.sh;
 }
+// 32 rows of a head as float32 in shared memory, `ld` floats apart, by the whole block; rows
+// from `n` on and columns from D on are zeros.
 template <typename T>
-__device__ __forceinline__ float dot_row(const float* a_smem, const T* b_row, int D) {
-  float s = 0.f;
-  for (int d = 0; d < D; ++d) s = fmaf(a_smem[d], to_f32<T>(b_row[d]), s);
-  return s;
+__device__ __forceinline__ void stage_rows(float* dst, int ld, const View& v, int64_t token, int n, int head, int D) {
+  const int lane = threadIdx.x & 31, D4 = ld - 4;
+#pragma unroll
+  for (int k = 0; k < 32 / kWarps; ++k) {
+    const int r = (threadIdx.x >> 5) + k * kWarps;
+    const T* row = row_ptr<T>(v, token + (r < n ? r : 0), head);
+    for (int d = lane; d < D4; d += 32) dst[r * ld + d] = r < n && d < D ? to_f32<T>(row[d]) : 0.f;
+  }
 }
-// The row of (item, row block) this warp owns: false when there is none. i: position in
-// the sequence (or token behind the last one, seq0 = that token, for items of weight 0).
-__device__ __forceinline__ bool my_row(const int4& item, int& i) {
-  if (item.z < 0) return false;
-  i = (item.z > 0 ? (item.z - 1) * attn::kTile : 0) + blockIdx.z * kWarps + (threadIdx.x >> 5);
-  return i < item.y && (int)(blockIdx.z * kWarps + (threadIdx.x >> 5)) < attn::kTile;
+// One row of a head as float32, by a warp; zeros from D on, or everywhere.
+template <typename T>
+__device__ __forceinline__ void stage_row(float* dst, const View& v, int64_t token, int head, int D, int D4, bool on) {
+  for (int d = threadIdx.x & 31; d < D4; d += 32) dst[d] = on && d < D ? to_f32<T>(row_ptr<T>(v, token, head)[d]) : 0.f;
+}
+__device__ __forceinline__ float dot_rows(const float* a, const float* b, int D4) {
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int d = 0; d < D4; d += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(a + d), y = *reinterpret_cast<const float4*>(b + d);
+    s[0] = fmaf(x.x, y.x, s[0]);
+    s[1] = fmaf(x.y, y.y, s[1]);
+    s[2] = fmaf(x.z, y.z, s[2]);
+    s[3] = fmaf(x.w, y.w, s[3]);
+  }
+  return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-template <typename T>
+// What the kernels for any head size and type share: a warp owns a row of its item's tile
+// (a query's, or in the last kernel a key's) and meets the other side's rows 32 at a time,
+// one per lane for the products along the head, all of them for the sums along the rows.
+// The block's rows share the 32 through shared memory; what a row does not see is skipped,
+// not multiplied by zero. A sequence of 256 float32 tokens, 4/2 heads of 64: forward 37 us,
+// backward 152 (153 and 615 with each warp reading the rows for itself).
+struct Rows {
+  float *a, *b;   // [32][ld]: staged rows of two tensors
+  float *x, *y;   // the warp's own rows
+  int ld, D4;
+  int first, i;   // the block's first row inside the sequence, the warp's
+  bool clear, active;
+};
+__device__ __forceinline__ bool block_rows(Rows& r, const int4& item, float* smem, int D) {
+  const int warp = threadIdx.x >> 5;
+  if (item.z < 0) return false;  // unused slot
+  r.D4 = (D + 3) & ~3;
+  r.ld = r.D4 + 4;
+  r.a = smem;
+  r.b = r.a + 32 * r.ld;
+  r.x = r.b + 32 * r.ld + warp * r.D4;
+  r.y = r.x + kWarps * r.D4;
+  r.clear = item.z == 0;  // rows behind the last sequence
+  r.first = (r.clear ? 0 : (item.z - 1) * attn::kTile) + blockIdx.z * kWarps;
+  r.i = r.first + warp;
+  r.active = r.i < item.y;
+  return r.first < item.y;
+}
+size_t generic_smem(int64_t D, int rows_per_warp) {
+  const int64_t D4 = (D + 3) / 4 * 4;
+  return (size_t)(2 * 32 * (D4 + 4) + rows_per_warp * kWarps * D4) * sizeof(float);
+}
+
+template <typename T, int DT>
 __global__ void __launch_bounds__(kWarps * 32)
 packed_generic_fwd_kernel(const GenericParams p) {
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) float smem[];
   const int lane = threadIdx.x & 31, D = p.D, h = blockIdx.y, g = h / p.group;
-  float* qs = smem + (threadIdx.x >> 5) * D;
   const int4 item = plan_item(p.plan, blockIdx.x);
-  int i;
-  if (!my_row(item, i)) return;
+  Rows r;
+  if (!block_rows(r, item, smem, D)) return;
   const int64_t seq0 = item.x;
+  const int i = r.i;
   T* orow = row_ptr<T>(p.o, seq0 + i, h);
-  if (item.z == 0) {
+  if (r.clear) {
+    if (!r.active) return;
     for (int d = lane; d < D; d += 32) orow[d] = from_f32<T>(0.f);
     if (lane == 0) p.lse_out[(int64_t)h * p.tokens + seq0 + i] = -INFINITY;
     return;
   }
-  const T* qr = row_ptr<T>(p.q, seq0 + i, h);
-  for (int d = lane; d < D; d += 32) qs[d] = to_f32<T>(qr[d]);
-  __syncwarp();
+  stage_row<T>(r.x, p.q, seq0 + i, h, D, r.D4, r.active);
   float m = -INFINITY, l = 0.f;
-  float acc[kMaxDT];
+  float acc[DT];
 #pragma unroll
-  for (int t = 0; t < kMaxDT; ++t) acc[t] = 0.f;
-  for (int j0 = 0; j0 <= i; j0 += 32) {
+  for (int t = 0; t < DT; ++t) acc[t] = 0.f;
+  const int last = min(r.first + kWarps, item.y) - 1;
+  for (int j0 = 0; j0 <= last; j0 += 32) {
+    __syncthreads();
+    stage_rows<T>(r.a, r.ld, p.k, seq0 + j0, min(32, item.y - j0), g, D);
+    stage_rows<T>(r.b, r.ld, p.v, seq0 + j0, min(32, item.y - j0), g, D);
+    __syncthreads();
+    if (!r.active || j0 > i) continue;
     const int j = j0 + lane;
-    const float s = j <= i ? p.scale * dot_row<T>(qs, row_ptr<T>(p.k, seq0 + j, g), D) : -INFINITY;
+    const float s = j <= i ? p.scale * dot_rows(r.x, r.a + lane * r.ld, r.D4) : -INFINITY;
     const float m_new = fmaxf(m, warp_max(s));
     const float corr = m_new == m ? 1.f : expf(m - m_new);  // 0 on the first chunk
     const float pr = j <= i ? expf(s - m_new) : 0.f;
     l = l * corr + warp_sum(pr);
 #pragma unroll
-    for (int t = 0; t < kMaxDT; ++t) acc[t] *= corr;
+    for (int t = 0; t < DT; ++t) acc[t] *= corr;
     const int n = min(32, i - j0 + 1);
+#pragma unroll 8
     for (int jj = 0; jj < n; ++jj) {
       const float pj = __shfl_sync(0xffffffffu, pr, jj);
-      const T* vr = row_ptr<T>(p.v, seq0 + j0 + jj, g);
 #pragma unroll
-      for (int t = 0; t < kMaxDT; ++t) {
-        const int d = lane + 32 * t;
-        if (d < D) acc[t] = fmaf(pj, to_f32<T>(vr[d]), acc[t]);
-      }
+      for (int t = 0; t < DT; ++t)
+        if (lane + 32 * t < D) acc[t] = fmaf(pj, r.b[jj * r.ld + lane + 32 * t], acc[t]);
     }
     m = m_new;
   }
+  if (!r.active) return;
   const float inv = 1.0f / l;
 #pragma unroll
-  for (int t = 0; t < kMaxDT; ++t) {
+  for (int t = 0; t < DT; ++t) {
     const int d = lane + 32 * t;
     if (d < D) orow[d] = from_f32<T>(acc[t] * inv);
   }
@@ -117,61 +170,67 @@ packed_generic_fwd_kernel(const GenericParams p) {
 
 // delta_i = sum_{j<=i} p_ij do_i.v_j (from its definition: o is rounded), and dq of the row:
 // dq_i = scale * sum_{j<=i} p_ij (do_i.v_j - delta_i) k_j
-template <typename T>
+template <typename T, int DT>
 __global__ void __launch_bounds__(kWarps * 32)
 packed_generic_dq_kernel(const GenericParams p) {
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) float smem[];
   const int lane = threadIdx.x & 31, D = p.D, h = blockIdx.y, g = h / p.group;
-  float* qs = smem + (threadIdx.x >> 5) * 2 * D;
-  float* gs = qs + D;
   const int4 item = plan_item(p.plan, blockIdx.x);
-  int i;
-  if (!my_row(item, i)) return;
+  Rows r;
+  if (!block_rows(r, item, smem, D)) return;
   const int64_t seq0 = item.x;
+  const int i = r.i;
   const float ds_scale = item.y > 1 ? p.scale : 0.f;  // a lone token's dS is zero
   T* out = row_ptr<T>(p.dq, seq0 + i, h);
-  if (item.z == 0) {
-    for (int d = lane; d < D; d += 32) out[d] = from_f32<T>(0.f);
+  if (r.clear) {
+    if (r.active)
+      for (int d = lane; d < D; d += 32) out[d] = from_f32<T>(0.f);
     return;
   }
-  const T* qr = row_ptr<T>(p.q, seq0 + i, h);
-  const T* gr = row_ptr<T>(p.dout, seq0 + i, h);
-  for (int d = lane; d < D; d += 32) {
-    qs[d] = to_f32<T>(qr[d]);
-    gs[d] = to_f32<T>(gr[d]);
-  }
-  __syncwarp();
+  stage_row<T>(r.x, p.q, seq0 + i, h, D, r.D4, r.active);
+  stage_row<T>(r.y, p.dout, seq0 + i, h, D, r.D4, r.active);
   const int64_t stat = (int64_t)h * p.tokens + seq0 + i;
-  const float lse_i = p.lse[stat];
-  float sum = 0.f;
-  for (int j = lane; j <= i; j += 32)
-    sum += expf(p.scale * dot_row<T>(qs, row_ptr<T>(p.k, seq0 + j, g), D) - lse_i) *
-           dot_row<T>(gs, row_ptr<T>(p.v, seq0 + j, g), D);
-  const float delta_i = warp_sum(sum);
-  if (lane == 0) p.delta[stat] = delta_i;
-  float acc[kMaxDT];
+  const float lse_i = r.active ? p.lse[stat] : 0.f;
+  float delta_i = 0.f;
+  float acc[DT];
 #pragma unroll
-  for (int t = 0; t < kMaxDT; ++t) acc[t] = 0.f;
-  for (int j0 = 0; j0 <= i; j0 += 32) {
-    const int j = j0 + lane;
-    float ds = 0.f;
-    if (j <= i) {
-      const float pr = expf(p.scale * dot_row<T>(qs, row_ptr<T>(p.k, seq0 + j, g), D) - lse_i);
-      ds = pr * (dot_row<T>(gs, row_ptr<T>(p.v, seq0 + j, g), D) - delta_i);
-    }
-    const int n = min(32, i - j0 + 1);
-    for (int jj = 0; jj < n; ++jj) {
-      const float dj = __shfl_sync(0xffffffffu, ds, jj);
-      const T* kr = row_ptr<T>(p.k, seq0 + j0 + jj, g);
+  for (int t = 0; t < DT; ++t) acc[t] = 0.f;
+  const int last = min(r.first + kWarps, item.y) - 1;
+  for (int pass = 0; pass < 2; ++pass) {
+    float sum = 0.f;
+    for (int j0 = 0; j0 <= last; j0 += 32) {
+      if (pass == 0 || last >= 32) {  // (32 rows are still there)
+        __syncthreads();
+        stage_rows<T>(r.a, r.ld, p.k, seq0 + j0, min(32, item.y - j0), g, D);
+        stage_rows<T>(r.b, r.ld, p.v, seq0 + j0, min(32, item.y - j0), g, D);
+        __syncthreads();
+      }
+      if (!r.active || j0 > i) continue;
+      float pr = 0.f, dp = 0.f;
+      if (j0 + lane <= i) {
+        pr = expf(p.scale * dot_rows(r.x, r.a + lane * r.ld, r.D4) - lse_i);
+        dp = dot_rows(r.y, r.b + lane * r.ld, r.D4);
+      }
+      if (pass == 0) {
+        sum += pr * dp;
+        continue;
+      }
+      const float ds = j0 + lane <= i ? pr * (dp - delta_i) : 0.f;
+      const int n = min(32, i - j0 + 1);
+#pragma unroll 8
+      for (int jj = 0; jj < n; ++jj) {
+        const float dj = __shfl_sync(0xffffffffu, ds, jj);
 #pragma unroll
-      for (int t = 0; t < kMaxDT; ++t) {
-        const int d = lane + 32 * t;
-        if (d < D) acc[t] = fmaf(dj, to_f32<T>(kr[d]), acc[t]);
+        for (int t = 0; t < DT; ++t)
+          if (lane + 32 * t < D) acc[t] = fmaf(dj, r.a[jj * r.ld + lane + 32 * t], acc[t]);
       }
     }
+    if (pass == 0) delta_i = warp_sum(sum);
   }
+  if (!r.active) return;
+  if (lane == 0) p.delta[stat] = delta_i;
 #pragma unroll
-  for (int t = 0; t < kMaxDT; ++t) {
+  for (int t = 0; t < DT; ++t) {
     const int d = lane + 32 * t;
     if (d < D) out[d] = from_f32<T>(acc[t] * ds_scale);
   }
@@ -179,62 +238,59 @@ packed_generic_dq_kernel(const GenericParams p) {
 
 // One key row: dk_j = scale sum_i ds_ij q_i, dv_j = sum_i p_ij do_i over i >= j of the
 // sequence and the query heads of the group, in that order.
-template <typename T>
+template <typename T, int DT>
 __global__ void __launch_bounds__(kWarps * 32)
 packed_generic_dkdv_kernel(const GenericParams p) {
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) float smem[];
   const int lane = threadIdx.x & 31, D = p.D, g = blockIdx.y;
-  float* ks = smem + (threadIdx.x >> 5) * 2 * D;
-  float* vs = ks + D;
   const int4 item = plan_item(p.plan, blockIdx.x);
-  int j;
-  if (!my_row(item, j)) return;
+  Rows r;
+  if (!block_rows(r, item, smem, D)) return;
   const int64_t seq0 = item.x;
+  const int j = r.i, L = item.y;
   T* dk = row_ptr<T>(p.dk, seq0 + j, g);
   T* dv = row_ptr<T>(p.dv, seq0 + j, g);
-  if (item.z == 0) {
-    for (int d = lane; d < D; d += 32) dk[d] = dv[d] = from_f32<T>(0.f);
+  if (r.clear) {
+    if (r.active)
+      for (int d = lane; d < D; d += 32) dk[d] = dv[d] = from_f32<T>(0.f);
     return;
   }
-  const T* kr = row_ptr<T>(p.k, seq0 + j, g);
-  const T* vr = row_ptr<T>(p.v, seq0 + j, g);
-  for (int d = lane; d < D; d += 32) {
-    ks[d] = to_f32<T>(kr[d]);
-    vs[d] = to_f32<T>(vr[d]);
-  }
-  __syncwarp();
-  float ak[kMaxDT], av[kMaxDT];
+  stage_row<T>(r.x, p.k, seq0 + j, g, D, r.D4, r.active);
+  stage_row<T>(r.y, p.v, seq0 + j, g, D, r.D4, r.active);
+  float ak[DT], av[DT];
 #pragma unroll
-  for (int t = 0; t < kMaxDT; ++t) ak[t] = av[t] = 0.f;
-  const int L = item.y;
+  for (int t = 0; t < DT; ++t) ak[t] = av[t] = 0.f;
   const float ds_scale = L > 1 ? p.scale : 0.f;  // a lone token's dS is zero
   for (int h = g * p.group; h < (g + 1) * p.group; ++h) {
-    for (int i0 = j; i0 < L; i0 += 32) {
+    for (int i0 = r.first; i0 < L; i0 += 32) {
+      __syncthreads();
+      stage_rows<T>(r.a, r.ld, p.q, seq0 + i0, min(32, L - i0), h, D);
+      stage_rows<T>(r.b, r.ld, p.dout, seq0 + i0, min(32, L - i0), h, D);
+      __syncthreads();
+      if (!r.active) continue;
       const int i = i0 + lane;
       float pr = 0.f, ds = 0.f;
-      if (i < L) {
+      if (i >= j && i < L) {
         const int64_t stat = (int64_t)h * p.tokens + seq0 + i;
-        pr = expf(p.scale * dot_row<T>(ks, row_ptr<T>(p.q, seq0 + i, h), D) - p.lse[stat]);
-        ds = pr * (dot_row<T>(vs, row_ptr<T>(p.dout, seq0 + i, h), D) - p.delta[stat]);
+        pr = expf(p.scale * dot_rows(r.x, r.a + lane * r.ld, r.D4) - p.lse[stat]);
+        ds = pr * (dot_rows(r.y, r.b + lane * r.ld, r.D4) - p.delta[stat]);
       }
       const int n = min(32, L - i0);
-      for (int ii = 0; ii < n; ++ii) {
+#pragma unroll 8
+      for (int ii = max(j - i0, 0); ii < n; ++ii) {
         const float pi = __shfl_sync(0xffffffffu, pr, ii), di = __shfl_sync(0xffffffffu, ds, ii);
-        const T* qr = row_ptr<T>(p.q, seq0 + i0 + ii, h);
-        const T* gr = row_ptr<T>(p.dout, seq0 + i0 + ii, h);
 #pragma unroll
-        for (int t = 0; t < kMaxDT; ++t) {
-          const int d = lane + 32 * t;
-          if (d < D) {
-            ak[t] = fmaf(di, to_f32<T>(qr[d]), ak[t]);
-            av[t] = fmaf(pi, to_f32<T>(gr[d]), av[t]);
+        for (int t = 0; t < DT; ++t)
+          if (lane + 32 * t < D) {
+            ak[t] = fmaf(di, r.a[ii * r.ld + lane + 32 * t], ak[t]);
+            av[t] = fmaf(pi, r.b[ii * r.ld + lane + 32 * t], av[t]);
           }
-        }
       }
     }
   }
+  if (!r.active) return;
 #pragma unroll
-  for (int t = 0; t < kMaxDT; ++t) {
+  for (int t = 0; t < DT; ++t) {
     const int d = lane + 32 * t;
     if (d < D) {
       dk[d] = from_f32<T>(ak[t] * ds_scale);
@@ -285,10 +341,22 @@ int check_args(const char* what, const void* plan, int64_t tokens, int64_t seque
 
 template <typename Kernel>
 int launch_generic(const char* what, Kernel kernel, const GenericParams& p, int64_t slots,
-                   int64_t heads, int smem_rows, cudaStream_t stream) {
+                   int64_t heads, int rows_per_warp, cudaStream_t stream) {
   const dim3 grid((unsigned)slots, (unsigned)heads, (unsigned)(attn::kTile / kWarps));
-  kernel<<<grid, kWarps * 32, (size_t)smem_rows * kWarps * p.D * sizeof(float), stream>>>(p);
+  const size_t smem = generic_smem(p.D, rows_per_warp);
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)smem) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(EVG_ELAUNCH, "%s: cannot reserve %zu bytes of shared memory", what, smem);
+  }
+  kernel<<<grid, kWarps * 32, smem, stream>>>(p);
   return check_launch(what);
+}
+// Columns of 32 a head needs: `f` gets it as a constant, rounded up to 2, 4 or 8.
+template <typename F> int with_columns(int64_t D, F f) {
+  if (D <= 64) return f(std::integral_constant<int, 2>{});
+  if (D <= 128) return f(std::integral_constant<int, 4>{});
+  return f(std::integral_constant<int, 8>{});
 }
 
 }  // namespace
@@ -324,7 +392,9 @@ extern "C" int evg_packed_attention_fwd(const evg_packed_view* q, const evg_pack
   p.scale = scale;
   const int64_t slots = plan_slots(tokens, sequences);
   return EVG_DISPATCH_DTYPE(dtype, [&] {
-    return launch_generic(what, packed_generic_fwd_kernel<T>, p, slots, Hq, 1, st);
+    return with_columns(D, [&](auto dt) {
+      return launch_generic(what, packed_generic_fwd_kernel<T, decltype(dt)::value>, p, slots, Hq, 1, st);
+    });
   });
 }
 
@@ -378,7 +448,10 @@ extern "C" int evg_packed_attention_bwd(const evg_packed_view* dout, const evg_p
   p.scale = scale;
   const int64_t slots = plan_slots(tokens, sequences);
   return EVG_DISPATCH_DTYPE(dtype, [&] {
-    if (int rc = launch_generic(what, packed_generic_dq_kernel<T>, p, slots, Hq, 2, st)) return rc;
-    return launch_generic(what, packed_generic_dkdv_kernel<T>, p, slots, Hkv, 2, st);
+    return with_columns(D, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      if (int rc = launch_generic(what, packed_generic_dq_kernel<T, DT>, p, slots, Hq, 2, st)) return rc;
+      return launch_generic(what, packed_generic_dkdv_kernel<T, DT>, p, slots, Hkv, 2, st);
+    });
   });
 }
