@@ -7,7 +7,10 @@
 // owns one key tile of one k/v head and walks the query tiles behind it, for every
 // query head of the group. A tile's two halves of 64 queries are two streams:
 //   S^T   = K Q^T,  dP^T = V dO^T   [128 keys x 64 queries], A from tensor memory
-//   P^T, dS^T in registers, then 16 bits back into tensor memory over dP^T
+//   P^T, dS^T in registers, then 16 bits back into tensor memory over dP^T (the products'
+//   operand type: with delta from the rounded o it takes the relative error of bf16 dq and dk
+//   from 0.0017, their own last rounding, to 0.0025; a second operand with the remainder
+//   would double the dK and dQ products)
 //   dV   += P^T dO,  dK += dS^T Q   (A from tensor memory)
 //   dQ^T  = K^T dS^T                [128 head columns x 64 queries], A the K tile in shared
 // Each stream has eight compute warps of its own, so one stream's exponentials and dS run
