@@ -74,6 +74,24 @@ __device__ __forceinline__ float chunk_squares(const T* p, int n, bool vec) {
   }
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
+// A thread whose squares leave float32 (elements from 1.8e19 on) adds the same elements again
+// in float64.
+template <typename T>
+__device__ __forceinline__ double chunk_sum(const T* p, int n, bool vec) {
+  const float s = chunk_squares(p, n, vec);
+  if (s <= 3.402823466e38f) return (double)s;
+  double d = 0.0;
+  auto add = [&](int i) {
+    const double f = (double)to_f32<T>(p[i]);
+    d = fma(f, f, d);
+  };
+  constexpr int N = Vec<T>::N;
+  const int nv = vec ? n / N : 0;
+  for (int v = threadIdx.x; v < nv; v += kThreads)
+    for (int i = 0; i < N; ++i) add(v * N + i);
+  for (int i = nv * N + threadIdx.x; i < n; i += kThreads) add(i);
+  return d;
+}
 
 template <typename T>
 __device__ __forceinline__ void chunk_scale(const T* in, T* out, int n, bool vec, float c) {
@@ -123,9 +141,9 @@ grad_squares_kernel(const __grid_constant__ Table<CAP> t, double* __restrict__ p
     const int n = (int)(e.n - at < kChunk ? e.n - at : kChunk);
     const bool vec = e.dtype & 8;
     switch (e.dtype & 7) {
-      case EVG_F32: mine += (double)chunk_squares((const float*)e.in + at, n, vec); break;
-      case EVG_F16: mine += (double)chunk_squares((const __half*)e.in + at, n, vec); break;
-      default: mine += (double)chunk_squares((const __nv_bfloat16*)e.in + at, n, vec); break;
+      case EVG_F32: mine += chunk_sum((const float*)e.in + at, n, vec); break;
+      case EVG_F16: mine += chunk_sum((const __half*)e.in + at, n, vec); break;
+      default: mine += chunk_sum((const __nv_bfloat16*)e.in + at, n, vec); break;
     }
   }
   const double s = block_sum(mine, scratch);

@@ -66,6 +66,22 @@ def test_alignment_order_and_repeats():
 
 
 @pytest.mark.gpu
+def test_squares_beyond_float32():
+    """Elements whose squares overflow float32 leave the norm finite and the scaling exact to
+    the float32 rounding of the factor and one rounding of the result."""
+    from evograd_b200 import ops
+
+    g = [1e25 * torch.randn(40001, device="cuda"), (3e30 * torch.randn(5000, device="cuda")).bfloat16()[1:],
+         torch.randn(70, device="cuda")]
+    want, keep = norm64(g), [t.double().clone() for t in g]
+    norm = ops.clip_grad_norm(g, 2.0)
+    assert abs(float(norm) - want) <= 1e-6 * want
+    for t, k in zip(g[:2], keep):
+        u = torch.finfo(t.dtype).eps / 2
+        assert bool(((t.double() - k * (2.0 / want)).abs() <= (u + 1e-6) * k.abs() * (2.0 / want) + 1e-44).all())
+
+
+@pytest.mark.gpu
 def test_norms_that_are_not_finite():
     from evograd_b200 import ops
 
