@@ -144,7 +144,8 @@ packed_generic_fwd_kernel(const GenericParams p) {
     const float s = j <= i ? p.scale * dot_rows(r.x, r.a + lane * r.ld, r.D4) : -INFINITY;
     const float m_new = fmaxf(m, warp_max(s));
     const float corr = m_new == m ? 1.f : expf(m - m_new);  // 0 on the first chunk
-    const float pr = j <= i ? expf(s - m_new) : 0.f;
+    // (scores of -infinity are zero weights, also while a row has seen nothing else)
+    const float pr = j <= i ? expf(s - (m_new == -INFINITY ? 0.f : m_new)) : 0.f;
     l = l * corr + warp_sum(pr);
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[t] *= corr;

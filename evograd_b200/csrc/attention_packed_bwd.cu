@@ -85,7 +85,7 @@ struct BwdParams {
   const int* plan;
   float* lse2;    // [Hq][slots * 128] log-sum-exp in log2 units, +inf behind a sequence
   float* delta;   // [Hq][slots * 128]
-  float* dq_acc;  // [Hq][slots * 128][HD]
+  float* dq_acc;  // [Hq][tokens / 128 tiles][128 x HD], tiles as acc_tile numbers them
   View k, v, dq, dk, dv;
   int tokens, slots, units, head_group, group, D;
   float scale;
@@ -93,6 +93,12 @@ struct BwdParams {
   uint32_t smem_bytes;
 };
 
+// Place of query tile t >= 1 of a sequence in the float32 copy. The n - 1 tiles behind the
+// first of a sequence at rows [s, s + len) lie before row s + len when counted from s / 128, so
+// no two sequences share one and tokens / 128 are enough however many sequences there are.
+__device__ __forceinline__ int64_t acc_tile(const BwdParams& p, int head, int seq0, int t) {
+  return (int64_t)head * (p.tokens / kTile) + seq0 / kTile + t - 1;
+}
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -446,11 +452,15 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     const uint32_t lane_base = (uint32_t)(r.quarter * 32) << 16;
     constexpr uint32_t kPiece = kDqBytes / 2;
     constexpr int kRows = kPiece / (HD * 4);  // queries: half of a half tile, or all of it
+    // (row of the copy, as acc_tile numbers it: the address once per tile, 64-bit, and the loop
+    // below not unrolled, or the accumulator's 64 registers spill: 226 us against 216 for the
+    // step over 16 sequences of 1 to 900 tokens)
+    const int64_t head_rows = (int64_t)(p.tokens / kTile) * kTile, row0 = (int64_t)(seq0 / kTile + kvt - 1) * kTile;
     const bool issuer = r.warp == 2 + kComputeWarps && r.lane == 0;
     int it = 0, head = bh * p.group;
     for (int c = 0; c < n_git; ++c) {
       const uint32_t par = (uint32_t)(c & 1);
-      float* tile_dst = p.dq_acc + (head * P + prow0 + (int64_t)it * kTile) * HD;
+      float* tile_dst = p.dq_acc + (head * head_rows + row0 + (int64_t)it * kTile) * HD;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         mbar_wait(dq_full + b, par, ctx, 841);
@@ -474,7 +484,7 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
                   (uint16_t)pack2<FMT>(__uint_as_float(acc[j >> 5][j & 31]) * ds_scale, 0.f);
           }
           named_barrier_sync(1, 128);
-#pragma unroll
+#pragma unroll 1
           for (int k = 0; k < 64 * TPR / 128; ++k) {
             const int i = r.row + 128 * k, row = b * 64 + i / TPR, col = i % TPR;
             if (row < L && col * 8 < p.D)
@@ -709,7 +719,7 @@ packed_prepare_kernel(const View dout, const View q, const View o, const float* 
       s = row_sum(mine ? dot8<FMT>(g, ld_vec(view_row(o, token, head) + part * 16)) : 0.f);
     }
     if (item.z > 1) {
-      uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (prow0 + r) * HD + part * 8);
+      uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (acc_tile(p, head, item.x, item.z - 1) * kTile + r) * HD + part * 8);
       acc[0] = acc[1] = make_uint4(0, 0, 0, 0);
     }
     if (part == 0) {
@@ -733,11 +743,10 @@ packed_finish_kernel(const BwdParams p) {
   if (part * 8 >= p.D) return;
   const int tile0 = item.z > 0 ? (item.z - 1) * kTile : 0;
   const int rows = min(kTile, item.y - tile0);
-  const int64_t prow0 = (int64_t)head * p.slots * kTile + (int64_t)item.w * kTile + tile0;
   for (int qd = threadIdx.x / TPR + blockIdx.z * QUADS; qd * 4 < rows; qd += QUADS * gridDim.z) {
     float v[4][8];
     if (item.z > 0) {
-      const float4* src = reinterpret_cast<const float4*>(p.dq_acc + (prow0 + qd * 4) * HD) + part * 8;
+      const float4* src = reinterpret_cast<const float4*>(p.dq_acc + (acc_tile(p, head, item.x, item.z - 1) * kTile + qd * 4) * HD) + part * 8;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const float4 f = __ldcs(src + c);
@@ -808,7 +817,7 @@ namespace packed {
 
 int64_t bwd_workspace_bytes(int64_t tokens, int64_t sequences, int64_t Hq, int64_t D) {
   const int64_t rows = plan_slots(tokens, sequences) * kTile * Hq;
-  return rows * ((D > 64 ? 128 : 64) + 2) * 4;
+  return rows * 2 * 4 + tokens / kTile * kTile * Hq * (D > 64 ? 128 : 64) * 4;
 }
 
 int launch_bwd(const View& dout, const View& q, const View& k, const View& v, const View& o,

@@ -316,8 +316,8 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
       m_run = m_new;
       // Probabilities: 64 score columns -> 32 packed columns over them. P is rounded to 16
       // bits as the tensor cores' operand; its sum is taken before rounding. A masked score
-      // of -infinity gives zero.
-      const f32x2 neg_m2 = f2_splat(-m_run), scale2 = f2_splat(scale_log2);
+      // of -infinity gives zero, also while a row has seen nothing else (m_run is -infinity).
+      const f32x2 neg_m2 = f2_splat(m_run == -INFINITY ? 0.f : -m_run), scale2 = f2_splat(scale_log2);
       f32x2 ls2[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {

@@ -422,8 +422,9 @@ int64_t evg_packed_attention_bwd_workspace_bytes(int64_t tokens, int64_t sequenc
  * a group. Rows behind the last sequence get zero gradients. dk and dv are
  * bit-reproducible; on the tensor-core path dq is summed with float32 global
  * adds and can differ in the last bit from run to run. The workspace (16-byte
- * aligned) holds the row statistics and a float32 copy of dq, padded to whole
- * 128-row tiles per sequence.
+ * aligned) holds two floats per query head and row, rows padded to whole 128-row
+ * tiles per sequence, and a float32 copy of dq behind the sequences' first tiles
+ * (tokens / 128 tiles at most).
  */
 int evg_packed_attention_bwd(const evg_packed_view* dout, const evg_packed_view* q,
                              const evg_packed_view* k, const evg_packed_view* v,
@@ -495,8 +496,8 @@ int evg_post_pre_norm_bwd(const void* dy, const void* dh, const void* x,
  * clip != 0 every tensor is multiplied by min(1, max_norm / (norm + 1e-6)), in
  * place, or into `outs` when that is not NULL. grads, outs, numel, dtypes are HOST
  * arrays (of device pointers, element counts, evg_dtype), read before the call
- * returns. Squares and a thread's sums are float32, sums of blocks float64, in a
- * fixed order: bit-reproducible. A norm that is not finite scales as the formula
+ * returns. Squares and a thread's sums are float32 (float64 where those would
+ * overflow), sums of blocks float64, in a fixed order: bit-reproducible. A norm that is not finite scales as the formula
  * says (infinite: to zero, NaN: to NaN). No counterpart in the reference.
  */
 int64_t evg_clip_grads_workspace_bytes(int64_t count);

@@ -130,6 +130,43 @@ def test_lone_tokens_have_no_score_gradient(hq, hkv, d, dtype):
     assert bool(dq[1:6].any()) and bool(dk[1:6].any())
 
 
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(4, 2, 128, "bf16"), (3, 1, 128, "bf16"), (2, 2, 64, "fp16"), (2, 1, 16, "fp32")])
+def test_scores_of_minus_infinity_have_no_weight(hq, hkv, d, dtype):
+    """Keys 0 .. 127 score -inf with every query: behind them, rows see only the others, also
+    where a whole tile of keys comes before the first finite score."""
+    from evograd_b200 import ops
+
+    L, cut = 300, 128
+    q, k, v, _, cu = make([L], 0, hq, hkv, d, dtype)
+    q[:, :, 0] = q[:, :, 0].abs() + 0.5
+    k[:cut, :, 0] = float("-inf")
+    o, lse = ops.packed_attention_fwd(q, k, v, ops.packed_plan(cu, L))
+    assert torch.isnan(o[:cut]).all()
+    qd, kd, vd = q[cut:].double(), k[cut:].double(), v[cut:].double()
+    kd, vd = (t.repeat_interleave(hq // hkv, 1) for t in (kd, vd))
+    s = torch.einsum("ihd,jhd->hij", qd, kd) / d ** 0.5
+    s = s.masked_fill(~torch.ones(L - cut, L - cut, dtype=torch.bool, device="cuda").tril(), float("-inf"))
+    want = torch.einsum("hij,jhd->ihd", s.softmax(-1), vd)
+    u = torch.finfo(q.dtype).eps / 2
+    assert rel(o[cut:], want) <= 3 * u + 1e-5
+    assert float((lse[:, cut:].double() - s.logsumexp(-1)).abs().max()) <= 1e-4
+
+
+def test_many_short_sequences_among_long_ones():
+    """The float32 copy of dq has no room per sequence: lengths around multiples of the tile,
+    packed without gaps, must not share rows of it."""
+    lens = [129, 1, 256, 257, 127, 385, 2, 128, 130, 1, 1, 640, 126, 131]
+    q, k, v, do, cu = make(lens, 3, 4, 2, 64, "bf16")
+    got = run(q, k, v, do, cu)
+    start = 0
+    for n in lens:
+        one = torch.tensor([0, n], device="cuda", dtype=torch.int32)
+        sl = slice(start, start + n)
+        alone = run(q[sl].contiguous(), k[sl].contiguous(), v[sl].contiguous(), do[sl].contiguous(), one)
+        same([t[:, sl] if i == 1 else t[sl] for i, t in enumerate(got)], alone)
+        start += n
+
+
 def test_invalid_offsets_make_a_plan_without_sequences():
     from evograd_b200 import ops
 

@@ -128,3 +128,12 @@ def test_cpu_tensors_are_refused():
             call()
     with pytest.raises(TypeError):
         ops.packed_plan([0, 4], 4)
+
+
+def test_backward_workspace_follows_the_tokens(lib):
+    """One-token sequences pad their statistics to whole tiles, not the float32 copy of dq."""
+    need = lib.evg_packed_attention_bwd_workspace_bytes
+    tokens, heads = 16384, 32
+    copy = tokens * heads * 128 * 4
+    assert need(tokens, 1, heads, 128) <= copy + (tokens + 256) * heads * 8
+    assert need(tokens, tokens, heads, 128) <= copy + (tokens + tokens // 128 + 1) * 128 * heads * 8
