@@ -120,3 +120,22 @@ def test_plain_kernels_against_float64(lens, pad, hq, hkv, d, dtype):
 @pytest.mark.parametrize("lens,pad,hq,hkv,d", [([2100, 700, 1300], 0, 8, 2, 128), ([1500, 40], 9, 5, 5, 64)])
 def test_longer_sequences(lens, pad, hq, hkv, d):
     check(lens, pad, hq, hkv, d, "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", list(range(8, 129, 8)))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_every_head_size_of_the_tensor_cores(d, dtype):
+    check([140, 1, 260], 4, 4, 2, d, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,hq,hkv,d,dtype", [
+    ([4200], 3, 1, 128, "bf16"),              # two neighbouring tiles of one head per block
+    ([4100, 4300], 3, 1, 96, "fp16"),
+    ([70] * 40, 6, 2, 128, "bf16"),           # one tile per block
+    ([300, 301], 4, 2, 128, "fp16"),          # two heads' tiles per block
+    ([385, 640, 1000], 2, 2, 64, "bf16"),
+    ([300], 4, 1, 64, "fp32"), ([97, 64, 33], 2, 2, 130, "bf16")])
+def test_every_shape_of_the_blocks(lens, hq, hkv, d, dtype):
+    check(lens, 0, hq, hkv, d, dtype)
