@@ -19,8 +19,8 @@
 // it to a float32 copy of dQ by asynchronous bulk reductions, so dq can differ in the last
 // bit from run to run; a last kernel scales and rounds the copy. Only one block contributes
 // to a sequence's first query tile: it rounds and writes those rows at once (32/8 heads of
-// 128, 16384 tokens: sequences of 128 tokens 367 -> 240 us, of 512 473 -> 437, of 1024
-// 584 -> 577).
+// 128, 16384 tokens: sequences of 128 tokens 367 -> 208 us, of 512 473 -> 433, of 1024
+// 584 -> 564).
 //
 // K and V are kept in tensor memory as well (HD / 2 columns each): a product of two
 // shared-memory operands with 64 columns needs 192 bytes a clock of the shared memory's
@@ -43,9 +43,11 @@
 // of their own, three stages of Q and dO, and a stream's next S^T and dP^T are formed behind
 // its dV and dK of this tile; per half tile
 //   S(c+1)[b]  dV,dK(c)[b]  dP(c+1)[b]  dQ(c)[b]
-// (16/16 heads, 16384 tokens in sequences of 4096: 600 -> 546 us with one 16 KB piece of dQ
+// (16/16 heads, 16384 tokens in sequences of 4096: 600 -> 542 us with one 16 KB piece of dQ
 // per half; what is left is spread over the dQ warps' turns, 12 %, and waits: no single part
-// taken out brings more than 4 %).
+// taken out brings more than 4 %). Leaving out stream 1 where a last query tile has at most 64
+// rows cost more registers than it saved work (64-token sequences 177 -> 165 us, 512-token
+// ones 433 -> 449).
 // Tensor memory: S^T [0,128), dP^T [128,256), K [256,288), V [288,320), dV [320,384),
 // dK [384,448), dQ^T [448,512). The dQ^T product keeps its 128 rows: the A operand's second
 // 64 columns are whatever follows K in shared memory, and the rows they give are not read
