@@ -220,6 +220,23 @@ def test_another_stream():
     ops.device_status()
 
 
+def test_two_streams_at_once():
+    """Calls that overlap share SMs, tensor memory and nothing else."""
+    sets = [make([700, 64, 300], 9, 4, 2, 128, "bf16"), make([513, 1, 90], 0, 6, 3, 64, "fp16", seed=7)]
+    want = [run(*t) for t in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            same(r, want[i])
+
+
 def test_tensors_of_more_than_two_to_the_31_elements():
     """135168 tokens x 128 heads x 128: offsets beyond 32 bits in q, o, do, dq and in the
     float32 copy of dq. The last sequences are compared with the same rows alone."""
