@@ -237,6 +237,13 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     prefetch_tensormap(&map_v); prefetch_tensormap(&map_do);
   }
   __syncthreads();
+  if (threadIdx.x == 0) {  // the first copies do not wait for the tensor memory
+    mbar_expect_tx(done, 2 * TB);
+    load_tile<HD>(sK, &map_k, seq0 + kv0, bh, done);
+    load_tile<HD>(sDS, &map_v, seq0 + kv0, bh, done);  // V only passes through
+    mbar_expect_tx(q_full, TB);
+    load_tile<HD>(sQ0, &map_q, seq0 + kv0, bh * p.group, q_full);
+  }
   if (r.warp == 1) { tmem_alloc(bs.tmem_slot, 512); tmem_relinquish(); }
   tc_fence_before_sync();
   __syncthreads();
@@ -254,9 +261,6 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   constexpr uint32_t kDQ = kSplit ? 0 : 64;
 
   if (r.is_tma && r.lane == 0) {
-    mbar_expect_tx(done, 2 * TB);
-    load_tile<HD>(sK, &map_k, seq0 + kv0, bh, done);
-    load_tile<HD>(sDS, &map_v, seq0 + kv0, bh, done);  // V only passes through
     int it = 0, head = bh * p.group, git = 0;
     for (; git < n_git; ++git) {
       const int st = git % NST;
@@ -264,8 +268,10 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
       const int q0 = seq0 + (kvt + it) * kTile;
       if (git >= NST) mbar_wait(q_empty + st, reuse, ctx, 821);
       if (*ctx.abort_flag) break;  // no new copies after a timeout
-      mbar_expect_tx(q_full + st, TB);
-      load_tile<HD>(sQ0 + st * TB, &map_q, q0, head, q_full + st);
+      if (git > 0) {
+        mbar_expect_tx(q_full + st, TB);
+        load_tile<HD>(sQ0 + st * TB, &map_q, q0, head, q_full + st);
+      }
       if (git >= NST) mbar_wait(do_empty + st, reuse, ctx, 831);
       if (!*ctx.abort_flag) {
         const int64_t prow = head * P + prow0 + (int64_t)it * kTile;

@@ -153,6 +153,15 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
     prefetch_tensormap(&map_q); prefetch_tensormap(&map_k); prefetch_tensormap(&map_v);
   }
   __syncthreads();
+  if (threadIdx.x == 0) {  // the first copies do not wait for the tensor memory
+    mbar_expect_tx(q_full, (b_active ? 2 : 1) * TB);
+    load_tile<HD>(sQ[0], &map_q, seq0 + qt[0] * kTile, head[0], q_full);
+    if (b_active) load_tile<HD>(sQ[1], &map_q, seq0 + qt[1] * kTile, head[1], q_full);
+    mbar_expect_tx(k_full, TB);
+    load_tile<HD>(sK, &map_k, seq0, head_kv, k_full);
+    mbar_expect_tx(v_full, TB);
+    load_tile<HD>(sV, &map_v, seq0, head_kv, v_full);
+  }
   if (warp == 1) { tmem_alloc(bs.tmem_slot, 256 * TILES); tmem_relinquish(); }
   tc_fence_before_sync();
   __syncthreads();
@@ -164,10 +173,7 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
 
   if (warp == 0) {
     if (lane == 0) {
-      mbar_expect_tx(q_full, (b_active ? 2 : 1) * TB);
-      load_tile<HD>(sQ[0], &map_q, seq0 + qt[0] * kTile, head[0], q_full);
-      if (b_active) load_tile<HD>(sQ[1], &map_q, seq0 + qt[1] * kTile, head[1], q_full);
-      int j = 0;
+      int j = 1;
       for (; j < n_max; ++j) {
         const int st = j % KST;
         const uint32_t reuse = (uint32_t)((j / KST - 1) & 1);
