@@ -20,7 +20,8 @@
 // still fills both groups. Otherwise they are two neighbouring tiles of one head.
 //
 // O leaves through shared memory as whole rows: with a thread writing its own row, 128
-// sequences of 128 tokens (32/8 heads of 128) took 143 us, now 134.
+// sequences of 128 tokens (32/8 heads of 128) took 143 us, 134 this way
+// (132 with the first copies ahead of the tensor memory's allocation).
 //
 // Tiles start at the sequence's first token (a TMA coordinate along the token axis
 // has no alignment rule). The last tile's rows behind the sequence's end are other
