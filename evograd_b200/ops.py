@@ -764,8 +764,9 @@ def rope_inv_freq(rotary_dim: int, base: float = 10000.0, *, scaling: str | None
     slowest component is divided and the fastest kept; ``"wavelength"`` divides the
     components that turn less than ``slow`` times over ``original_context`` positions,
     keeps those above ``fast`` turns and blends linearly in the number of turns between;
-    ``"ramp"`` blends linearly in the component's index between the (rounded) indices
-    that make ``fast`` and ``slow`` turns and sets ``mscale = 0.1 ln(factor) + 1``."""
+    ``"ramp"`` blends linearly in the component's index between the indices that make ``fast``
+    and ``slow`` turns (rounded outwards, limited to 0 .. rotary_dim - 1) and sets
+    ``mscale = 0.1 ln(factor) + 1``."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
     if not base > 1.0 or not factor > 0.0 or original_context < 1 or not 0.0 < slow < fast:
@@ -786,7 +787,8 @@ def rope_inv_freq(rotary_dim: int, base: float = 10000.0, *, scaling: str | None
         def index_of(turns):
             return n * math.log(original_context / (turns * 2.0 * math.pi)) / math.log(base)
 
-        lo, hi = max(math.floor(index_of(fast)), 0), min(math.ceil(index_of(slow)), n - 1)
+        # (not the number of pairs: over a long context `slow` turns lie behind the last one)
+        lo, hi = max(math.floor(index_of(fast)), 0), min(math.ceil(index_of(slow)), rotary_dim - 1)
         keep = 1.0 - ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
         f = f * (keep + (1.0 - keep) / factor)
         mscale = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
