@@ -3,8 +3,8 @@
 //
 // Two kernels over a list of tensors that travels in the kernel's parameters (no copy
 // to the device, capturable): every block squares its 16384-element chunks in float32 (a
-// thread's at most 64 squares per chunk) and adds the chunks up in float64, one partial
-// per block; the second kernel's blocks each add all partials in the same fixed order
+// thread's at most 64 squares per chunk; in float64 where float32 has too little range) and
+// adds the chunks up in float64, one partial per block; the second kernel's blocks each add all partials in the same fixed order
 // and scale their chunks. Fixed order throughout, so the result is reproducible. The
 // second kernel walks the chunks backwards: what the first one read last is still in L2.
 //
@@ -45,9 +45,12 @@ __device__ __forceinline__ int find_entry(const Table<CAP>& t, int chunk) {
   return lo;
 }
 
+// A thread's part of a chunk's squares; `bits`: all elements' bits but the signs, or-ed.
 template <typename T>
-__device__ __forceinline__ float chunk_squares(const T* p, int n, bool vec) {
+__device__ __forceinline__ float chunk_squares(const T* p, int n, bool vec, uint32_t& bits) {
   constexpr int N = Vec<T>::N;
+  constexpr uint32_t kNoSigns = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
+  bits = 0;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   int done = 0;
   if (vec) {
@@ -63,6 +66,7 @@ __device__ __forceinline__ float chunk_squares(const T* p, int n, bool vec) {
         if (base + u * kThreads < nv) {
           float f[N];
           unpack<T>(v[u], f);
+          bits |= (v[u].x | v[u].y | v[u].z | v[u].w) & kNoSigns;
 #pragma unroll
           for (int i = 0; i < N; ++i) s[u & 3] = fmaf(f[i], f[i], s[u & 3]);
         }
@@ -70,16 +74,20 @@ __device__ __forceinline__ float chunk_squares(const T* p, int n, bool vec) {
   }
   for (int i = done + threadIdx.x; i < n; i += kThreads) {
     const float f = to_f32<T>(p[i]);
+    bits |= __float_as_uint(f) & 0x7fffffffu;
     s[0] = fmaf(f, f, s[0]);
   }
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
-// A thread whose squares leave float32 (elements from 1.8e19 on) adds the same elements again
-// in float64.
+// A thread whose squares leave float32 adds the same elements again in float64: an infinite sum
+// (elements from 1.8e19 on), or one below 2^-110 with an element that is not zero (elements
+// below 2.8e-17; a square below 2^-126 is off by up to 2^-150, 64 of them from there on by less
+// than 2^-33 of the sum). Chunks of zeros, common in the gradients of embeddings, are read once.
 template <typename T>
 __device__ __forceinline__ double chunk_sum(const T* p, int n, bool vec) {
-  const float s = chunk_squares(p, n, vec);
-  if (s <= 3.402823466e38f) return (double)s;
+  uint32_t bits;
+  const float s = chunk_squares(p, n, vec, bits);
+  if (s <= 3.402823466e38f && (s >= 0x1p-110f || bits == 0)) return (double)s;
   double d = 0.0;
   auto add = [&](int i) {
     const double f = (double)to_f32<T>(p[i]);

@@ -497,7 +497,9 @@ int evg_post_pre_norm_bwd(const void* dy, const void* dh, const void* x,
  * place, or into `outs` when that is not NULL. grads, outs, numel, dtypes are HOST
  * arrays (of device pointers, element counts, evg_dtype), read before the call
  * returns. Squares and a thread's sums are float32 (float64 where those would
- * overflow), sums of blocks float64, in a fixed order: bit-reproducible. A norm that is not finite scales as the formula
+ * overflow, or are so small that they lose bits), sums of blocks float64, in a fixed
+ * order: bit-reproducible. A norm beyond float32 is returned as infinity, the scaling
+ * goes by its float64 value. A norm that is not finite in float64 scales as the formula
  * says (infinite: to zero, NaN: to NaN). No counterpart in the reference.
  */
 int64_t evg_clip_grads_workspace_bytes(int64_t count);
