@@ -1023,10 +1023,10 @@ def grad_norm(grads) -> torch.Tensor:
 def clip_grad_norm(grads, max_norm: float, outs=None) -> torch.Tensor:
     """Scale all tensors by ``min(1, max_norm / (norm + 1e-6))`` with ``norm`` their global
     2-norm, in place or into ``outs`` (per gradient a tensor of its type with as many
-    elements in the same memory order, which must not overlap the gradients unless it is
-    them). Returns the norm before clipping, a float32 scalar on the device; nothing is
+    elements in the same memory order, the gradient itself or other memory). Returns the norm before clipping, a float32 scalar on the device; nothing is
     read back. A norm that is not finite scales as the formula says (infinite: finite
-    elements to zero; NaN: everything to NaN). The same tensor must not be listed twice."""
+    elements to zero; NaN: everything to NaN). Lists in which a tensor is there twice, or what
+    is written overlaps another tensor, are refused."""
     grads, dev, codes, plain, ptrs, numel = _grad_list(grads, "clip_grad_norm")
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")

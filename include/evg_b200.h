@@ -494,13 +494,15 @@ int evg_post_pre_norm_bwd(const void* dy, const void* dh, const void* x,
 /* ------------------------------------------- global gradient norm, clipping
  * norm (device float32) = sqrt(sum over `count` tensors of all squares); with
  * clip != 0 every tensor is multiplied by min(1, max_norm / (norm + 1e-6)), in
- * place, or into `outs` when that is not NULL. grads, outs, numel, dtypes are HOST
- * arrays (of device pointers, element counts, evg_dtype), read before the call
- * returns. Squares and a thread's sums are float32 (float64 where those would
- * overflow, or are so small that they lose bits), sums of blocks float64, in a fixed
- * order: bit-reproducible. A norm beyond float32 is returned as infinity, the scaling
- * goes by its float64 value. A norm that is not finite in float64 scales as the formula
- * says (infinite: to zero, NaN: to NaN). No counterpart in the reference.
+ * place, or into `outs` when that is not NULL (an entry of `outs` may be its gradient;
+ * otherwise what is written may overlap nothing that is read or written: EVG_EBADSHAPE).
+ * grads, outs, numel, dtypes are HOST arrays (of device pointers, element counts,
+ * evg_dtype), read before the call returns. Squares and a thread's sums are float32
+ * (float64 where those would overflow, or are so small that they lose bits), sums of
+ * blocks float64, in a fixed order: bit-reproducible. A norm beyond float32 is returned
+ * as infinity, the scaling goes by its float64 value. A norm that is not finite in
+ * float64 scales as the formula says (infinite: to zero, NaN: to NaN). No counterpart
+ * in the reference.
  */
 int64_t evg_clip_grads_workspace_bytes(int64_t count);
 int evg_clip_grads(const void* const* grads, void* const* outs, const int64_t* numel,
