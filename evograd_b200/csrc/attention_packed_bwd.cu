@@ -53,6 +53,19 @@
 // 64 columns are whatever follows K in shared memory, and the rows they give are not read
 // (a 64-row product has another layout in tensor memory).
 //
+// float16 has five bits of exponent, so its P and dS go into the products scaled by powers of
+// two, which come out of the results again: P by 4 (a shift of the log-sum-exp), dS by 4 G with
+//   4 G 2 HD max|do| max|v| <= 2^15,  G max|v| <= 2^15   (largest elements of a sequence and
+// k/v head), so that neither |dS_ij| <= P_ij (|do_i . v_j| + |delta_i|) nor V G overflows. G is
+// applied to V on its way into tensor memory and to delta in the subtraction, so the walk over
+// the tiles has no instruction more for it. (V G is rounded again only below 2^-14: by 2^-25,
+// 2^-13 of the largest |V| G at worst, where |do| reaches 65504.) Gradients of any size keep the
+// bits that gradients of size one have: unscaled, do of 2^-14 over 16000 tokens gave later rows of
+// dq and dk errors of 21 % (their own rounding to float16: 1.8 %), and dS above 65504 infinities.
+// The largest elements cost a read of V and a memset before: 4 x 4096 tokens, 32/8 heads of 128,
+// under 2 %; 128 x 128 tokens 242 us against bfloat16's 218; 16/16 heads of 64, 4096 tokens in
+// four sequences, forward and backward, 121 -> 125 us.
+//
 // Tiles start at the sequence's first token; rows of K, V, Q and dO behind its end are
 // other tokens and are zeroed in shared memory, and their statistics make P zero.
 #include "attention_bwd_parts.cuh"
@@ -88,6 +101,9 @@ struct BwdParams {
   float* lse2;    // [Hq][slots * 128] log-sum-exp in log2 units, +inf behind a sequence
   float* delta;   // [Hq][slots * 128]
   float* dq_acc;  // [Hq][tokens / 128 tiles][128 x HD], tiles as acc_tile numbers them
+  uint32_t* range;  // float16: [do, v][Hkv][seq_tiles], DsRange's words at a sequence's first
+                    // padded tile
+  int seq_tiles;
   View k, v, dq, dk, dv;
   int tokens, slots, units, head_group, group, D;
   float scale;
@@ -101,6 +117,24 @@ struct BwdParams {
 __device__ __forceinline__ int64_t acc_tile(const BwdParams& p, int head, int seq0, int t) {
   return (int64_t)head * (p.tokens / kTile) + seq0 / kTile + t - 1;
 }
+// float16: exponent of P's scale, and that of G for a sequence (by its first padded tile) and a
+// k/v head, from the largest |do| and |v| as float16 bits (infinities and NaN as 65504: their
+// sequence's gradients are not finite whatever the scale).
+constexpr int kPExponent = 2;
+struct DsRange {
+  uint32_t most_do, most_v;
+  __device__ __forceinline__ void load(const BwdParams& p, int tile0, int head_kv) {
+    const uint32_t* at = p.range + (int64_t)head_kv * p.seq_tiles + tile0;
+    most_do = at[0];
+    most_v = at[(int64_t)p.units * p.seq_tiles];
+  }
+  template <int HD> __device__ __forceinline__ int exponent() const {
+    // below 2^(k + 1); k = -15 for subnormal ones
+    const int k_do = min((int)(most_do >> 10), 30) - 15, k_v = min((int)(most_v >> 10), 30) - 15;
+    return min(15 - (kPExponent + 1) - (HD == 128 ? 7 : 6) - (k_do + 1) - (k_v + 1), 15 - (k_v + 1));  // -27 .. 29
+  }
+};
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -218,7 +252,9 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
   const float scale_log2 = p.scale * kLog2e;
   // A lone token's probability is one whatever its score: its dS is zero, and only rounding
   // noise of dP - delta stands in the accumulators.
-  const float ds_scale = L > 1 ? p.scale : 0.f;
+  float ds_scale = L > 1 ? p.scale : 0.f;
+  DsRange range = {0, 0};
+  if constexpr (FMT == 0) range.load(p, item.w, bh);
 
   if (threadIdx.x == 0) {
     *bs.abort_flag = 0;
@@ -465,6 +501,7 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     // step over 16 sequences of 1 to 900 tokens)
     const int64_t head_rows = (int64_t)(p.tokens / kTile) * kTile, row0 = (int64_t)(seq0 / kTile + kvt - 1) * kTile;
     const bool issuer = r.warp == 2 + kComputeWarps && r.lane == 0;
+    if constexpr (FMT == 0) ds_scale *= power_of_two(-kPExponent - range.exponent<HD>());
     int it = 0, head = bh * p.group;
     for (int c = 0; c < n_git; ++c) {
       const uint32_t par = (uint32_t)(c & 1);
@@ -530,7 +567,6 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     const int col0 = ((r.warp - 2) % kStreamWarps / 4) * 32;  // first query column inside its half tile
     const uint32_t tY = tY0 + 64 * b + lane_base + col0;
     const f32x2 neg_scale2 = f2_splat(-scale_log2);
-    const f32x2 minus_one2 = f2_splat(-1.0f);
     // Stream 0's warps put K, stream 1's V into tensor memory: a thread its key's row (half
     // of it), two 16-bit elements per column, zero behind the sequence's end. (Read from
     // global memory row by row this took 8500 cycles per block.)
@@ -549,12 +585,23 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
                            : make_uint4(0, 0, 0, 0);
         w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
       }
+      if (FMT == 0 && b) {
+        const int gain = range.exponent<HD>();
+        const __half2 g1 = __float2half2_rn(power_of_two(gain >> 1)), g2 = __float2half2_rn(power_of_two(gain - (gain >> 1)));
+#pragma unroll
+        for (int i = 0; i < 4 * PW; ++i) {
+          const __half2 x = __hmul2(__hmul2(*reinterpret_cast<const __half2*>(&w[i]), g1), g2);
+          w[i] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+      }
       const uint32_t dst = (b ? tV : tK) + lane_base + piece0 * 4;
 #pragma unroll
       for (int i = 0; i < PW / 4; ++i) tmem_st(dst + 16 * i, *reinterpret_cast<uint32_t(*)[16]>(&w[16 * i]));
       tmem_wait_st();
       warp_arrive(kv_full, r.lane);
     }
+    const float minus_gain = FMT == 0 ? -power_of_two(range.exponent<HD>()) : -1.f;
+    const f32x2 minus_gain2 = f2_splat(minus_gain);
     int it = 0;
     for (int c = 0; c < n_git; ++c) {
       const int st = c % NST;
@@ -616,9 +663,9 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const float4 d4 = del4[g];
-          const f32x2 a01 = f2_fma(f2_make(d4.x, d4.y), minus_one2,
+          const f32x2 a01 = f2_fma(f2_make(d4.x, d4.y), minus_gain2,
                                    f2_make(__uint_as_float(dr[4 * g]), __uint_as_float(dr[4 * g + 1])));
-          const f32x2 a23 = f2_fma(f2_make(d4.z, d4.w), minus_one2,
+          const f32x2 a23 = f2_fma(f2_make(d4.z, d4.w), minus_gain2,
                                    f2_make(__uint_as_float(dr[4 * g + 2]), __uint_as_float(dr[4 * g + 3])));
           float d[4], pe[4];
           f2_split(f2_mul(p2[8 * k + 2 * g], a01), d[0], d[1]);
@@ -662,8 +709,8 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
     mbar_wait(done, 1, ctx, 847);
     __syncwarp();
     tc_fence_after_sync();
-    accumulator_to_tile<HD, FMT>(tDV, sDO0, 1.0f, r);
-    accumulator_to_tile<HD, FMT>(tDK, sDO0 + TB, ds_scale, r);
+    accumulator_to_tile<HD, FMT>(tDV, sDO0, FMT == 0 ? power_of_two(-kPExponent) : 1.0f, r);
+    accumulator_to_tile<HD, FMT>(tDK, sDO0 + TB, FMT == 0 ? ds_scale * power_of_two(-kPExponent) / -minus_gain : ds_scale, r);
     named_barrier_sync(2, 32 * kComputeWarps);
     const int t = (r.warp - 2) * 32 + r.lane;
     tile_to_view<HD>(sDO0, p.dv, bh, seq0, kv0, L, p.D, t);
@@ -683,7 +730,8 @@ attn_packed_bwd_kernel(const __grid_constant__ CUtensorMap map_q,
 // and 5, rows 8 to 19: 0.27 and 2 to 3; with delta from its definition 0.23 and 0.4 in all of
 // them. So the first kExactRows rows of every sequence sum sum_j P_ij do_i . v_j. (Later rows
 // whose softmax rests on one or two keys have the same small difference and take o.)
-// A block takes 256 / (HD / 8) rows of one head.
+// A block takes 256 / (HD / 8) rows of one head at a time; bound by the latency of its loads, so six
+// blocks share an SM (134 MB of do and o each: 57 us, 120 with two blocks).
 constexpr int kExactRows = 8;
 template <int FMT> __device__ __forceinline__ float dot8(const uint4& a, const uint4& b) {
   float af[8], bf[8], s = 0.f;
@@ -692,6 +740,19 @@ template <int FMT> __device__ __forceinline__ float dot8(const uint4& a, const u
 #pragma unroll
   for (int i = 0; i < 8; ++i) s += af[i] * bf[i];
   return s;
+}
+
+// Maxima of m's and the vector's float16 without their signs (NaN left out), as two halves.
+__device__ __forceinline__ uint32_t most_of(uint32_t m, const uint4& v) {
+  const __half2* x = reinterpret_cast<const __half2*>(&v);
+  __half2 a = __hmax2(__habs2(x[0]), __habs2(x[1])), b = __hmax2(__habs2(x[2]), __habs2(x[3]));
+  a = __hmax2(__hmax2(a, b), *reinterpret_cast<const __half2*>(&m));
+  return *reinterpret_cast<const uint32_t*>(&a);
+}
+// *at = max(*at, both halves of every lane's m).
+__device__ __forceinline__ void raise(uint32_t* at, uint32_t m) {
+  m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+  if ((threadIdx.x & 31) == 0 && m) atomicMax(at, m);
 }
 
 // c += A B^T over 16 columns of A's rows 0 .. 7 (rows 8 .. 15 are zero) and B's rows 0 .. 7.
@@ -708,9 +769,9 @@ __device__ __forceinline__ void mma_8x8(float (&c)[4], uint32_t a0, uint32_t a1,
 // do and values) in a few matrix instructions each. Lane l holds row l / 4 of either side, 16
 // bytes of every 32 columns; which column of a product's 16 they stand for is the same on both
 // sides and does not matter. Latency-bound (three dependent loads), so eight sequences share a
-// block of their own. Backward of 128 sequences of 128 tokens, 32/8 heads of 128: 222 us, 212
-// with delta from o, 266 with these rows summed one by one beside the others; of 32 sequences of
-// 512: 445 and 441.
+// block of their own. Backward of 128 sequences of 128 tokens, 32/8 heads of 128, bfloat16: 218
+// us, 212 with delta from o, 266 with these rows summed one by one beside the others; of 32
+// sequences of 512: 443 and 441.
 template <int HD, int FMT>
 __device__ __forceinline__ void exact_delta(const View& dout, const View& q, const float* lse, const BwdParams& p,
                                             const int4& item, int head, float* delta) {
@@ -718,20 +779,16 @@ __device__ __forceinline__ void exact_delta(const View& dout, const View& q, con
   const bool ok = r < item.y;
   const int64_t token = item.x + (ok ? r : 0);
   auto product = [&](const uint8_t* a_row, const uint8_t* b_row, float (&c)[4]) {
-    uint4 a[HD / 32], b[HD / 32];
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) {
       const int col = 32 * i + 8 * part;
-      a[i] = b[i] = make_uint4(0, 0, 0, 0);
+      uint4 a = make_uint4(0, 0, 0, 0), b = a;
       if (ok && col < p.D) {
-        a[i] = ld_vec(a_row + 2 * col);
-        b[i] = ld_vec(b_row + 2 * col);
+        a = ld_vec(a_row + 2 * col);
+        b = ld_vec(b_row + 2 * col);
       }
-    }
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-      mma_8x8<FMT>(c, a[i].x, a[i].y, b[i].x, b[i].y);
-      mma_8x8<FMT>(c, a[i].z, a[i].w, b[i].z, b[i].w);
+      mma_8x8<FMT>(c, a.x, a.y, b.x, b.y);
+      mma_8x8<FMT>(c, a.z, a.w, b.z, b.w);
     }
   };
   float s[4] = {0.f, 0.f, 0.f, 0.f}, dp[4] = {0.f, 0.f, 0.f, 0.f};
@@ -748,7 +805,7 @@ __device__ __forceinline__ void exact_delta(const View& dout, const View& q, con
 }
 
 template <int HD, int FMT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 6)
 packed_prepare_kernel(const View dout, const View q, const View o, const float* __restrict__ lse,
                       const BwdParams p) {
   constexpr int TPR = HD / 8;
@@ -766,24 +823,40 @@ packed_prepare_kernel(const View dout, const View q, const View o, const float* 
   const int part = threadIdx.x % TPR;
   const int tile0 = (item.z - 1) * kTile;
   const int64_t prow0 = (int64_t)head * p.slots * kTile + (int64_t)item.w * kTile + tile0;
+  const bool takes_v = FMT == 0 && head % p.group == 0;
+  uint32_t most_do = 0, most_v = 0;  // two float16 each, signs off: ordered as the numbers
+#pragma unroll 1
   for (int r = threadIdx.x / TPR + blockIdx.z * ROWS; r < kTile; r += ROWS * gridDim.z) {
     const bool ok = tile0 + r < item.y, mine = ok && part * 8 < p.D;
     const int64_t token = item.x + tile0 + r;
-    const uint4 none = make_uint4(0, 0, 0, 0);
-    const uint4 g = mine ? ld_vec(view_row(dout, token, head) + part * 16) : none;
+    uint4 g, ov, vv;
+    g = ov = vv = make_uint4(0, 0, 0, 0);
+    if (mine) {
+      g = ld_vec(view_row(dout, token, head) + part * 16);
+      ov = ld_vec(view_row(o, token, head) + part * 16);
+      if (takes_v) vv = ld_vec(view_row(p.v, token, head / p.group) + part * 16);
+    }
     const float lse_row = ok ? lse[(int64_t)head * p.tokens + token] : 0.f;
-    float s = 0.f;
-    if (mine) s = dot8<FMT>(g, ld_vec(view_row(o, token, head) + part * 16));
+    float s = dot8<FMT>(g, ov);
 #pragma unroll
     for (int off = TPR / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if constexpr (FMT == 0) {
+      most_do = most_of(most_do, g);
+      if (takes_v) most_v = most_of(most_v, vv);
+    }
     if (item.z > 1) {
       uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (acc_tile(p, head, item.x, item.z - 1) * kTile + r) * HD + part * 8);
       acc[0] = acc[1] = make_uint4(0, 0, 0, 0);
     }
     if (part == 0) {
       if (item.z > 1 || r >= kExactRows) p.delta[prow0 + r] = ok ? s : 0.f;
-      p.lse2[prow0 + r] = ok ? lse_row * kLog2e : INFINITY;
+      p.lse2[prow0 + r] = ok ? lse_row * kLog2e - (FMT == 0 ? kPExponent : 0) : INFINITY;
     }
+  }
+  if constexpr (FMT == 0) {
+    uint32_t* at = p.range + (int64_t)(head / p.group) * p.seq_tiles + item.w;
+    raise(at, most_do);
+    if (takes_v) raise(at + (int64_t)p.units * p.seq_tiles, most_v);
   }
 }
 
@@ -801,6 +874,14 @@ packed_finish_kernel(const BwdParams p) {
   if (part * 8 >= p.D) return;
   const int tile0 = item.z > 0 ? (item.z - 1) * kTile : 0;
   const int rows = min(kTile, item.y - tile0);
+  float scale = p.scale;
+  if constexpr (FMT == 0) {
+    if (item.z > 0) {
+      DsRange range;
+      range.load(p, item.w, head / p.group);
+      scale *= power_of_two(-kPExponent - range.exponent<HD>());
+    }
+  }
   for (int qd = threadIdx.x / TPR + blockIdx.z * QUADS; qd * 4 < rows; qd += QUADS * gridDim.z) {
     float v[4][8];
     if (item.z > 0) {
@@ -818,10 +899,10 @@ packed_finish_kernel(const BwdParams p) {
     for (int i = 0; i < 4; ++i)
       if (qd * 4 + i < rows) {
         uint4 pk;
-        pk.x = pack2<FMT>(v[i][0] * p.scale, v[i][1] * p.scale);
-        pk.y = pack2<FMT>(v[i][2] * p.scale, v[i][3] * p.scale);
-        pk.z = pack2<FMT>(v[i][4] * p.scale, v[i][5] * p.scale);
-        pk.w = pack2<FMT>(v[i][6] * p.scale, v[i][7] * p.scale);
+        pk.x = pack2<FMT>(v[i][0] * scale, v[i][1] * scale);
+        pk.y = pack2<FMT>(v[i][2] * scale, v[i][3] * scale);
+        pk.z = pack2<FMT>(v[i][4] * scale, v[i][5] * scale);
+        pk.w = pack2<FMT>(v[i][6] * scale, v[i][7] * scale);
         *reinterpret_cast<uint4*>(view_row(p.dq, item.x + tile0 + qd * 4 + i, head) + part * 16) = pk;
       }
   }
@@ -861,6 +942,8 @@ int launch(const View& dout, const View& q, const View& o, const float* lse, Bwd
   const int64_t want = (4 * (int64_t)device_info().sm_count + tiles - 1) / tiles;
   const int parts = (int)(want < 1 ? 1 : want > kMostParts ? kMostParts : want);
   const dim3 rows_grid((unsigned)p.slots, (unsigned)Hq, (unsigned)parts);
+  if (FMT == 0 && cudaMemsetAsync(p.range, 0, (size_t)2 * p.units * p.seq_tiles * 4, stream) != cudaSuccess)
+    return check_launch("packed_attention_bwd range");
   const dim3 prepare_grid((unsigned)(p.slots + (p.slots + 7) / 8), rows_grid.y, rows_grid.z);
   packed_prepare_kernel<HD, FMT><<<prepare_grid, 256, 0, stream>>>(dout, q, o, lse, p);
   if (int rc = check_launch("packed_attention_bwd statistics")) return rc;
@@ -874,9 +957,13 @@ int launch(const View& dout, const View& q, const View& o, const float* lse, Bwd
 
 namespace packed {
 
+// Most padded tiles of all sequences together.
+int64_t sequence_tiles(int64_t tokens, int64_t sequences) {
+  return (tokens + (kTile - 1) * (sequences < tokens ? sequences : tokens)) / kTile;
+}
 int64_t bwd_workspace_bytes(int64_t tokens, int64_t sequences, int64_t Hq, int64_t D) {
   const int64_t rows = plan_slots(tokens, sequences) * kTile * Hq;
-  return rows * 2 * 4 + tokens / kTile * kTile * Hq * (D > 64 ? 128 : 64) * 4;
+  return rows * 2 * 4 + tokens / kTile * kTile * Hq * (D > 64 ? 128 : 64) * 4 + sequence_tiles(tokens, sequences) * Hq * 8;
 }
 
 int launch_bwd(const View& dout, const View& q, const View& k, const View& v, const View& o,
@@ -891,6 +978,8 @@ int launch_bwd(const View& dout, const View& q, const View& k, const View& v, co
   p.lse2 = (float*)workspace;
   p.delta = p.lse2 + rows;
   p.dq_acc = p.delta + rows;
+  p.range = (uint32_t*)(p.dq_acc + tokens / kTile * kTile * Hq * (D > 64 ? 128 : 64));
+  p.seq_tiles = (int)sequence_tiles(tokens, sequences);
   p.k = k;
   p.v = v;
   p.dq = dq;

@@ -423,8 +423,10 @@ int64_t evg_packed_attention_bwd_workspace_bytes(int64_t tokens, int64_t sequenc
  * bit-reproducible; on the tensor-core path dq is summed with float32 global
  * adds and can differ in the last bit from run to run. The workspace (16-byte
  * aligned) holds two floats per query head and row, rows padded to whole 128-row
- * tiles per sequence, and a float32 copy of dq behind the sequences' first tiles
- * (tokens / 128 tiles at most).
+ * tiles per sequence, a float32 copy of dq behind the sequences' first tiles
+ * (tokens / 128 tiles at most), and two words per padded tile and query head.
+ * float16 gradients are formed at a scale of their own per sequence and k/v head: dout
+ * may be of any size (a loss scale) whose results float16 holds.
  */
 int evg_packed_attention_bwd(const evg_packed_view* dout, const evg_packed_view* q,
                              const evg_packed_view* k, const evg_packed_view* v,
