@@ -8,6 +8,7 @@
 #include <string>
 
 #include "evg_common.cuh"
+#include "shared_memory.cuh"
 
 namespace evg {
 
@@ -62,6 +63,33 @@ int tune(const char* key) {
   auto& m = tune_map();
   auto it = m.find(key);
   return it == m.end() ? 0 : it->second;
+}
+
+bool allow_shared_memory(const void* kernel, size_t bytes) {
+  // A thread remembers what it has raised (the calls take the host as long as a launch); raising
+  // again, here or in another thread, sets the same value.
+  struct Raised {
+    const void* kernel;
+    int device;
+    size_t most;
+  };
+  constexpr int kSlots = 64;
+  static thread_local Raised raised[kSlots] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  Raised& r = raised[(reinterpret_cast<uintptr_t>(kernel) / 16 + (uintptr_t)dev) % kSlots];
+  if (r.kernel != kernel || r.device != dev) {
+    cudaFuncAttributes attr;
+    const size_t room = (size_t)device_info().max_smem_optin;
+    if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess || attr.sharedSizeBytes > room ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)(room - attr.sharedSizeBytes)) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
+    r = Raised{kernel, dev, room - attr.sharedSizeBytes};
+  }
+  return bytes <= r.most;
 }
 
 const DeviceInfo& device_info() {

@@ -117,11 +117,8 @@ inline long long wait_limit_cycles2() {
 
 template <typename Kernel>
 int reserve_smem(Kernel kernel, size_t bytes) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
-      cudaSuccess) {
-    cudaGetLastError();
+  if (!allow_shared_memory((const void*)kernel, bytes))
     return fail(EVG_ELAUNCH, "attention backward: cannot reserve %zu bytes of shared memory", bytes);
-  }
   return EVG_OK;
 }
 

@@ -4,6 +4,7 @@
 #pragma once
 
 #include "evg_common.cuh"
+#include "shared_memory.cuh"
 #include "sm100_umma.cuh"
 
 namespace evg {

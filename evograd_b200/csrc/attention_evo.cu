@@ -468,13 +468,10 @@ size_t evo_smem(Kernel kernel, int bufs, int64_t N, int64_t D, int* staged) {
   const size_t base = (size_t)kWarps * bufs * D * sizeof(float);
   const size_t want = base + 2 * (size_t)N * staged_pitch((int)D) * sizeof(T);
   *staged = 0;
-  if (!tune("evoattention.no_stage") && want <= (size_t)device_info().max_smem_optin &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)want) ==
-          cudaSuccess) {
+  if (!tune("evoattention.no_stage") && allow_shared_memory((const void*)kernel, want)) {
     *staged = 1;
     return want;
   }
-  cudaGetLastError();
   return base;
 }
 

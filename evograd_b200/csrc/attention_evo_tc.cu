@@ -811,11 +811,8 @@ long long evo_wait_limit() {
 
 template <typename Kernel>
 int evo_reserve(Kernel kernel, size_t bytes) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) !=
-      cudaSuccess) {
-    cudaGetLastError();
+  if (!allow_shared_memory((const void*)kernel, bytes))
     return fail(EVG_ELAUNCH, "evoattention: cannot reserve %zu bytes of shared memory", bytes);
-  }
   return EVG_OK;
 }
 

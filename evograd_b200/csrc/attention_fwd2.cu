@@ -302,11 +302,8 @@ int launch_fwd2(const void* q, const void* k, const void* v, void* o, float* lse
     return fail(EVG_ELAUNCH, "causal_attention_fwd: cuTensorMapEncodeTiled failed");
   const size_t smem = 6 * tile_bytes<HD>() + kControlBytes + 1024;
   auto kern = attn_fwd2_kernel<HD, FMT>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-      cudaSuccess) {
-    cudaGetLastError();
+  if (!allow_shared_memory((const void*)kern, smem))
     return fail(EVG_ELAUNCH, "causal_attention_fwd: cannot reserve %zu bytes of shared memory", smem);
-  }
   const int64_t n_tiles = (S + kTile - 1) / kTile;
   const int64_t n_pairs = (n_tiles + 1) / 2;
   dim3 grid((unsigned)(n_pairs * B * H));

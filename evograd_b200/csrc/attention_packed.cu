@@ -345,11 +345,8 @@ int launch_generic(const char* what, Kernel kernel, const GenericParams& p, int6
                    int64_t heads, int rows_per_warp, cudaStream_t stream) {
   const dim3 grid((unsigned)slots, (unsigned)heads, (unsigned)(attn::kTile / kWarps));
   const size_t smem = generic_smem(p.D, rows_per_warp);
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)smem) != cudaSuccess) {
-    cudaGetLastError();
+  if (smem > 48 * 1024 && !allow_shared_memory((const void*)kernel, smem))
     return fail(EVG_ELAUNCH, "%s: cannot reserve %zu bytes of shared memory", what, smem);
-  }
   kernel<<<grid, kWarps * 32, smem, stream>>>(p);
   return check_launch(what);
 }

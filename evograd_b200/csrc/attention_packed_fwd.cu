@@ -421,11 +421,8 @@ int launch(const View& q, const View& k, const View& v, const FwdParams& p, int6
     return fail(EVG_ELAUNCH, "packed_attention_fwd: cuTensorMapEncodeTiled failed");
   const size_t smem = fwd_smem_tiles<HD, TILES>() * tile_bytes<HD>() + kControlBytes + 1024;
   auto kern = attn_packed_fwd_kernel<HD, FMT, TILES>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-      cudaSuccess) {
-    cudaGetLastError();
+  if (!allow_shared_memory((const void*)kern, smem))
     return fail(EVG_ELAUNCH, "packed_attention_fwd: cannot reserve %zu bytes of shared memory", smem);
-  }
   kern<<<(unsigned)((int64_t)p.slots * p.units), fwd_threads(TILES), smem, stream>>>(mq, mk, mv, p);
   return check_launch("packed_attention_fwd");
 }

@@ -23,6 +23,7 @@
 // sums stay in registers. Column sums leave as one float32 partial row per block and are
 // added by a second kernel in a fixed order.
 #include "evg_common.cuh"
+#include "shared_memory.cuh"
 #include "sm100_umma.cuh"
 
 namespace evg {
@@ -899,7 +900,7 @@ int occupancy(const void* kernel, int threads, size_t smem) {
   int occ = 0;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kernel, threads, smem) != cudaSuccess) {
     cudaGetLastError();
-    occ = 1;
+    return 1;  // of this call only
   }
   if (occ < 1) occ = 1;
   known[next++ % 8] = Known{kernel, dev, threads, occ, smem};
@@ -921,11 +922,8 @@ template <typename Kernel>
 int launch_rows(const char* what, Kernel kernel, const NormArgs& a, const Shape& s, size_t smem,
                 cudaStream_t st, int& blocks) {
   // (the limit without the attribute, 48 KB, includes the static part)
-  if (smem > 32 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)smem) != cudaSuccess) {
-    cudaGetLastError();
+  if (smem > 32 * 1024 && !allow_shared_memory((const void*)kernel, smem))
     return fail(EVG_ELAUNCH, "%s: cannot reserve %zu bytes of shared memory", what, smem);
-  }
   blocks = blocks_for(kernel, s, a.rows, smem);
   kernel<<<blocks, s.threads, smem, st>>>(a);
   return check_launch(what);
