@@ -21,8 +21,10 @@ all layers. ``clip_grad_norm`` of :mod:`evograd_b200.ops` takes the gradients as
 come.
 
 Saved state: y, the projection (rotated), the attention's output and log-sum-exp, both
-blocks' outputs, both residual streams, the four float32 rstd vectors and the MLP's
-gate / up activations; y1 and the SwiGLU product are formed again in the backward.
+blocks' outputs, both residual streams, y1, the four float32 rstd vectors and the MLP's
+gate / up activations; the SwiGLU product is formed again in the backward, from the same
+numbers. (y1 could not be: the forward normalises h1 before it is rounded, so a y1 formed
+from the saved h1 differs in the last bits from the one that the projections multiplied.)
 """
 
 from __future__ import annotations
@@ -85,14 +87,15 @@ def packed_layer_forward(h, y, w: PackedLayerWeights, batch: PackedBatch, *, hea
     g, u = torch.mm(y1, w.mlp_gate.t()), torch.mm(y1, w.mlp_up.t())
     mlp = torch.mm(ops.swiglu_fwd(g, u), w.mlp_down.t())
     h2, y2, rc, rd = ops.post_pre_norm_fwd(mlp, h1, w.post_mlp, w.pre_next, w.gate_mlp, alpha=alpha, eps=eps)
-    return h2, y2, (y, qkv, o, lse, attn, h1, mlp, h2, ra, rb, rc, rd, g, u)
+    return h2, y2, (y, qkv, o, lse, attn, h1, y1, mlp, h2, ra, rb, rc, rd, g, u)
 
 
 def packed_layer_backward(dh2, dy2, saved, w: PackedLayerWeights, batch: PackedBatch, *, heads: int,
                           kv_heads: int, alpha: float = 1.0, eps: float = 1e-6):
     """From the gradients of ``h2`` and ``y2``: ``(dh, dy, dw)`` with ``dw`` a
-    :class:`PackedLayerWeights` of gradients."""
-    y, qkv, o, lse, attn, h1, mlp, h2, ra, rb, rc, rd, g, u = saved
+    :class:`PackedLayerWeights` of gradients. Arguments as in the forward (whose rstd vectors
+    are saved: ``eps`` enters no sum here)."""
+    y, qkv, o, lse, attn, h1, y1, mlp, h2, ra, rb, rc, rd, g, u = saved
     q, k, v = _thirds(qkv, heads, kv_heads, o.shape[2])
 
     d_mlp, dh1, d_post_mlp, d_pre_next, d_gate_mlp = ops.post_pre_norm_bwd(
@@ -100,7 +103,6 @@ def packed_layer_backward(dh2, dy2, saved, w: PackedLayerWeights, batch: PackedB
     act = ops.swiglu_fwd(g, u)
     d_down = torch.mm(d_mlp.t(), act)
     dg, du = ops.swiglu_bwd(torch.mm(d_mlp, w.mlp_down), g, u)
-    y1, _ = ops.rmsnorm_fwd(h1, w.pre_mlp, eps)
     d_mlp_gate, d_mlp_up = torch.mm(dg.t(), y1), torch.mm(du.t(), y1)
     dy1 = torch.addmm(torch.mm(dg, w.mlp_gate), du, w.mlp_up)
 
