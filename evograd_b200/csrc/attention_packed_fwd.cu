@@ -426,13 +426,6 @@ int launch(const View& q, const View& k, const View& v, const FwdParams& p, int6
   kern<<<(unsigned)((int64_t)p.slots * p.units), fwd_threads(TILES), smem, stream>>>(mq, mk, mv, p);
   return check_launch("packed_attention_fwd");
 }
-template <int HD, int FMT>
-int launch_tiles(const View& q, const View& k, const View& v, const FwdParams& p, int tiles, int64_t Hq,
-                 int64_t Hkv, cudaStream_t stream) {
-  return tiles == 1 ? launch<HD, FMT, 1>(q, k, v, p, Hq, Hkv, stream)
-                    : launch<HD, FMT, 2>(q, k, v, p, Hq, Hkv, stream);
-}
-
 }  // namespace
 
 namespace packed {
@@ -466,11 +459,11 @@ int launch_fwd(const View& q, const View& k, const View& v, const View& o, float
   p.scale_log2 = scale * kLog2e;
   const int t = tune("attention.wait_limit");
   p.wait_limit = t > 0 ? (long long)t * 1000000ll : 2000000000ll;
-  if (D > 64)
-    return fmt == 1 ? launch_tiles<128, 1>(q, k, v, p, tiles, Hq, Hkv, stream)
-                    : launch_tiles<128, 0>(q, k, v, p, tiles, Hq, Hkv, stream);
-  return fmt == 1 ? launch_tiles<64, 1>(q, k, v, p, tiles, Hq, Hkv, stream)
-                  : launch_tiles<64, 0>(q, k, v, p, tiles, Hq, Hkv, stream);
+  if (D <= 64)
+    return fmt == 1 ? launch<64, 1, 1>(q, k, v, p, Hq, Hkv, stream) : launch<64, 0, 1>(q, k, v, p, Hq, Hkv, stream);
+  if (tiles == 1)
+    return fmt == 1 ? launch<128, 1, 1>(q, k, v, p, Hq, Hkv, stream) : launch<128, 0, 1>(q, k, v, p, Hq, Hkv, stream);
+  return fmt == 1 ? launch<128, 1, 2>(q, k, v, p, Hq, Hkv, stream) : launch<128, 0, 2>(q, k, v, p, Hq, Hkv, stream);
 }
 
 }  // namespace packed

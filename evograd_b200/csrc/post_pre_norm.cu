@@ -48,7 +48,7 @@ struct NormArgs {
 
 // How a row reaches its threads.
 //   kWarp    a warp per row, global loads (rows of up to 64 16-byte vectors)
-//   kDirect  a block per row, global loads (rows of which two do not fit shared memory)
+//   kDirect  a block per row, global loads (rows of more than 1024 vectors: four per thread)
 //   kRing    a block per row; the block's next rows are on their way into a ring of
 //            shared-memory stages (untiled bulk copies, one issuing thread, bounded waits)
 enum Mode { kWarp = 0, kDirect = 1, kRing = 2 };
@@ -847,8 +847,7 @@ struct Shape {
 // against the kernels that read the row three times: 201 columns 138 -> 34 us, 1001
 // 284 -> 105, 4098 961 -> 526, 6001 1668 -> 648, 8001 2418 -> 1204; with one shape of 16
 // elements from 4097 on, 4098 took 894); all wider rows the kernels for any width.
-// `arrays`: rows read per row.
-Shape pick_shape(int64_t C, size_t elem, bool aligned, int arrays, bool backward) {
+Shape pick_shape(int64_t C, size_t elem, bool aligned, bool backward) {
   const int one_vector_most = backward ? 256 : 512;
   Shape s{};
   if (!aligned || (C * elem) % 16 != 0 || C * elem / 16 > 2048) {
@@ -872,11 +871,10 @@ Shape pick_shape(int64_t C, size_t elem, bool aligned, int arrays, bool backward
   }
   s.V = nvec <= one_vector_most ? 1 : nvec <= 1024 ? 2 : 4;
   s.threads = ((nvec + s.V - 1) / s.V + 31) / 32 * 32;
-  // Ring of two stages where one block's fit: a third or fourth stage, or wider vectors for
-  // fewer blocks, measured 1-4 % slower (a block waits for its own reductions, not for its
-  // rows, so more blocks beat deeper rings).
-  const int64_t room = device_info().max_smem_optin - 1024;
-  s.mode = kMaxStages * arrays * C * (int64_t)elem <= room && s.V <= 2 ? kRing : kDirect;
+  // Ring of two stages for rows of up to 1024 vectors (five arrays of 16 KB twice: 160 KB); a third
+  // or fourth stage, or wider vectors for fewer blocks, measured 1-4 % slower (a block waits for
+  // its own reductions, not for its rows, so more blocks beat deeper rings).
+  s.mode = s.V <= 2 ? kRing : kDirect;
   s.stages = kMaxStages;
   return s;
 }
@@ -975,7 +973,7 @@ int run_fwd(const NormArgs& a, int gate, const Shape& s, cudaStream_t st) {
   }
   if (s.mode == kWarp) return s.V == 1 ? launch_fwd<T, 1, kWarp>(a, gate, s, st) : launch_fwd<T, 2, kWarp>(a, gate, s, st);
   if (s.mode == kRing) return s.V == 1 ? launch_fwd<T, 1, kRing>(a, gate, s, st) : launch_fwd<T, 2, kRing>(a, gate, s, st);
-  return s.V == 2 ? launch_fwd<T, 2, kDirect>(a, gate, s, st) : launch_fwd<T, 4, kDirect>(a, gate, s, st);
+  return launch_fwd<T, 4, kDirect>(a, gate, s, st);
 }
 
 template <typename T>
@@ -1003,15 +1001,14 @@ int run_bwd_rows(const NormArgs& a, int gate, const Shape& s, cudaStream_t st, i
     return s.V == 1 ? launch_bwd<T, 1, kWarp>(a, gate, s, st, blocks) : launch_bwd<T, 2, kWarp>(a, gate, s, st, blocks);
   if (s.mode == kRing)
     return s.V == 1 ? launch_bwd<T, 1, kRing>(a, gate, s, st, blocks) : launch_bwd<T, 2, kRing>(a, gate, s, st, blocks);
-  return s.V == 2 ? launch_bwd<T, 2, kDirect>(a, gate, s, st, blocks) : launch_bwd<T, 4, kDirect>(a, gate, s, st, blocks);
+  return launch_bwd<T, 4, kDirect>(a, gate, s, st, blocks);
 }
 
-int check_norm_args(const char* what, int64_t rows, int64_t C, int gate, float alpha, int dtype) {
+int check_norm_args(const char* what, int64_t rows, int64_t C, int gate, int dtype) {
   if (rows < 0 || C <= 0 || rows > 0x7fffffff || C > (1 << 26))
     return fail(EVG_EBADSHAPE, "%s: rows=%lld hidden=%lld", what, (long long)rows, (long long)C);
   if (gate < kNone || gate > kFull) return fail(EVG_EBADSHAPE, "%s: gate kind %d", what, gate);
   if (dtype != EVG_F32 && dtype != EVG_F16 && dtype != EVG_BF16) return fail(EVG_EDTYPE, "%s: dtype %d", what, dtype);
-  (void)alpha;
   return EVG_OK;
 }
 
@@ -1025,7 +1022,7 @@ extern "C" int evg_post_pre_norm_fwd(const void* x, const void* h, const void* w
                                      void* y, float* rstd_post, float* rstd_pre, int64_t rows,
                                      int64_t hidden, float alpha, float eps, int dtype, void* stream) {
   const char* what = "post_pre_norm_fwd";
-  if (int rc = check_norm_args(what, rows, hidden, gate_kind, alpha, dtype)) return rc;
+  if (int rc = check_norm_args(what, rows, hidden, gate_kind, dtype)) return rc;
   if (rows == 0) return EVG_OK;
   if (!x || !h || !w_post || !w_pre || !h_out || !y || !rstd_post || !rstd_pre ||
       (gate_kind != kNone && !gate))
@@ -1037,7 +1034,7 @@ extern "C" int evg_post_pre_norm_fwd(const void* x, const void* h, const void* w
   bool aligned = true;
   for (const void* p : {x, h, w_post, w_pre, (const void*)h_out, (const void*)y}) aligned = aligned && aligned16(p);
   if (gate_kind == kChannel || gate_kind == kFull) aligned = aligned && aligned16(gate);
-  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned, gate_kind == kFull ? 3 : 2, false);
+  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned, false);
   a.stages = s.stages;
   return EVG_DISPATCH_DTYPE(dtype, [&] { return run_fwd<T>(a, gate_kind, s, (cudaStream_t)stream); });
 }
@@ -1056,7 +1053,7 @@ extern "C" int evg_post_pre_norm_bwd(const void* dy, const void* dh, const void*
                                      void* workspace, int64_t workspace_bytes, int64_t rows,
                                      int64_t hidden, float alpha, int dtype, void* stream) {
   const char* what = "post_pre_norm_bwd";
-  if (int rc = check_norm_args(what, rows, hidden, gate_kind, alpha, dtype)) return rc;
+  if (int rc = check_norm_args(what, rows, hidden, gate_kind, dtype)) return rc;
   if (rows == 0) return fail(EVG_EBADSHAPE, "%s: rows=0", what);
   if (!dy || !dh || !x || !h_out || !w_post || !w_pre || !rstd_post || !rstd_pre || !dx || !dres ||
       !dw_post || !dw_pre || (gate_kind != kNone && (!gate || !dgate)))
@@ -1075,7 +1072,7 @@ extern "C" int evg_post_pre_norm_bwd(const void* dy, const void* dh, const void*
   for (const void* p : {dy, dh, x, h_out, w_post, w_pre, (const void*)dx, (const void*)dres}) aligned = aligned && aligned16(p);
   if (gate_kind == kChannel) aligned = aligned && aligned16(gate);
   if (gate_kind == kFull) aligned = aligned && aligned16(gate) && aligned16(dgate);
-  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned, gate_kind == kFull ? 5 : 4, true);
+  const Shape s = pick_shape(hidden, dtype_size(dtype), aligned, true);
   a.stages = s.stages;
   cudaStream_t st = (cudaStream_t)stream;
   return EVG_DISPATCH_DTYPE(dtype, [&] {
