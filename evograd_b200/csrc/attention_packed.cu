@@ -340,6 +340,15 @@ int check_args(const char* what, const void* plan, int64_t tokens, int64_t seque
   return EVG_OK;
 }
 
+// Blocks read the inputs while others write: an output may not be an input or another output.
+int check_outputs(const char* what, const evg_packed_view* const* views, int inputs, int count) {
+  for (int i = inputs; i < count; ++i)
+    for (int j = 0; j < i; ++j)
+      if (views[i]->data == views[j]->data)
+        return fail(EVG_EBADSHAPE, "%s: an output starts where another tensor does", what);
+  return EVG_OK;
+}
+
 template <typename Kernel>
 int launch_generic(const char* what, Kernel kernel, const GenericParams& p, int64_t slots,
                    int64_t heads, int rows_per_warp, cudaStream_t stream) {
@@ -375,6 +384,8 @@ extern "C" int evg_packed_attention_fwd(const evg_packed_view* q, const evg_pack
   if (tokens == 0) return EVG_OK;
   if (!q->data || !k->data || !v->data || !o->data || !lse)
     return fail(EVG_ENULL, "%s: null pointer argument", what);
+  const evg_packed_view* views[4] = {q, k, v, o};
+  if (int rc = check_outputs(what, views, 3, 4)) return rc;
   const View vq = view_of(q), vk = view_of(k), vv = view_of(v), vo = view_of(o);
   cudaStream_t st = (cudaStream_t)stream;
   if (tensor_core_shape(D, dtype) && tile_view(vq) && tile_view(vk) && tile_view(vv) && tile_view(vo))
@@ -429,6 +440,7 @@ extern "C" int evg_packed_attention_bwd(const evg_packed_view* dout, const evg_p
     return fail(EVG_EWORKSPACE, "%s: workspace %lld bytes, need %lld", what,
                 (long long)workspace_bytes, (long long)need);
   if (!aligned16(workspace)) return fail(EVG_EALIGN, "%s: the workspace must be 16-byte aligned", what);
+  if (int rc = check_outputs(what, views, 5, 8)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   if (tiles)
     return launch_bwd(view_of(dout), view_of(q), view_of(k), view_of(v), view_of(o), lse,

@@ -277,6 +277,15 @@ extern "C" int evg_rope_positions(const evg_rope_positions_tensor* tensors, int 
     total += t.heads;
   }
   if (tokens == 0 || total == 0) return EVG_OK;
+  // Rows are turned at the same time: in place is one row over itself, anything else a race.
+  for (int i = 0; i < count; ++i)
+    for (int j = 0; j < count; ++j) {
+      const evg_rope_positions_tensor &y = tensors[i], &x = tensors[j];
+      if (y.heads == 0 || x.heads == 0) continue;
+      const bool moved = (tokens > 1 && y.y_stride_t != x.x_stride_t) || (x.heads > 1 && y.y_stride_h != x.x_stride_h);
+      if ((y.y == x.x && (i != j || moved)) || (i < j && y.y == x.y))
+        return fail(EVG_EBADSHAPE, "%s: output %d lies over another tensor, or over its own in another order", what, i);
+    }
   if (!positions || !inv_freq) return fail(EVG_ENULL, "%s: null pointer argument", what);
   if ((uintptr_t)positions % position_bytes || (uintptr_t)inv_freq % freq_bytes)
     return fail(EVG_EALIGN, "%s: positions / frequencies are not aligned to their element", what);

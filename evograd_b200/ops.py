@@ -847,8 +847,8 @@ def rope_positions_fwd(q, k, positions, inv_freq, *, interleaved: bool = False, 
     ``positions[t] * inv_freq[i]`` in one launch. The first ``2 * len(inv_freq)`` columns
     rotate, in two halves or, ``interleaved``, in neighbouring pairs; the rest is copied.
     cos and sin are multiplied by ``mscale``. Strided views are taken as they are; ``outs``
-    supplies the results and may be the inputs themselves (in place). Returns a tuple with
-    one tensor per input."""
+    supplies the results: the inputs themselves (in place), or tensors that overlap neither an
+    input nor one another. Returns a tuple with one tensor per input."""
     return _rope_positions((q, k), positions, inv_freq, interleaved, mscale, False, outs)
 
 

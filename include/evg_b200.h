@@ -408,7 +408,8 @@ typedef struct evg_packed_view {
  * (pointers, strides in multiples of 8 elements) run on the tensor cores;
  * everything else (float32, D <= 256) on plain CUDA-core kernels. Views are HOST
  * structs, read before the call returns. `plan` must have been made for the same
- * `tokens` and `sequences`.
+ * `tokens` and `sequences`. Outputs, here and in the backward, overlap neither an
+ * input nor one another (EVG_EBADSHAPE where they start at the same address).
  */
 int evg_packed_attention_fwd(const evg_packed_view* q, const evg_packed_view* k,
                              const evg_packed_view* v, const evg_packed_view* o,
@@ -447,7 +448,9 @@ int evg_packed_attention_bwd(const evg_packed_view* dout, const evg_packed_view*
  * columns behind rotary_dim are copied. The angle is formed and reduced in
  * float64. positions: int32 or int64 (position_bytes 4 / 8), any sign; inv_freq
  * [rotary_dim/2] float32 or float64 (freq_bytes 4 / 8), both on the device.
- * Strides in elements, last dimension contiguous; y may be x (same strides).
+ * Strides in elements, last dimension contiguous. A tensor's y may be its x (same
+ * strides); otherwise outputs overlap neither an input nor one another (EVG_EBADSHAPE
+ * where they start at the same address).
  * Where the reference's rope takes ready cos/sin tables, full heads and the half
  * layout (ops/level1/rope/forward_ref.py:28-47).
  */
