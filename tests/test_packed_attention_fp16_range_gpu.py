@@ -95,3 +95,37 @@ def test_gradients_of_zero():
     assert not any(bool(t.any()) for t in grads(q, k, v, torch.zeros_like(do), cu))
     dq, dk, dv = grads(q, k, torch.zeros_like(v), do, cu)
     assert not bool(dq.any()) and not bool(dk.any()) and bool(dv.any())
+
+
+def test_captured_and_replayed_with_gradients_of_other_sizes():
+    """The largest elements are found again in every replay: small gradients after large ones
+    have the bits of an eager call (dq up to the order of float32 sums)."""
+    from evograd_b200 import ops
+
+    q, k, v, do, cu = make([700, 130], 2, 4, 2, 64, "fp16", seed=8)
+    base = do.clone()
+
+    def step():
+        plan = ops.packed_plan(cu, q.shape[0])
+        o, lse = ops.packed_attention_fwd(q, k, v, plan)
+        return ops.packed_attention_bwd(do, q, k, v, o, lse, plan)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for power in (0, 9, -12, -3):
+        do.copy_((base.float() * 2.0 ** power).half())
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert torch.equal(out[1], eager[1]) and torch.equal(out[2], eager[2])
+        # six key tiles' sums in another order: a few float32 roundings of numbers up to the
+        # largest, and one of float16 on each side
+        a, b = out[0].double(), eager[0].double()
+        assert bool(((a - b).abs() <= 2 * U * b.abs() + 2.0 ** -24 + 2.0 ** -20 * b.abs().max()).all())
+        assert_close(out, reference(q, k, v, [700, 130], do)[2])
