@@ -17,6 +17,7 @@
 // same two-stage atomic-free column reduction as the other norm kernels.
 #include "norm_reduce.cuh"
 #include "rowcfg.cuh"
+#include "shared_memory.cuh"
 #include "sm100_umma.cuh"
 
 namespace evg {
@@ -140,7 +141,7 @@ int launch_add_rms_fwd(const void* x, const void* r, const void* w, void* y, flo
   if (cfg.G == g && cfg.VPT == v && smem <= (size_t)device_info().max_smem_optin) {         \
     auto kern = add_rms_fwd_kernel<T, g, v>;                                                \
     if (smem > 48 * 1024)                                                                   \
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);   \
+      allow_shared_memory((const void*)kern, smem);                                         \
     const int grid = persistent_grid(kern, cfg.threads, smem, rows, groups);                \
     kern<<<grid, cfg.threads, smem, stream>>>((const T*)x, (const T*)r, (const T*)w, (T*)y, \
                                               rstd, rows, (int)hidden, eps);                \
@@ -548,7 +549,7 @@ int launch_add_rms_bwd(const void* dy, const void* x, const void* r, const void*
   if (!launched && cfg.G == g && cfg.VPT == v) {                                               \
     auto kern = add_rms_bwd_kernel<T, g, v>;                                                   \
     if (smem > 48 * 1024)                                                                      \
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);      \
+      allow_shared_memory((const void*)kern, smem);                                            \
     blocks = persistent_grid(kern, cfg.threads, smem, rows, groups, cap);                      \
     kern<<<blocks, cfg.threads, smem, stream>>>((const T*)dy, (const T*)x, (const T*)r,        \
                                                 (const T*)w, rstd, (T*)dx, partial, rows,      \
@@ -575,7 +576,7 @@ int launch_add_rms_bwd(const void* dy, const void* x, const void* r, const void*
 #define EVG_RING(v)                                                                          \
   if (!launched && nvec <= (int64_t)v * kThreads) {                                          \
     auto kern = add_rms_bwd_ring_kernel<T, kThreads, v>;                                     \
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);      \
+    allow_shared_memory((const void*)kern, smem);                                            \
     blocks = persistent_grid(kern, kThreads, smem, rows, 1, cap);                            \
     kern<<<blocks, kThreads, smem, stream>>>((const T*)dy, (const T*)x, (const T*)r,         \
                                              (const T*)w, rstd, (T*)dx, partial, rows,       \

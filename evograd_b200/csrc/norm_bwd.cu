@@ -10,6 +10,7 @@
 
 #include "norm_reduce.cuh"
 #include "rowcfg.cuh"
+#include "shared_memory.cuh"
 #include "sm100_umma.cuh"
 
 namespace evg {
@@ -777,7 +778,7 @@ int launch_norm_bwd(const void* dy, const void* x, const void* w, const float* m
 #define EVG_RING(t, v)                                                                           \
   if (!launched && ring_threads == t && nvec <= (int64_t)v * t) {                                \
     auto kern = norm_bwd_ring_kernel<T, t, v, LN>;                                               \
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);          \
+    allow_shared_memory((const void*)kern, smem);                                                \
     blocks = persistent_grid(kern, t, smem, rows, 1, ring_cap);                                  \
     kern<<<blocks, t, smem, stream>>>((const T*)dy, (const T*)x, (const T*)w, mean, rstd,        \
                                       (T*)dx, partial, rows, (int)hidden, stages, wait_limit);   \
@@ -830,7 +831,7 @@ int launch_norm_bwd(const void* dy, const void* x, const void* w, const float* m
 #define EVG_TR(g, v, t)                                                                        \
   if (!launched && G == g && V == v && threads == t) {                                         \
     auto kern = norm_bwd_tile_ring_kernel<T, g, v, LN, t>;                                     \
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);        \
+    allow_shared_memory((const void*)kern, smem);                                              \
     blocks = even_rounds(persistent_grid(kern, t, smem, rows, t / g, cap), rows, t / g);       \
     kern<<<blocks, t, smem, stream>>>((const T*)dy, (const T*)x, (const T*)w, mean, rstd,      \
                                       (T*)dx, partial, rows, (int)hidden, stages, wait_limit); \
@@ -854,7 +855,7 @@ int launch_norm_bwd(const void* dy, const void* x, const void* w, const float* m
   if (!launched && cfg.G == g && cfg.VPT == v) {                                               \
     auto kern = norm_bwd_kernel<T, g, v, LN>;                                                  \
     if (smem > 48 * 1024)                                                                      \
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);      \
+      allow_shared_memory((const void*)kern, smem);                                            \
     blocks = persistent_grid(kern, cfg.threads, smem, rows, groups, cap);                      \
     kern<<<blocks, cfg.threads, smem, stream>>>((const T*)dy, (const T*)x, (const T*)w, mean,  \
                                                 rstd, (T*)dx, partial, rows, (int)hidden);     \

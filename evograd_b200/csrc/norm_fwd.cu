@@ -4,6 +4,7 @@
 // of statistics per row). The row lives in registers between the reduction
 // passes, so x is read from memory exactly once.
 #include "rowcfg.cuh"
+#include "shared_memory.cuh"
 
 namespace evg {
 namespace {
@@ -211,7 +212,7 @@ int launch_norm_fwd(const void* x, const void* w, const void* b, void* y, float*
   if (cfg.G == g && cfg.VPT == v && smem <= (size_t)device_info().max_smem_optin) {           \
     auto kern = norm_fwd_kernel<T, g, v, LN, (kCanPack && g >= 512)>;                         \
     if (smem > 48 * 1024)                                                                     \
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);     \
+      allow_shared_memory((const void*)kern, smem);                                           \
     const int grid = persistent_grid(kern, cfg.threads, smem, rows, groups);                  \
     kern<<<grid, cfg.threads, smem, stream>>>((const T*)x, (const T*)w, (const T*)b, (T*)y,   \
                                               mean, rstd, rows, (int)hidden, eps);            \

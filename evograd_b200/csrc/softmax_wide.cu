@@ -16,6 +16,7 @@
 #include <cooperative_groups.h>
 
 #include "evg_common.cuh"
+#include "shared_memory.cuh"
 #include "sm100_umma.cuh"
 #include "softmax_wide.cuh"
 
@@ -220,11 +221,7 @@ int launch_wide_threads(const void* a, const void* b, void* out, int64_t rows, i
   if (smem > (size_t)device_info().max_smem_optin) return EVG_OK;
 
   auto kern = softmax_wide_kernel<T, BWD, kWideThreads>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-      cudaSuccess) {
-    cudaGetLastError();
-    return EVG_OK;
-  }
+  if (!allow_shared_memory((const void*)kern, smem)) return EVG_OK;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

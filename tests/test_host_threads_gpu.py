@@ -78,3 +78,36 @@ def test_packed_attention_of_two_head_sizes():
     for got, ref in zip(together(calls, 300), want):
         for a, b in zip(got, ref):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("op,widths", [("layernorm", (4096, 8192)), ("rmsnorm", (4096, 6144)), ("fused_add", (2048, 4096)),
+                                       ("softmax", (32768, 128256))])
+def test_row_operators_of_two_widths(op, widths):
+    from evograd_b200 import ops
+
+    def call(C):
+        g = torch.Generator(device="cuda").manual_seed(C)
+        x, r, dy = (torch.randn(300, C, device="cuda", generator=g).bfloat16() for _ in range(3))
+        w, b = (torch.randn(C, device="cuda", generator=g).bfloat16() for _ in range(2))
+
+        def run():
+            if op == "layernorm":
+                y, mean, rstd = ops.layernorm_fwd(x, w, b)
+                return [y, *ops.layernorm_bwd(dy, x, w, mean, rstd)]
+            if op == "rmsnorm":
+                y, rstd = ops.rmsnorm_fwd(x, w)
+                return [y, *ops.rmsnorm_bwd(dy, x, w, rstd)]
+            if op == "fused_add":
+                y, rstd = ops.fused_add_rmsnorm_fwd(x, r, w)
+                out = ops.fused_add_rmsnorm_bwd(dy, x, r, w, rstd)
+                return [y, *out]
+            y = ops.softmax_fwd(x)
+            return [y, ops.softmax_bwd(y, dy)]
+        return run
+
+    calls = [call(C) for C in widths]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    for got, ref in zip(together(calls, 100), want):
+        for a, b in zip(got, ref):
+            assert torch.equal(a, b)
