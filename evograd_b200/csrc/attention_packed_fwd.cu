@@ -32,7 +32,8 @@
 // packing, TMEM store: 1700-1900 cycles for the two warps of a scheduler, the special-
 // function unit busy for 1024 of them) and, in long runs, the power limit. Forming a
 // quarter or a third of the exponentials by a polynomial on the FMA pipe was 5-7 %
-// slower. 12001 + 2500 + 1000 + 883 tokens, 32/8 heads of 128: 1068 us, 1166 TFLOP/s.
+// slower. 12001 + 2500 + 1000 + 883 tokens, 32/8 heads of 128: 1121 us after a pause (1111
+// TFLOP/s), 1155 to 1193 in a long run.
 #include "packed.cuh"
 
 namespace evg {
@@ -452,6 +453,9 @@ int launch_fwd(const View& q, const View& k, const View& v, const View& o, float
   //   2048 307 | 300, 16384 1912 | 1720
   //   128, odd group (9/3), where the second tile is the sequence's next: 64 28 | 46,
   //   512 50 | 58, 2048 107 | 109, 4096 190 | 187, 16384 706 | 651
+  // The lengths stay on the device, so the rule goes by the mean over the offsets' entries: empty
+  // entries, unused rows and short neighbours count, and one long document among many short ones
+  // gets what is best for those (by this table up to 11 % slower for it).
   const int64_t two_from = p.pair_heads ? 256 : 4096;  // tokens per sequence
   const int tiles = D <= 64 || tokens < two_from * sequences ? 1 : 2;
   p.units = (int)(tiles == 2 && p.pair_heads ? Hq / 2 : Hq);

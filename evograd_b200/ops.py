@@ -704,8 +704,8 @@ def packed_attention_fwd(q, k, v, plan: PackedPlan, scale: float | None = None, 
     are), each token attending to its own sequence's tokens up to itself. Returns
     ``(o, lse)`` with o like q and ``lse`` float32 ``[Hq, T]``; rows behind the last
     sequence are 0 and ``-inf``. float16 / bfloat16 with D a multiple of 8 up to 128 run on
-    the tensor cores, float32 and other D <= 256 on plain kernels. ``out`` receives o
-    (it must not overlap an input)."""
+    the tensor cores, float32 and other D <= 256 on plain kernels for small shapes. ``out``
+    receives o (it must not overlap an input; off a 16-byte boundary the plain kernels run)."""
     dev = _require_cuda(q, k, v)
     T, Hq, Hkv, D = _check_packed(q, k, v, plan, dev)
     en = _dtype_enum(q)
@@ -727,7 +727,8 @@ def packed_attention_bwd(do, q, k, v, o, lse, plan: PackedPlan, scale: float | N
     """Returns ``(dq, dk, dv)`` of :func:`packed_attention_fwd`; dk / dv are summed over the
     query heads of each group, rows behind the last sequence are zero. ``outs`` supplies the
     three output tensors, which may be strided views (the thirds of one projection's
-    gradient) but overlap neither an input nor one another. dq of the tensor-core path can
+    gradient; off a 16-byte boundary the plain kernels run) but overlap neither an input nor
+    one another. float16 gradients may be of any size that their type holds. dq of the tensor-core path can
     differ in the last bit from run to run (float32 global adds)."""
     dev = _require_cuda(do, q, k, v, o, lse)
     T, Hq, Hkv, D = _check_packed(q, k, v, plan, dev)

@@ -403,10 +403,14 @@ typedef struct evg_packed_view {
  * sequence, lse [Hq, tokens] float32 the log-sum-exp (natural log) of the scaled
  * scores. q, o: Hq heads; k, v: Hkv heads (Hq % Hkv == 0). Rows behind the last
  * sequence get o = 0 and lse = -inf; what q, k, v hold there reaches nothing, and
- * neither does one sequence's content (infinities and NaN included) another's.
+ * neither does one sequence's content (infinities and NaN included) another's. Inside
+ * a sequence, a token whose v (or, backward, do . v) is infinite or NaN can make NaN of
+ * earlier rows of its own 128-row tile: the tensor cores multiply what the mask drops by
+ * zero.
  * 16-bit tensors with D a multiple of 8 up to 128 and 16-byte aligned views
  * (pointers, strides in multiples of 8 elements) run on the tensor cores;
- * everything else (float32, D <= 256) on plain CUDA-core kernels. Views are HOST
+ * everything else (float32, other D <= 256, views off those boundaries) on plain
+ * CUDA-core kernels, which are for small shapes. Views are HOST
  * structs, read before the call returns. `plan` must have been made for the same
  * `tokens` and `sequences`. Outputs, here and in the backward, overlap neither an
  * input nor one another (EVG_EBADSHAPE where they start at the same address).
