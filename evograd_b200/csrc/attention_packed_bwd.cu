@@ -54,15 +54,18 @@
 // (a 64-row product has another layout in tensor memory).
 //
 // float16 has five bits of exponent, so its P and dS go into the products scaled by powers of
-// two, which come out of the results again: P by 4 (a shift of the log-sum-exp), dS by 4 G with
-//   4 G 2 HD max|do| max|v| <= 2^15,  G max|v| <= 2^15   (largest elements of a sequence and
-// k/v head), so that neither |dS_ij| <= P_ij (|do_i . v_j| + |delta_i|) nor V G overflows. G is
-// applied to V on its way into tensor memory and to delta in the subtraction, so the walk over
-// the tiles has no instruction more for it. (V G is rounded again only below 2^-14: by 2^-25,
-// 2^-13 of the largest |V| G at worst, where |do| reaches 65504.) Gradients of any size keep the
-// bits that gradients of size one have: unscaled, do of 2^-14 over 16000 tokens gave later rows of
-// dq and dk errors of 21 % (their own rounding to float16: 1.8 %), and dS above 65504 infinities.
-// The largest elements cost a read of V and a memset before: 4 x 4096 tokens, 32/8 heads of 128,
+// two, which come out of the results again: P by 64 (a shift of the log-sum-exp), dS by 64 G with
+//   64 G 2 max|do_i| max|v_j| <= 2^15,  G max|v| <= 2^15   (over a sequence and k/v head)
+// so that neither |dS_ij| <= P_ij (|do_i . v_j| + |delta_i|) nor V G overflows. The norms are bounded
+// by the largest sum of squares of eight neighbouring elements. G is applied to V on its way into
+// tensor memory and to delta in the subtraction, so the walk over the tiles has no instruction more
+// for it. (V G is rounded again only below 2^-14, by 2^-25: at worst 2^-13 of the largest |V| G
+// where |do| reaches 4096, 2^-9 where it reaches 65504.) Gradients of any size keep the bits that
+// gradients of size one have: unscaled, do of 2^-14 over 16000 tokens gave later rows of dq and dk
+// errors of 21 % (their own rounding to float16: 1.8 %), and dS above 65504 infinities. P's factor
+// is for long rows that rest on one key: 4100 others of weight 2^-21, dv off by 1.2 % without it,
+// by 0.06 % with it (a larger one would leave V G less).
+// The sums of squares cost a read of V and a memset before: 4 x 4096 tokens, 32/8 heads of 128,
 // under 2 %; 128 x 128 tokens 242 us against bfloat16's 218; 16/16 heads of 64, 4096 tokens in
 // four sequences, forward and backward, 121 -> 125 us.
 //
@@ -118,20 +121,21 @@ __device__ __forceinline__ int64_t acc_tile(const BwdParams& p, int head, int se
   return (int64_t)head * (p.tokens / kTile) + seq0 / kTile + t - 1;
 }
 // float16: exponent of P's scale, and that of G for a sequence (by its first padded tile) and a
-// k/v head, from the largest |do| and |v| as float16 bits (infinities and NaN as 65504: their
-// sequence's gradients are not finite whatever the scale).
-constexpr int kPExponent = 2;
+// k/v head.
+constexpr int kPExponent = 6;
 struct DsRange {
-  uint32_t most_do, most_v;
+  float most_do, most_v;  // largest sum of squares of eight neighbouring elements
   __device__ __forceinline__ void load(const BwdParams& p, int tile0, int head_kv) {
     const uint32_t* at = p.range + (int64_t)head_kv * p.seq_tiles + tile0;
-    most_do = at[0];
-    most_v = at[(int64_t)p.units * p.seq_tiles];
+    most_do = __uint_as_float(at[0]);
+    most_v = __uint_as_float(at[(int64_t)p.units * p.seq_tiles]);
   }
+  // sqrt(x) < 2^half(x)
+  static __device__ __forceinline__ int half(float x) { return ((int)(__float_as_uint(x) >> 23) - 127 + 2) >> 1; }
+  // |do_i . v_j| <= HD / 8 sqrt(most_do most_v), and no element of v is above sqrt(most_v).
   template <int HD> __device__ __forceinline__ int exponent() const {
-    // below 2^(k + 1); k = -15 for subnormal ones
-    const int k_do = min((int)(most_do >> 10), 30) - 15, k_v = min((int)(most_v >> 10), 30) - 15;
-    return min(15 - (kPExponent + 1) - (HD == 128 ? 7 : 6) - (k_do + 1) - (k_v + 1), 15 - (k_v + 1));  // -27 .. 29
+    const int for_ds = 15 - (kPExponent + 1) - (HD == 128 ? 4 : 3) - half(most_do * most_v);
+    return min(min(for_ds, 15 - half(most_v)), 29);  // -31 .. 29
   }
 };
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
@@ -742,16 +746,15 @@ template <int FMT> __device__ __forceinline__ float dot8(const uint4& a, const u
   return s;
 }
 
-// Maxima of m's and the vector's float16 without their signs (NaN left out), as two halves.
-__device__ __forceinline__ uint32_t most_of(uint32_t m, const uint4& v) {
-  const __half2* x = reinterpret_cast<const __half2*>(&v);
-  __half2 a = __hmax2(__habs2(x[0]), __habs2(x[1])), b = __hmax2(__habs2(x[2]), __habs2(x[3]));
-  a = __hmax2(__hmax2(a, b), *reinterpret_cast<const __half2*>(&m));
-  return *reinterpret_cast<const uint32_t*>(&a);
+// The larger of m and x >= 0 as float bits; infinities and NaN (their rows' gradients are not
+// finite whatever the scale) do not count.
+__device__ __forceinline__ uint32_t finite_max(uint32_t m, float x) {
+  const uint32_t b = __float_as_uint(x);
+  return b < 0x7f800000u && b > m ? b : m;
 }
-// *at = max(*at, both halves of every lane's m).
+// *at = max(*at, every lane's m).
 __device__ __forceinline__ void raise(uint32_t* at, uint32_t m) {
-  m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+  m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0 && m) atomicMax(at, m);
 }
 
@@ -824,7 +827,7 @@ packed_prepare_kernel(const View dout, const View q, const View o, const float* 
   const int tile0 = (item.z - 1) * kTile;
   const int64_t prow0 = (int64_t)head * p.slots * kTile + (int64_t)item.w * kTile + tile0;
   const bool takes_v = FMT == 0 && head % p.group == 0;
-  uint32_t most_do = 0, most_v = 0;  // two float16 each, signs off: ordered as the numbers
+  uint32_t most_do = 0, most_v = 0;  // float bits: ordered as the numbers
 #pragma unroll 1
   for (int r = threadIdx.x / TPR + blockIdx.z * ROWS; r < kTile; r += ROWS * gridDim.z) {
     const bool ok = tile0 + r < item.y, mine = ok && part * 8 < p.D;
@@ -841,8 +844,8 @@ packed_prepare_kernel(const View dout, const View q, const View o, const float* 
 #pragma unroll
     for (int off = TPR / 2; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
     if constexpr (FMT == 0) {
-      most_do = most_of(most_do, g);
-      if (takes_v) most_v = most_of(most_v, vv);
+      most_do = finite_max(most_do, dot8<FMT>(g, g));
+      if (takes_v) most_v = finite_max(most_v, dot8<FMT>(vv, vv));
     }
     if (item.z > 1) {
       uint4* acc = reinterpret_cast<uint4*>(p.dq_acc + (acc_tile(p, head, item.x, item.z - 1) * kTile + r) * HD + part * 8);

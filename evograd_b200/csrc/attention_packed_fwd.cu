@@ -83,6 +83,14 @@ __device__ __forceinline__ void clear_rows(const FwdParams& p, int row0, int row
     p.lse[(int64_t)head * p.tokens + row0 + r] = -INFINITY;
 }
 
+// P and its sum carry a factor 2^p_exponent, which the division by the sum takes out again. float16
+// reaches down to 2^-14 with all its bits: where one key has nearly all of a row's weight (a first
+// token, say), the others' probabilities can lie below that although they are the result (4100
+// keys of 2^-21 each beside one whose value is zero: o off by 1.2 %, 0.035 % with the factor). P is
+// at most 2^kRescaleThreshold times it.
+template <int FMT> __host__ __device__ constexpr float p_exponent() { return FMT == 0 ? 7.f : 0.f; }
+static_assert(kRescaleThreshold + 7.f <= 15.f, "P stays below 65504");
+
 template <int HD, int FMT, int TILES>
 __global__ void __launch_bounds__(fwd_threads(TILES), 3 - TILES)
 attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
@@ -272,6 +280,7 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
     const int n_mine = wg ? n_half[1] : n_half[0];
     const uint32_t tOw = tmem + TILES * 128 + wg * 128;
     const float scale_log2 = p.scale_log2;
+    constexpr float kPExponent = p_exponent<FMT>();
     float m_run = -INFINITY, l_run = 0.f;
     for (int g = 0; g < n_mine; ++g) {
       const int hf = g & 1;
@@ -325,7 +334,7 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
       // Probabilities: 64 score columns -> 32 packed columns over them. P is rounded to 16
       // bits as the tensor cores' operand; its sum is taken before rounding. A masked score
       // of -infinity gives zero, also while a row has seen nothing else (m_run is -infinity).
-      const f32x2 neg_m2 = f2_splat(m_run == -INFINITY ? 0.f : -m_run), scale2 = f2_splat(scale_log2);
+      const f32x2 neg_m2 = f2_splat(kPExponent - (m_run == -INFINITY ? 0.f : m_run)), scale2 = f2_splat(scale_log2);
       f32x2 ls2[2] = {0ull, 0ull};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -379,7 +388,7 @@ attn_packed_fwd_kernel(const __grid_constant__ CUtensorMap map_q,
       }
       const bool row_ok = q_pos < L;
       const int64_t token = seq0 + (row_ok ? q_pos : 0);
-      if (row_ok) p.lse[(int64_t)my_head * p.tokens + token] = (m_run + log2f(l_run)) * kLn2;
+      if (row_ok) p.lse[(int64_t)my_head * p.tokens + token] = (m_run + (log2f(l_run) - kPExponent)) * kLn2;
       named_barrier_sync(1 + wg, 128);
       uint8_t* out = reinterpret_cast<uint8_t*>(p.o) +
                      ((int64_t)(seq0 + my_tile * kTile) * p.o_st + (int64_t)my_head * p.o_sh) * 2;

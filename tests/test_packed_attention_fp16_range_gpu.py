@@ -98,7 +98,7 @@ def test_gradients_of_zero():
 
 
 def test_captured_and_replayed_with_gradients_of_other_sizes():
-    """The largest elements are found again in every replay: small gradients after large ones
+    """The norms that set the scale are found again in every replay: small gradients after large ones
     have the bits of an eager call (dq up to the order of float32 sums)."""
     from evograd_b200 import ops
 
